@@ -141,6 +141,9 @@ SIGNATURES = {
     "bmv_bn_chunks": [c_i, c_l],
     "bmv_bn_train_fwd": [c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_l, c_fl, c_fl, c_fl, c_f, c_f, c_f, c_f, c_f],
     "bmv_bn_train_bwd": [c_f, c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_l, c_fl, c_f, c_f, c_f, c_f, c_f],
+    "bmv_group_norm_workspace": [c_i, c_i, c_l, c_i, c_i, c_i, c_i],
+    "bmv_group_norm_fwd": [c_f, c_f, c_f, c_i, c_i, c_l, c_i, c_i, c_i, c_i, C.c_double, c_i, c_fl, c_f, c_f, c_f, c_f, c_f],
+    "bmv_group_norm_bwd": [c_f, c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_l, c_i, c_i, c_i, c_i, c_i, c_fl, c_f, c_f, c_f, c_f, c_f],
     "bmv_conv_top_fwd": [c_f, c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_i, c_fl, c_i, c_f],
     "bmv_conv0_fused_fwd": [c_f, c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_i, c_i, c_fl, c_fl, c_f],
     "bmv_conv_heads_fwd": [c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_i, c_i, c_i, c_f],
@@ -195,6 +198,7 @@ def load():
     lib.bmv_mvs_mlp_train_act_floats.restype = C.c_long
     lib.bmv_mvs_mlp_train_scratch_floats.restype = C.c_long
     lib.bmv_conv_wgrad_workspace.restype = C.c_long
+    lib.bmv_group_norm_workspace.restype = C.c_long
     lib.bmv_last_error.argtypes = []
     lib.bmv_last_error.restype = C.c_char_p
     lib.bmv_tuning_name.restype = C.c_char_p

@@ -224,6 +224,27 @@ class BatchNormTrain(torch.autograd.Function):
         return dx, dw, db, None, None, None, None, None
 
 
+class GroupNormAct(torch.autograd.Function):
+    """Group norm with an activation (`relu`: False, True, a leaky slope, "silu") on csrc/group_norm.hip: what stands in for
+    BatchNormTrain where a step sees one image.  fp32 / bf16 / fp16, channel-last or planar; no double backward."""
+
+    @staticmethod
+    def forward(ctx, x, groups, weight, bias, eps=1e-5, relu=False):
+        y, mean, rstd = ops.group_norm_fwd(x, groups, weight, bias, eps, relu)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        ctx.cfg = (groups, relu)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        groups, relu = ctx.cfg
+        _, _, want_w, want_b, _, _ = ctx.needs_input_grad
+        dx, dw, db = ops.group_norm_bwd(x, dy, groups, weight, bias, mean, rstd, relu, want_params=want_w or want_b)
+        return dx, None, dw if want_w else None, db if want_b else None, None, None
+
+
 class MvsSweep(torch.autograd.Function):
     """a19 + a20 (MVSNeRF's padded sweep): gradient to the source features through the masked-variance channels."""
 

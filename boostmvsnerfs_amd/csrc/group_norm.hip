@@ -1,0 +1,762 @@
+// Group normalisation with an activation, forward and backward, on channel-last and planar maps: what stands in for
+// csrc/bn.hip where a step sees one image (batch statistics of one image are that image's own, differ between training and
+// inference and have to be exchanged between ranks; a group's statistics are per sample and none of that).
+//
+//   mean, var over the M = C / G * S values of a (sample, group);  z = (x - mean) rstd w_c + b_c;  y = act(z)
+//   g = dy act'(z);  db_c = sum g;  dw_c = sum g xhat;  dx = rstd (g w - (sum_g g w + xhat sum_g g w xhat) / M)
+//   act(v) = v > 0 ? v : slope v (1 none, 0 ReLU, 0.01 leaky ReLU), or v / (1 + exp(-v)) (SiLU)
+//
+// Numbers.  Sums are 64-bit (mean and variance as sum x and sum x^2: x^2 of a 32-bit x is exact in 64 bits, so the difference
+// loses 1e-16 (mean / std)^2 and no pivot is needed).  That is not only for long sums: act' of the ReLUs jumps at z = 0, so
+// the backward has to decide the sign of z as the exact value has it.  It computes z in 32 bits and, where |z| is within
+// 2^-18 of its terms (a few values in a million), again in 64 with the saved 64-bit statistics.  x - mean is taken as
+// (x - mh) - ml with mean = mh + ml, so a large common offset costs no accuracy.
+//
+// What bounds it: bytes.  Two launches each way: sums of a chunk per workgroup -> partials; then every workgroup joins the
+// partials of the groups it touches (always in the same order: bit-reproducible, no atomics) and writes its chunk, which it
+// finds in its XCD's L2 or the last-level cache because the chunk -> workgroup map of both launches is the same.
+#include "bmv_common.hpp"
+
+namespace bmv {
+
+constexpr int kGnThreads = 256, kGnWaves = kGnThreads / 64;
+
+template <int DT> struct GnType;
+template <> struct GnType<0> { using T = float; };
+template <> struct GnType<1> { using T = __bf16; };
+template <> struct GnType<2> { using T = _Float16; };
+
+// V values of T, loaded and stored as one access of V * sizeof(T) <= 16 bytes
+template <typename T, int V>
+struct alignas(sizeof(T) * V) GnVec {
+  T v[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ GnVec<T, V> gn_load(const T* p) {
+  return *reinterpret_cast<const GnVec<T, V>*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void gn_store(T* p, const float* f) {
+  GnVec<T, V> o;
+#pragma unroll
+  for (int j = 0; j < V; ++j) o.v[j] = (T)f[j];      // to nearest even: the one rounding of a result
+  *reinterpret_cast<GnVec<T, V>*>(p) = o;
+}
+
+// affine parameters: 32 bits (wdt 0) or the map's type
+template <typename T>
+__device__ __forceinline__ float gn_param(const void* p, int c, int wdt, float dflt) {
+  if (!p) return dflt;
+  return wdt == 0 ? static_cast<const float*>(p)[c] : (float)static_cast<const T*>(p)[c];
+}
+
+struct GnArgs {
+  const void *x, *dy, *w, *b;
+  void *out, *dw, *db;           // y / dx; dw, db (backward)
+  double *mean, *rstd;           // (N, G): written by the forward, read by the backward
+  double2* part;                 // [N * G][pieces]: (sum, sum of squares) / (sum g w, sum g w xhat)
+  double2* partc;                // backward: per channel and piece (sum g, sum g xhat), element n * pcn + k * pck + c * pcc
+  long S, M;
+  long pcn, pck, pcc;
+  int N, C, G, cg, wdt;
+  int chunks, slabs, width;      // channel-last: row chunks, channel slabs of `width` channels.  planar: chunks of a plane
+  int pieces, npc;               // pieces a (sample, group) is joined from; pieces per channel of partc
+  int slab_pieces;               // channel-last: slabs that share a group (1 where slabs hold whole groups)
+  int dwb;                       // backward: workgroups behind the map's that finish dw and db
+  float slope;
+  double eps;
+};
+
+__device__ __forceinline__ double gn_wave_sum(double v) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  return v;
+}
+
+// sum of the pieces of one (sample, group), by one wave, every lane gets it
+__device__ __forceinline__ double2 gn_join(const double2* __restrict__ p, int pieces) {
+  double a = 0., b = 0.;
+  for (int k = threadIdx.x & 63; k < pieces; k += 64) a += p[k].x, b += p[k].y;
+  return {gn_wave_sum(a), gn_wave_sum(b)};
+}
+
+struct GnStat {
+  double mean, rstd;
+};
+__device__ __forceinline__ GnStat gn_stat(double2 s, double M, double eps) {
+  const double mean = s.x / M, var = s.y / M - mean * mean;
+  return {mean, 1. / sqrt((var > 0. || var != var ? var : 0.) + eps)};
+}
+
+// z > 0 as the exact z has it (see above)
+__device__ __forceinline__ bool gn_positive(float z, float dsc, float b, float x, double mean, double rstd, float w) {
+  if (fabsf(z) > 0x1p-18f * (fabsf(dsc) + fabsf(b))) return z > 0.f;
+  return ((double)x - mean) * (rstd * (double)w) + (double)b > 0.;
+}
+
+template <bool SILU>
+__device__ __forceinline__ float gn_act(float z, float slope) {
+  if (SILU) return z / (1.f + __expf(-z));
+  return z > 0.f ? z : (slope == 0.f ? (z != z ? z : 0.f) : slope * z);   // (0 * -inf would be NaN)
+}
+
+// g = dy act'(z)
+template <bool SILU>
+__device__ __forceinline__ float gn_grad(float dy, float x, float d, float sc, float b, float w, float slope, double mean,
+                                         double rstd) {
+  const float dsc = d * sc, z = dsc + b;
+  if (SILU) {
+    const float s = 1.f / (1.f + __expf(-z));
+    return dy * s * (1.f + z * (1.f - s));
+  }
+  if (slope == 1.f) return dy;
+  return gn_positive(z, dsc, b, x, mean, rstd, w) ? dy : (slope == 0.f ? 0.f : slope * dy);
+}
+
+// ---- channel-last ----------------------------------------------------------------------------------------------------
+// Workgroup = (sample, channel slab, row chunk); thread = V consecutive channels (one 16-byte access where C allows) of
+// every `rpi`-th row, so a thread's channels never change.  Lanes run over the slab's channels first: accesses are coalesced
+// whatever C is.  ONE: V channels always lie in one group (C / G a multiple of V): one pair of sums instead of V.
+struct GnCl {
+  int n, slab, k, c0, nch, wv, cv, r0, rpi, c;
+  long begin, end;
+  bool on;
+};
+template <int V>
+__device__ __forceinline__ GnCl gn_cl(const GnArgs& a, int bid) {
+  GnCl t;
+  t.k = bid % a.chunks;
+  bid /= a.chunks;
+  t.slab = bid % a.slabs, t.n = bid / a.slabs;
+  t.c0 = t.slab * a.width, t.nch = min(a.width, a.C - t.c0);
+  t.wv = t.nch / V, t.rpi = kGnThreads / t.wv;
+  t.r0 = threadIdx.x / t.wv, t.cv = threadIdx.x - t.r0 * t.wv;
+  t.on = t.r0 < t.rpi, t.c = t.c0 + t.cv * V;
+  const long per = (a.S + a.chunks - 1) / a.chunks;
+  t.begin = min((long)t.k * per, a.S), t.end = min(t.begin + per, a.S);
+  return t;
+}
+
+// The workgroup's sums of E values per thread (E = 1: the thread's V channels together; V: each) -> a piece of every group
+// of the slab.  sh: kGnThreads * E double2.
+template <int V, int E>
+__device__ __forceinline__ void gn_cl_pieces(const GnArgs& a, const GnCl& t, double2* sh, bool groups) {
+  const int ne = t.wv * E;                          // entries of a row of the table
+  __syncthreads();
+  int half = 1;
+  while (half < t.rpi) half <<= 1;
+  for (half >>= 1; half >= 1; half >>= 1) {          // rows r0 + half onto r0
+    for (int i = threadIdx.x; i < half * ne; i += kGnThreads)
+      if (i + half * ne < t.rpi * ne) sh[i].x += sh[i + half * ne].x, sh[i].y += sh[i + half * ne].y;
+    __syncthreads();
+  }
+  if (!groups) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g0 = t.c0 / a.cg, g1 = (t.c0 + t.nch - 1) / a.cg;
+  for (int g = g0 + wave; g <= g1; g += kGnWaves) {
+    const int lo = max(g * a.cg, t.c0) - t.c0, hi = min((g + 1) * a.cg, t.c0 + t.nch) - t.c0;   // channels of the slab
+    const int step = V / E;
+    double x = 0., y = 0.;
+    for (int i = lo / step + lane; i < hi / step; i += 64) x += sh[i].x, y += sh[i].y;
+    x = gn_wave_sum(x), y = gn_wave_sum(y);
+    if (lane == 0) {
+      const int first = g * a.cg / a.width;          // the group's first slab
+      a.part[((long)t.n * a.G + g) * a.pieces + (t.slab - first) * a.chunks + t.k] = {x, y};
+    }
+  }
+  // (a group that fewer slabs share than others: its missing pieces are zero)
+  for (int g = g0 + (int)threadIdx.x; g <= g1; g += kGnThreads) {
+    const int first = g * a.cg / a.width, last = ((g + 1) * a.cg - 1) / a.width;
+    if (t.slab == last)
+      for (int s = last - first + 1; s < a.slab_pieces; ++s)
+        a.part[((long)t.n * a.G + g) * a.pieces + s * a.chunks + t.k] = {0., 0.};
+  }
+}
+
+template <int DT, int V, bool ONE>
+__global__ void __launch_bounds__(kGnThreads) gn_cl_stats_kernel(GnArgs a) {
+  using T = typename GnType<DT>::T;
+  constexpr int E = ONE ? 1 : V;
+  __shared__ double2 sh[kGnThreads * E];
+  const GnCl t = gn_cl<V>(a, blockIdx.x);
+  if (t.on) {
+    double s[E], q[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e] = q[e] = 0.;
+    const T* p = static_cast<const T*>(a.x) + (long)t.n * a.S * a.C + t.c;
+    constexpr int U = 4;
+    long r = t.begin + t.r0;
+    for (; r + (U - 1) * t.rpi < t.end; r += U * t.rpi) {
+      GnVec<T, V> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = gn_load<T, V>(p + (r + u * t.rpi) * a.C);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const double f = (double)(float)v[u].v[j];
+          s[ONE ? 0 : j] += f, q[ONE ? 0 : j] += f * f;
+        }
+    }
+    for (; r < t.end; r += t.rpi) {
+      const GnVec<T, V> v = gn_load<T, V>(p + r * a.C);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const double f = (double)(float)v.v[j];
+        s[ONE ? 0 : j] += f, q[ONE ? 0 : j] += f * f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sh[threadIdx.x * E + e] = {s[e], q[e]};
+  }
+  gn_cl_pieces<V, E>(a, t, sh, true);
+}
+
+// one piece per (sample, group) out of many: in front of the apply launch where its workgroups would join too many
+__global__ void __launch_bounds__(kGnThreads) gn_finish_kernel(const double2* __restrict__ part, int pieces, long n,
+                                                               double2* __restrict__ out) {
+  const long i = (long)blockIdx.x * kGnWaves + (threadIdx.x >> 6);
+  if (i >= n) return;
+  const double2 s = gn_join(part + i * pieces, pieces);
+  if ((threadIdx.x & 63) == 0) out[i] = s;
+}
+
+template <int DT, int V, bool SILU>
+__global__ void __launch_bounds__(kGnThreads) gn_cl_apply_kernel(GnArgs a) {
+  using T = typename GnType<DT>::T;
+  extern __shared__ GnStat st[];                     // the slab's groups
+  const GnCl t = gn_cl<V>(a, blockIdx.x);
+  const int g0 = t.c0 / a.cg, g1 = (t.c0 + t.nch - 1) / a.cg;
+  for (int g = g0 + (threadIdx.x >> 6); g <= g1; g += kGnWaves) {
+    const long i = (long)t.n * a.G + g;
+    const GnStat s = gn_stat(gn_join(a.part + i * a.pieces, a.pieces), (double)a.M, a.eps);
+    if ((threadIdx.x & 63) == 0) {
+      st[g - g0] = s;
+      if (t.k == 0) a.mean[i] = s.mean, a.rstd[i] = s.rstd;     // (slabs that share a group write the same value)
+    }
+  }
+  __syncthreads();
+  if (!t.on) return;
+  float mh[V], ml[V], sc[V], b[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const GnStat s = st[(t.c + j) / a.cg - g0];
+    mh[j] = (float)s.mean, ml[j] = (float)(s.mean - (double)mh[j]);
+    sc[j] = (float)(s.rstd * (double)gn_param<T>(a.w, t.c + j, a.wdt, 1.f)), b[j] = gn_param<T>(a.b, t.c + j, a.wdt, 0.f);
+  }
+  const long off = (long)t.n * a.S * a.C + t.c;
+  const T* p = static_cast<const T*>(a.x) + off;
+  T* o = static_cast<T*>(a.out) + off;
+  constexpr int U = 4;
+  long r = t.begin + t.r0;
+  for (; r + (U - 1) * t.rpi < t.end; r += U * t.rpi) {
+    GnVec<T, V> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = gn_load<T, V>(p + (r + u * t.rpi) * a.C);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = gn_act<SILU>((((float)v[u].v[j] - mh[j]) - ml[j]) * sc[j] + b[j], a.slope);
+      gn_store<T, V>(o + (r + u * t.rpi) * a.C, f);
+    }
+  }
+  for (; r < t.end; r += t.rpi) {
+    const GnVec<T, V> v = gn_load<T, V>(p + r * a.C);
+    float f[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = gn_act<SILU>((((float)v.v[j] - mh[j]) - ml[j]) * sc[j] + b[j], a.slope);
+    gn_store<T, V>(o + r * a.C, f);
+  }
+}
+
+template <int DT, int V, bool SILU>
+__global__ void __launch_bounds__(kGnThreads) gn_cl_bwd_reduce_kernel(GnArgs a) {
+  using T = typename GnType<DT>::T;
+  __shared__ double2 sh[kGnThreads * V];
+  const GnCl t = gn_cl<V>(a, blockIdx.x);
+  if (t.on) {
+    float mh[V], ml[V], sc[V], b[V], w[V];
+    double mean[V], rstd[V], s[V], q[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const long i = (long)t.n * a.G + (t.c + j) / a.cg;
+      mean[j] = a.mean[i], rstd[j] = a.rstd[i], s[j] = q[j] = 0.;
+      mh[j] = (float)mean[j], ml[j] = (float)(mean[j] - (double)mh[j]);
+      w[j] = gn_param<T>(a.w, t.c + j, a.wdt, 1.f), b[j] = gn_param<T>(a.b, t.c + j, a.wdt, 0.f);
+      sc[j] = (float)(rstd[j] * (double)w[j]);
+    }
+    const long off = (long)t.n * a.S * a.C + t.c;
+    const T *p = static_cast<const T*>(a.x) + off, *pd = static_cast<const T*>(a.dy) + off;
+    constexpr int U = 4;
+    for (long r = t.begin + t.r0; r < t.end; r += U * t.rpi) {
+      GnVec<T, V> v[U], e[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long ru = min(r + u * t.rpi, t.end - 1);      // (rows behind the chunk: read again, counted below as zero)
+        v[u] = gn_load<T, V>(p + ru * a.C), e[u] = gn_load<T, V>(pd + ru * a.C);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        // four terms in 32 bits, their sum in 64: a sum of four adds one 32-bit rounding to the terms' own
+        float fs = 0.f, fq = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float x = (float)v[u].v[j], d = (x - mh[j]) - ml[j];
+          const float g = gn_grad<SILU>((float)e[u].v[j], x, d, sc[j], b[j], w[j], a.slope, mean[j], rstd[j]);
+          if (r + u * t.rpi < t.end) fs += g, fq += g * d;
+        }
+        s[j] += (double)fs, q[j] += (double)fq;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) sh[threadIdx.x * V + j] = {s[j], q[j] * rstd[j]};
+  }
+  gn_cl_pieces<V, V>(a, t, sh, false);
+  for (int i = threadIdx.x; i < t.nch; i += kGnThreads) {
+    const double2 v = sh[i];
+    const int c = t.c0 + i;
+    if (a.partc) a.partc[t.n * a.pcn + t.k * a.pck + c * a.pcc] = v;
+    const double w = (double)gn_param<T>(a.w, c, a.wdt, 1.f);
+    sh[i] = {v.x * w, v.y * w};
+  }
+  GnCl one = t;
+  one.rpi = 1;
+  gn_cl_pieces<V, V>(a, one, sh, true);
+}
+
+// dw and db out of the pieces: 8 channels a workgroup, 32 threads each, the samples and pieces of a channel in a fixed order
+template <int DT>
+__device__ __forceinline__ void gn_param_grads(const GnArgs& a, int wg) {
+  using T = typename GnType<DT>::T;
+  __shared__ double2 sw[kGnThreads];
+  const int cl = threadIdx.x & 7, q = threadIdx.x >> 3, c = wg * 8 + cl;
+  double x = 0., y = 0.;
+  if (c < a.C)
+    for (int i = q; i < a.N * a.npc; i += 32) {
+      const int n = i / a.npc, k = i - n * a.npc;
+      const double2 v = a.partc[n * a.pcn + k * a.pck + c * a.pcc];
+      x += v.x, y += v.y;
+    }
+  sw[threadIdx.x] = {x, y};
+  __syncthreads();
+  if (q || c >= a.C) return;
+  for (int i = 1; i < 32; ++i) x += sw[i * 8 + cl].x, y += sw[i * 8 + cl].y;
+  if (a.wdt == 0) {
+    if (a.db) static_cast<float*>(a.db)[c] = (float)x;
+    if (a.dw) static_cast<float*>(a.dw)[c] = (float)y;
+  } else {
+    if (a.db) static_cast<T*>(a.db)[c] = (T)(float)x;
+    if (a.dw) static_cast<T*>(a.dw)[c] = (T)(float)y;
+  }
+}
+
+template <int DT, int V, bool SILU>
+__global__ void __launch_bounds__(kGnThreads) gn_cl_bwd_apply_kernel(GnArgs a) {
+  using T = typename GnType<DT>::T;
+  extern __shared__ double2 sg[];                    // the slab's groups: the two sums over M
+  if ((int)blockIdx.x < a.dwb) return gn_param_grads<DT>(a, blockIdx.x);
+  const GnCl t = gn_cl<V>(a, blockIdx.x - a.dwb);
+  const int g0 = t.c0 / a.cg, g1 = (t.c0 + t.nch - 1) / a.cg;
+  for (int g = g0 + (threadIdx.x >> 6); g <= g1; g += kGnWaves) {
+    const double2 s = gn_join(a.part + ((long)t.n * a.G + g) * a.pieces, a.pieces);
+    if ((threadIdx.x & 63) == 0) sg[g - g0] = {s.x / (double)a.M, s.y / (double)a.M};
+  }
+  __syncthreads();
+  if (!t.on) return;
+  // dx = rstd w g - rstd m1 - (x - mean) rstd^2 m2
+  float mh[V], ml[V], sc[V], b[V], w[V], c1[V], c2[V];
+  double mean[V], rstd[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int g = (t.c + j) / a.cg;
+    const long i = (long)t.n * a.G + g;
+    mean[j] = a.mean[i], rstd[j] = a.rstd[i];
+    mh[j] = (float)mean[j], ml[j] = (float)(mean[j] - (double)mh[j]);
+    w[j] = gn_param<T>(a.w, t.c + j, a.wdt, 1.f), b[j] = gn_param<T>(a.b, t.c + j, a.wdt, 0.f);
+    sc[j] = (float)(rstd[j] * (double)w[j]);
+    c1[j] = (float)(rstd[j] * sg[g - g0].x), c2[j] = (float)(rstd[j] * rstd[j] * sg[g - g0].y);
+  }
+  const long off = (long)t.n * a.S * a.C + t.c;
+  const T *p = static_cast<const T*>(a.x) + off, *pd = static_cast<const T*>(a.dy) + off;
+  T* o = static_cast<T*>(a.out) + off;
+  constexpr int U = 4;
+  for (long r = t.begin + t.r0; r < t.end; r += U * t.rpi) {
+    GnVec<T, V> v[U], e[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long ru = min(r + u * t.rpi, t.end - 1);
+      v[u] = gn_load<T, V>(p + ru * a.C), e[u] = gn_load<T, V>(pd + ru * a.C);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (r + u * t.rpi >= t.end) break;
+      float f[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float x = (float)v[u].v[j], d = (x - mh[j]) - ml[j];
+        const float g = gn_grad<SILU>((float)e[u].v[j], x, d, sc[j], b[j], w[j], a.slope, mean[j], rstd[j]);
+        f[j] = (sc[j] * g - c1[j]) - d * c2[j];
+      }
+      gn_store<T, V>(o + (r + u * t.rpi) * a.C, f);
+    }
+  }
+}
+
+// ---- planar ----------------------------------------------------------------------------------------------------------
+// Unit = (sample, channel, chunk of the plane), by a workgroup (TPU 256) or, where planes are short, by a wave (TPU 64);
+// V values of the plane per access.
+struct GnPl {
+  long plane, begin, end;
+  int n, c, k, t;
+  bool on;
+};
+template <int TPU>
+__device__ __forceinline__ GnPl gn_pl(const GnArgs& a, long bid) {
+  GnPl p;
+  const long unit = bid * (kGnThreads / TPU) + (TPU == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  p.on = unit < (long)a.N * a.C * a.chunks;
+  p.t = threadIdx.x & (TPU - 1);
+  p.k = (int)(unit % a.chunks), p.plane = unit / a.chunks;
+  p.c = (int)(p.plane % a.C), p.n = (int)(p.plane / a.C);
+  const long per = ((a.S + a.chunks - 1) / a.chunks + 15) & ~15l;      // chunks begin at 16-byte borders of the plane
+  p.begin = min((long)p.k * per, a.S), p.end = min(p.begin + per, a.S);
+  return p;
+}
+// sum over the unit; every thread of a wave-unit, thread 0 of a workgroup-unit has it
+template <int TPU>
+__device__ __forceinline__ double2 gn_unit_sum(double x, double y) {
+  x = gn_wave_sum(x), y = gn_wave_sum(y);
+  if (TPU == 64) return {x, y};
+  __shared__ double2 sh[kGnWaves];
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = {x, y};
+  __syncthreads();
+  x = y = 0.;
+#pragma unroll
+  for (int i = 0; i < kGnWaves; ++i) x += sh[i].x, y += sh[i].y;
+  return {x, y};
+}
+
+template <int DT, int V, int TPU>
+__global__ void __launch_bounds__(kGnThreads) gn_pl_stats_kernel(GnArgs a) {
+  using T = typename GnType<DT>::T;
+  const GnPl t = gn_pl<TPU>(a, blockIdx.x);
+  double s = 0., q = 0.;
+  if (t.on) {
+    const T* p = static_cast<const T*>(a.x) + t.plane * a.S;
+    constexpr int U = 4;
+    long i = t.begin + t.t * V;
+    for (; i + (U - 1) * TPU * V < t.end; i += U * TPU * V) {
+      GnVec<T, V> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = gn_load<T, V>(p + i + u * TPU * V);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const double f = (double)(float)v[u].v[j];
+          s += f, q += f * f;
+        }
+    }
+    for (; i < t.end; i += TPU * V) {
+      const GnVec<T, V> v = gn_load<T, V>(p + i);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const double f = (double)(float)v.v[j];
+        s += f, q += f * f;
+      }
+    }
+  }
+  const double2 v = gn_unit_sum<TPU>(s, q);
+  if (t.on && t.t == 0) {
+    const int g = t.c / a.cg;
+    a.part[((long)t.n * a.G + g) * a.pieces + (t.c - g * a.cg) * a.chunks + t.k] = v;
+  }
+}
+
+template <int DT, int V, int TPU, bool SILU>
+__global__ void __launch_bounds__(kGnThreads) gn_pl_apply_kernel(GnArgs a) {
+  using T = typename GnType<DT>::T;
+  const GnPl t = gn_pl<TPU>(a, blockIdx.x);
+  if (!t.on) return;                                 // (workgroup-units: the whole workgroup)
+  const int g = t.c / a.cg;
+  const long ig = (long)t.n * a.G + g;
+  const GnStat s = gn_stat(gn_join(a.part + ig * a.pieces, a.pieces), (double)a.M, a.eps);
+  if (t.t == 0 && t.k == 0 && t.c == g * a.cg) a.mean[ig] = s.mean, a.rstd[ig] = s.rstd;
+  const float mh = (float)s.mean, ml = (float)(s.mean - (double)mh);
+  const float sc = (float)(s.rstd * (double)gn_param<T>(a.w, t.c, a.wdt, 1.f)), b = gn_param<T>(a.b, t.c, a.wdt, 0.f);
+  const T* p = static_cast<const T*>(a.x) + t.plane * a.S;
+  T* o = static_cast<T*>(a.out) + t.plane * a.S;
+  for (long i = t.begin + t.t * V; i < t.end; i += TPU * V) {
+    const GnVec<T, V> v = gn_load<T, V>(p + i);
+    float f[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = gn_act<SILU>((((float)v.v[j] - mh) - ml) * sc + b, a.slope);
+    gn_store<T, V>(o + i, f);
+  }
+}
+
+template <int DT, int V, int TPU, bool SILU>
+__global__ void __launch_bounds__(kGnThreads) gn_pl_bwd_reduce_kernel(GnArgs a) {
+  using T = typename GnType<DT>::T;
+  const GnPl t = gn_pl<TPU>(a, blockIdx.x);
+  double s = 0., q = 0., rstd = 0.;
+  float w = 0.f;
+  if (t.on) {
+    const long ig = (long)t.n * a.G + t.c / a.cg;
+    const double mean = a.mean[ig];
+    rstd = a.rstd[ig];
+    const float mh = (float)mean, ml = (float)(mean - (double)mh), b = gn_param<T>(a.b, t.c, a.wdt, 0.f);
+    w = gn_param<T>(a.w, t.c, a.wdt, 1.f);
+    const float sc = (float)(rstd * (double)w);
+    const T *p = static_cast<const T*>(a.x) + t.plane * a.S, *pd = static_cast<const T*>(a.dy) + t.plane * a.S;
+    constexpr int U = 4;
+    for (long i = t.begin + t.t * V; i < t.end; i += U * TPU * V) {
+      GnVec<T, V> v[U], e[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long iu = i + u * TPU * V < t.end ? i + u * TPU * V : i;
+        v[u] = gn_load<T, V>(p + iu), e[u] = gn_load<T, V>(pd + iu);
+      }
+      float fs = 0.f, fq = 0.f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float x = (float)v[u].v[j], d = (x - mh) - ml;
+          const float gr = gn_grad<SILU>((float)e[u].v[j], x, d, sc, b, w, a.slope, mean, rstd);
+          if (i + u * TPU * V < t.end) fs += gr, fq += gr * d;
+        }
+      s += (double)fs, q += (double)fq;
+    }
+  }
+  double2 v = gn_unit_sum<TPU>(s, q);
+  if (t.on && t.t == 0) {
+    v.y *= rstd;
+    if (a.partc) a.partc[t.n * a.pcn + t.k * a.pck + t.c * a.pcc] = v;
+    const int g = t.c / a.cg;
+    a.part[((long)t.n * a.G + g) * a.pieces + (t.c - g * a.cg) * a.chunks + t.k] = {v.x * (double)w, v.y * (double)w};
+  }
+}
+
+template <int DT, int V, int TPU, bool SILU>
+__global__ void __launch_bounds__(kGnThreads) gn_pl_bwd_apply_kernel(GnArgs a) {
+  using T = typename GnType<DT>::T;
+  if ((int)blockIdx.x < a.dwb) return gn_param_grads<DT>(a, blockIdx.x);
+  const GnPl t = gn_pl<TPU>(a, (long)blockIdx.x - a.dwb);
+  if (!t.on) return;
+  const long ig = (long)t.n * a.G + t.c / a.cg;
+  const double2 sum = gn_join(a.part + ig * a.pieces, a.pieces);
+  const double mean = a.mean[ig], rstd = a.rstd[ig];
+  const float mh = (float)mean, ml = (float)(mean - (double)mh), b = gn_param<T>(a.b, t.c, a.wdt, 0.f);
+  const float w = gn_param<T>(a.w, t.c, a.wdt, 1.f), sc = (float)(rstd * (double)w);
+  const float c1 = (float)(rstd * sum.x / (double)a.M), c2 = (float)(rstd * rstd * sum.y / (double)a.M);
+  const T *p = static_cast<const T*>(a.x) + t.plane * a.S, *pd = static_cast<const T*>(a.dy) + t.plane * a.S;
+  T* o = static_cast<T*>(a.out) + t.plane * a.S;
+  for (long i = t.begin + t.t * V; i < t.end; i += TPU * V) {
+    const GnVec<T, V> v = gn_load<T, V>(p + i), e = gn_load<T, V>(pd + i);
+    float f[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float x = (float)v.v[j], d = (x - mh) - ml;
+      f[j] = (sc * gn_grad<SILU>((float)e.v[j], x, d, sc, b, w, a.slope, mean, rstd) - c1) - d * c2;
+    }
+    gn_store<T, V>(o + i, f);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+constexpr int kGnMaxJoin = 1024;      // double2 that a workgroup of the apply launch joins; above, one more launch does
+
+struct GnPlan {
+  GnArgs a;
+  int V, tpu;
+  bool last, finish;
+  long wgs, part, partc, fin;          // workgroups of the map; double2 of the workspace's three parts
+};
+
+static int gn_vec(long n, int size) {  // values per access: 16 bytes where the contiguous extent allows it
+  for (int v = 16 / size; v > 1; v >>= 1)
+    if (n % v == 0) return v;
+  return 1;
+}
+
+static GnPlan gn_plan(int N, int C, long S, int G, int dtype, int last) {
+  GnPlan p{};
+  GnArgs& a = p.a;
+  a.N = N, a.C = C, a.S = S, a.G = G, a.cg = C / G, a.M = (long)a.cg * S;
+  const int size = dtype == 0 ? 4 : 2;
+  p.last = last != 0;
+  if (p.last) {
+    p.V = gn_vec(C, size);
+    const int cv = C / p.V;
+    // slabs: as many threads of the 256 at work as possible, whole groups where they fit
+    int best = 0, wv = cv;
+    for (int k = (cv + kGnThreads - 1) / kGnThreads; k <= (cv + kGnThreads - 1) / kGnThreads + 3; ++k) {
+      int w = (cv + k - 1) / k;
+      const int unit = a.cg % p.V == 0 ? a.cg / p.V : a.cg;        // vectors from one group border to the next on a vector border
+      if (unit <= kGnThreads && (w + unit - 1) / unit * unit <= kGnThreads) w = (w + unit - 1) / unit * unit;
+      if (w > cv) w = cv;
+      const int used = kGnThreads / w * w;
+      if (used > best + 16) best = used, wv = w;
+    }
+    a.width = wv * p.V, a.slabs = (C + a.width - 1) / a.width;
+    a.slab_pieces = 1;
+    for (int g = 0; g < G; ++g) {
+      const int shared = ((g + 1) * a.cg - 1) / a.width - g * a.cg / a.width + 1;
+      if (shared > a.slab_pieces) a.slab_pieces = shared;
+    }
+    long chunks = (S * wv + kGnThreads * 8 - 1) / (kGnThreads * 8);
+    long cap = 2048 / ((long)N * a.slabs);
+    if (cap < 1) cap = 1;
+    if (chunks > cap) chunks = cap;
+    if (chunks < 1) chunks = 1;
+    a.chunks = (int)chunks, a.pieces = a.chunks * a.slab_pieces, a.npc = a.chunks;
+    a.pcn = (long)a.chunks * C, a.pck = C, a.pcc = 1;
+    p.wgs = (long)N * a.slabs * a.chunks;
+    const long touched = (a.width + a.cg - 1) / a.cg + 1;
+    p.finish = (touched < G ? touched : G) * a.pieces > kGnMaxJoin;
+  } else {
+    p.V = gn_vec(S, size);
+    p.tpu = S >= 4096 ? 256 : 64;
+    long chunks = (S + p.tpu * p.V * 8 - 1) / (p.tpu * p.V * 8);
+    long cap = 2048 / ((long)N * C) * (256 / p.tpu);
+    if (cap < 1) cap = 1;
+    if (chunks > cap) chunks = cap;
+    a.chunks = (int)chunks, a.pieces = a.cg * a.chunks, a.npc = a.chunks;
+    a.pcn = (long)C * a.chunks, a.pck = 1, a.pcc = a.chunks;
+    p.wgs = ((long)N * C * a.chunks * p.tpu + 255) / 256;
+    p.finish = a.pieces > (p.tpu == 64 ? kGnMaxJoin / 4 : kGnMaxJoin);
+  }
+  p.part = (long)N * G * a.pieces, p.fin = p.finish ? (long)N * G : 0, p.partc = (long)N * C * a.npc;
+  return p;
+}
+
+template <int DT, int V>
+static void gn_fwd_launch(const GnPlan& p, GnArgs a, bool silu, hipStream_t st) {
+  const dim3 grid((unsigned)p.wgs), block(kGnThreads);
+  if (p.last) {
+    if (a.cg % V == 0) hipLaunchKernelGGL((gn_cl_stats_kernel<DT, V, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((gn_cl_stats_kernel<DT, V, false>), grid, block, 0, st, a);
+  } else if (p.tpu == 256) hipLaunchKernelGGL((gn_pl_stats_kernel<DT, V, 256>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((gn_pl_stats_kernel<DT, V, 64>), grid, block, 0, st, a);
+  if (p.finish) {
+    hipLaunchKernelGGL(gn_finish_kernel, dim3(cdiv((long)a.N * a.G, kGnWaves)), block, 0, st, a.part, a.pieces, (long)a.N * a.G, a.part + p.part);
+    a.part += p.part, a.pieces = 1;
+  }
+  const unsigned lds = (unsigned)((a.width + a.cg - 1) / a.cg + 1) * sizeof(GnStat);
+#define BMV_GN_APPLY(SILU)                                                                                      \
+  if (p.last) hipLaunchKernelGGL((gn_cl_apply_kernel<DT, V, SILU>), grid, block, lds, st, a);                   \
+  else if (p.tpu == 256) hipLaunchKernelGGL((gn_pl_apply_kernel<DT, V, 256, SILU>), grid, block, 0, st, a);     \
+  else hipLaunchKernelGGL((gn_pl_apply_kernel<DT, V, 64, SILU>), grid, block, 0, st, a)
+  if (silu) { BMV_GN_APPLY(true); } else { BMV_GN_APPLY(false); }
+#undef BMV_GN_APPLY
+}
+
+template <int DT, int V, bool SILU>
+static void gn_bwd_launch(const GnPlan& p, GnArgs a, hipStream_t st) {
+  const dim3 grid((unsigned)p.wgs), block(kGnThreads);
+  a.dwb = a.partc ? (a.C + 7) / 8 : 0;
+  if (p.last) hipLaunchKernelGGL((gn_cl_bwd_reduce_kernel<DT, V, SILU>), grid, block, 0, st, a);
+  else if (p.tpu == 256) hipLaunchKernelGGL((gn_pl_bwd_reduce_kernel<DT, V, 256, SILU>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((gn_pl_bwd_reduce_kernel<DT, V, 64, SILU>), grid, block, 0, st, a);
+  if (p.finish) {
+    hipLaunchKernelGGL(gn_finish_kernel, dim3(cdiv((long)a.N * a.G, kGnWaves)), block, 0, st, a.part, a.pieces, (long)a.N * a.G, a.part + p.part);
+    a.part += p.part, a.pieces = 1;
+  }
+  const dim3 grid2((unsigned)(p.wgs + a.dwb));
+  const unsigned lds = (unsigned)((a.width + a.cg - 1) / a.cg + 1) * sizeof(double2);
+  if (p.last) hipLaunchKernelGGL((gn_cl_bwd_apply_kernel<DT, V, SILU>), grid2, block, lds, st, a);
+  else if (p.tpu == 256) hipLaunchKernelGGL((gn_pl_bwd_apply_kernel<DT, V, 256, SILU>), grid2, block, 0, st, a);
+  else hipLaunchKernelGGL((gn_pl_bwd_apply_kernel<DT, V, 64, SILU>), grid2, block, 0, st, a);
+}
+
+template <int DT, int V>
+static void gn_launch(const GnPlan& p, const GnArgs& a, bool bwd, bool silu, hipStream_t st) {
+  if (!bwd) gn_fwd_launch<DT, V>(p, a, silu, st);
+  else if (silu) gn_bwd_launch<DT, V, true>(p, a, st);
+  else gn_bwd_launch<DT, V, false>(p, a, st);
+}
+
+static void gn_dispatch(const GnPlan& p, const GnArgs& a, int dtype, bool bwd, bool silu, hipStream_t st) {
+#define BMV_GN_V(DT, VEC) if (p.V == VEC) return gn_launch<DT, VEC>(p, a, bwd, silu, st)
+  if (dtype == 0) {
+    BMV_GN_V(0, 4);
+    BMV_GN_V(0, 2);
+    BMV_GN_V(0, 1);
+  } else if (dtype == 1) {
+    BMV_GN_V(1, 8);
+    BMV_GN_V(1, 4);
+    BMV_GN_V(1, 2);
+    BMV_GN_V(1, 1);
+  } else {
+    BMV_GN_V(2, 8);
+    BMV_GN_V(2, 4);
+    BMV_GN_V(2, 2);
+    BMV_GN_V(2, 1);
+  }
+#undef BMV_GN_V
+}
+
+static bool gn_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+static const char* gn_bad_shape(int N, int C, long S, int G, int dtype) {
+  if (N <= 0 || C <= 0 || S <= 0) return "bad shape";
+  if (G <= 0 || C % G) return "the channels are no multiple of the groups";
+  if (dtype < 0 || dtype > 2) return "unknown type";
+  if ((long)N * C > (1l << 24) || S > (1l << 40) / ((long)N * C)) return "the map is too large";
+  return nullptr;
+}
+
+}  // namespace bmv
+
+using namespace bmv;
+
+extern "C" {
+
+long bmv_group_norm_workspace(int N, int C, long S, int G, int dtype, int channels_last, int backward) {
+  const char* bad = gn_bad_shape(N, C, S, G, dtype);
+  BMV_REQUIRE(!bad, "bmv_group_norm_workspace: %s (N %d, C %d, S %ld, groups %d)", bad, N, C, S, G);
+  const GnPlan p = gn_plan(N, C, S, G, dtype, channels_last);
+  return 2 * (p.part + p.fin + (backward ? p.partc : 0));
+}
+
+int bmv_group_norm_fwd(const void* x, const void* weight, const void* bias, int N, int C, long S, int G, int dtype,
+                       int param_dtype, int channels_last, double eps, int act, float slope, double* workspace, double* mean,
+                       double* rstd, void* y, bmv_stream_t stream) {
+  BMV_REQUIRE(x && workspace && mean && rstd && y, "bmv_group_norm_fwd: null pointer");
+  const char* bad = gn_bad_shape(N, C, S, G, dtype);
+  BMV_REQUIRE(!bad, "bmv_group_norm_fwd: %s (N %d, C %d, S %ld, groups %d)", bad, N, C, S, G);
+  BMV_REQUIRE(param_dtype == 0 || param_dtype == dtype, "bmv_group_norm_fwd: weight and bias are 32-bit or of the map's type");
+  BMV_REQUIRE(eps >= 0., "bmv_group_norm_fwd: eps must not be negative");
+  BMV_REQUIRE(act == 0 || act == 1, "bmv_group_norm_fwd: unknown activation %d", act);
+  BMV_REQUIRE(gn_aligned(x) && gn_aligned(y) && gn_aligned(workspace), "bmv_group_norm_fwd: x, y and workspace begin at 16-byte addresses");
+  const GnPlan p = gn_plan(N, C, S, G, dtype, channels_last);
+  GnArgs a = p.a;
+  a.x = x, a.w = weight, a.b = bias, a.out = y, a.mean = mean, a.rstd = rstd, a.wdt = param_dtype, a.eps = eps, a.slope = slope;
+  a.part = reinterpret_cast<double2*>(workspace);
+  gn_dispatch(p, a, dtype, false, act == 1, as_stream(stream));
+  BMV_LAUNCH_END("bmv_group_norm_fwd");
+}
+
+int bmv_group_norm_bwd(const void* x, const void* dy, const void* weight, const void* bias, const double* mean,
+                       const double* rstd, int N, int C, long S, int G, int dtype, int param_dtype, int channels_last, int act,
+                       float slope, double* workspace, void* dx, void* dweight, void* dbias, bmv_stream_t stream) {
+  BMV_REQUIRE(x && dy && mean && rstd && workspace && dx, "bmv_group_norm_bwd: null pointer");
+  const char* bad = gn_bad_shape(N, C, S, G, dtype);
+  BMV_REQUIRE(!bad, "bmv_group_norm_bwd: %s (N %d, C %d, S %ld, groups %d)", bad, N, C, S, G);
+  BMV_REQUIRE(param_dtype == 0 || param_dtype == dtype, "bmv_group_norm_bwd: weight and bias are 32-bit or of the map's type");
+  BMV_REQUIRE(act == 0 || act == 1, "bmv_group_norm_bwd: unknown activation %d", act);
+  BMV_REQUIRE(gn_aligned(x) && gn_aligned(dy) && gn_aligned(dx) && gn_aligned(workspace),
+              "bmv_group_norm_bwd: x, dy, dx and workspace begin at 16-byte addresses");
+  const GnPlan p = gn_plan(N, C, S, G, dtype, channels_last);
+  GnArgs a = p.a;
+  a.x = x, a.dy = dy, a.w = weight, a.b = bias, a.out = dx, a.dw = dweight, a.db = dbias, a.wdt = param_dtype, a.slope = slope;
+  a.mean = const_cast<double*>(mean), a.rstd = const_cast<double*>(rstd);
+  a.part = reinterpret_cast<double2*>(workspace);
+  a.partc = dweight || dbias ? a.part + p.part + p.fin : nullptr;
+  gn_dispatch(p, a, dtype, true, act == 1, as_stream(stream));
+  BMV_LAUNCH_END("bmv_group_norm_bwd");
+}
+
+}  // extern "C"

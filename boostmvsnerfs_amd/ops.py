@@ -5,6 +5,7 @@ Everything runs on torch's current stream.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
@@ -1344,6 +1345,145 @@ def bn_train_bwd(x, y, dy, weight, mean, invstd, relu):
                                   dptr(mean), dptr(invstd), N, C_, S, _act_slope(relu), dptr(ws), dptr(dx), dptr(dw), dptr(db),
                                   stream())
     _lib.check(rc, "bn_train_bwd")
+    return dx, dw, db
+
+
+_FLOAT_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # include/bmv.h: dtype
+
+
+def _on_device_of(t):
+    """A context in which `t`'s device is the current one (launches and allocations go there)."""
+    return contextlib.nullcontext() if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def _gpu_float(t, name, like=None):
+    """`t` is a GPU tensor of a supported floating type (and of `like`'s device); raises otherwise."""
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name}: expected a tensor, got {type(t)}")
+    if t.dtype not in _FLOAT_CODES:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name}: the BoostMVSNeRFs hot path runs on the GPU only (tensor is on {t.device}); "
+                           "there is no CPU fallback")
+    if like is not None and t.device != like.device:
+        raise RuntimeError(f"{name}: on {t.device}, expected {like.device}")
+    return t
+
+
+def _addr(t):
+    """Address of a dense tensor of any layout, kept referenced until the launch is enqueued (see _lib.dptr)."""
+    if t is None:
+        return None
+    _lib._held_list().append(t)
+    return t.data_ptr()
+
+
+def _gn_dense(x):
+    """(x dense in one of the two layouts, 1 for channel-last / 0 for planar)."""
+    last = x.dim() > 2 and ((x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last))
+                            or (x.dim() == 5 and x.is_contiguous(memory_format=torch.channels_last_3d))
+                            or (x.dim() == 3 and x.transpose(1, 2).is_contiguous()))
+    if not (last or x.is_contiguous()):
+        x = x.contiguous()
+    if x.data_ptr() & 15:           # (a view that begins inside a 16-byte piece)
+        x = x.clone(memory_format=torch.preserve_format)
+    # (where both layouts are one -- a single position -- the channel axis is the contiguous one)
+    return x, int(last and x.shape[1] > 1 or x.numel() == x.shape[0] * x.shape[1])
+
+
+def _gn_check(x, groups, weight, bias, relu):
+    _gpu_float(x, "x")
+    if x.dim() < 2:
+        raise ValueError(f"x: expected (N, C, *spatial), got {tuple(x.shape)}")
+    groups = int(groups)
+    if groups <= 0 or x.shape[1] == 0 or x.shape[1] % groups:
+        raise ValueError(f"groups: {groups} do not divide {x.shape[1]} channels")
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        _gpu_float(t, name, x)
+        if tuple(t.shape) != (x.shape[1],):
+            raise ValueError(f"{name}: expected ({x.shape[1]},), got {tuple(t.shape)}")
+        if t.dtype not in (torch.float32, x.dtype):
+            raise TypeError(f"{name}: expected float32 or {x.dtype}, got {t.dtype}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"weight and bias: {weight.dtype} and {bias.dtype}, expected one type")
+    if isinstance(relu, str):
+        if relu != "silu":
+            raise ValueError(f"relu: expected False, True, a slope or 'silu', got {relu!r}")
+        return groups, 1, 0.0
+    return groups, 0, _act_slope(relu)
+
+
+def _gn_param_code(x, weight, bias):
+    p = weight if weight is not None else bias
+    return 0 if p is None else _FLOAT_CODES[p.dtype]
+
+
+def group_norm_fwd(x, groups, weight=None, bias=None, eps=1e-5, relu=False):
+    """Group norm with an activation of x (N,C,*spatial), fp32 / bf16 / fp16, channel-last or planar (any other strides are
+    copied to planar): y = act((x - mean) / sqrt(var + eps) * weight + bias), statistics over a sample's C / groups channels.
+    `relu`: False, True, a leaky slope, or "silu".  weight / bias (C): fp32 or x's type, or None.
+    -> y (x's layout and type), mean, rstd (N, groups; float64, what `group_norm_bwd` reads)."""
+    groups, act, slope = _gn_check(x, groups, weight, bias, relu)
+    if not eps >= 0:
+        raise ValueError(f"eps: {eps} is negative")
+    with _on_device_of(x):
+        x, last = _gn_dense(x)
+        N, C_ = x.shape[:2]
+        S = x.numel() // max(1, N * C_)
+        y = torch.empty_like(x)
+        stats = torch.empty(2, N, groups, device=x.device, dtype=torch.float64)
+        mean, rstd = stats[0], stats[1]
+        if x.numel() == 0:
+            mean.zero_(), rstd.zero_()
+            return y, mean, rstd
+        lib = _lib.load()
+        code = _FLOAT_CODES[x.dtype]
+        n_ws = lib.bmv_group_norm_workspace(N, C_, S, groups, code, last, 0)
+        if n_ws < 0:
+            _lib.check(int(n_ws), "group_norm_workspace")
+        ws = torch.empty(n_ws, device=x.device, dtype=torch.float64)
+        with ktimer.region("group_norm_fwd"):
+            rc = lib.bmv_group_norm_fwd(_addr(x), _addr(weight if weight is None else _c(weight)), _addr(bias if bias is None else _c(bias)),
+                                        N, C_, S, groups, code, _gn_param_code(x, weight, bias), last, float(eps), act, slope,
+                                        _addr(ws), _addr(mean), _addr(rstd), _addr(y), stream())
+        _lib.check(rc, "group_norm_fwd")
+    return y, mean, rstd
+
+
+def group_norm_bwd(x, dy, groups, weight, bias, mean, rstd, relu=False, want_params=True):
+    """-> dx (x's layout and type), dweight, dbias (C; None where weight / bias is None or not `want_params`)."""
+    groups, act, slope = _gn_check(x, groups, weight, bias, relu)
+    _gpu_float(dy, "dy", x)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError(f"dy: expected {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if tuple(t.shape) != (x.shape[0], groups) or t.dtype != torch.float64 or t.device != x.device:
+            raise ValueError(f"{name}: expected ({x.shape[0]}, {groups}) float64 on {x.device}")
+    with _on_device_of(x):
+        x, last = _gn_dense(x)
+        if dy.stride() != x.stride() or dy.data_ptr() & 15:
+            dy = torch.empty_like(x).copy_(dy)
+        N, C_ = x.shape[:2]
+        S = x.numel() // max(1, N * C_)
+        dx = torch.empty_like(x)
+        dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if weight is not None and want_params else None
+        db = torch.empty_like(bias, memory_format=torch.contiguous_format) if bias is not None and want_params else None
+        if x.numel() == 0:
+            return dx, dw if dw is None else dw.zero_(), db if db is None else db.zero_()
+        lib = _lib.load()
+        code = _FLOAT_CODES[x.dtype]
+        n_ws = lib.bmv_group_norm_workspace(N, C_, S, groups, code, last, 1)
+        if n_ws < 0:
+            _lib.check(int(n_ws), "group_norm_workspace")
+        ws = torch.empty(n_ws, device=x.device, dtype=torch.float64)
+        with ktimer.region("group_norm_bwd"):
+            rc = lib.bmv_group_norm_bwd(_addr(x), _addr(dy), _addr(weight if weight is None else _c(weight)),
+                                        _addr(bias if bias is None else _c(bias)), _addr(_c(mean)), _addr(_c(rstd)), N, C_, S, groups, code,
+                                        _gn_param_code(x, weight, bias), last, act, slope, _addr(ws), _addr(dx), _addr(dw),
+                                        _addr(db), stream())
+        _lib.check(rc, "group_norm_bwd")
     return dx, dw, db
 
 

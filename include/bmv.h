@@ -346,6 +346,21 @@ int bmv_bn_train_bwd(const float* x, const float* y, const float* dy, const floa
                      const float* save_invstd, int N, int C, long S, float act_slope, float* workspace, float* dx,
                      float* dweight, float* dbias, bmv_stream_t stream);
 
+/* ---- group normalisation (+ activation), training and inference: bmv_bn_train_*'s stand-in where a step sees one image
+ * x, y, dy, dx: (N, C, S) planar or (N, S, C) channel-last, S = H*W or D*H*W, of `dtype` (0 fp32, 1 bf16, 2 fp16), beginning
+ * at 16-byte addresses.  weight, bias, dweight, dbias (C): `param_dtype` = 0 (fp32) or dtype; each may be NULL.
+ * y = act((x - mean) rstd w + b) with the mean and (biased) variance of a sample's group of C / G channels, rstd =
+ * 1 / sqrt(var + eps); act 0: v > 0 ? v : slope * v (1 none, 0 ReLU), act 1: v / (1 + exp(-v)) (slope ignored).
+ * mean, rstd (N, G) are 64-bit: the backward recomputes z and decides its sign with them.
+ * workspace: bmv_group_norm_workspace(...) doubles (backward = 1 for the gradients' call). */
+long bmv_group_norm_workspace(int N, int C, long S, int G, int dtype, int channels_last, int backward);
+int bmv_group_norm_fwd(const void* x, const void* weight, const void* bias, int N, int C, long S, int G, int dtype,
+                       int param_dtype, int channels_last, double eps, int act, float slope, double* workspace, double* mean,
+                       double* rstd, void* y, bmv_stream_t stream);
+int bmv_group_norm_bwd(const void* x, const void* dy, const void* weight, const void* bias, const double* mean,
+                       const double* rstd, int N, int C, long S, int G, int dtype, int param_dtype, int channels_last, int act,
+                       float slope, double* workspace, void* dx, void* dweight, void* dbias, bmv_stream_t stream);
+
 /* ======================= MVSNeRF backbone (lib/networks/mvsnerf) ======================= */
 
 /* ---- a18 Network.get_proj_mats            lib/networks/mvsnerf/network.py:1070-1090
