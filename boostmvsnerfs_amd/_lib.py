@@ -144,6 +144,11 @@ SIGNATURES = {
     "bmv_group_norm_workspace": [c_i, c_i, c_l, c_i, c_i, c_i, c_i],
     "bmv_group_norm_fwd": [c_f, c_f, c_f, c_i, c_i, c_l, c_i, c_i, c_i, c_i, C.c_double, c_i, c_fl, c_f, c_f, c_f, c_f, c_f],
     "bmv_group_norm_bwd": [c_f, c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_l, c_i, c_i, c_i, c_i, c_i, c_fl, c_f, c_f, c_f, c_f, c_f],
+    "bmv_newton_schulz_workspace": [c_i, C.POINTER(C.c_int), C.POINTER(C.c_int)],
+    "bmv_newton_schulz": [c_i, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_int), C.POINTER(C.c_int), c_i, c_i, c_fl, c_fl,
+                          c_fl, c_fl, c_f, c_f],
+    "bmv_muon_step": [c_i, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_int), C.POINTER(C.c_int),
+                      C.POINTER(C.c_float), c_i, C.c_double, c_i, C.c_double, c_i, c_fl, c_fl, c_fl, c_fl, c_f, c_f],
     "bmv_conv_top_fwd": [c_f, c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_i, c_fl, c_i, c_f],
     "bmv_conv0_fused_fwd": [c_f, c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_i, c_i, c_fl, c_fl, c_f],
     "bmv_conv_heads_fwd": [c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_i, c_i, c_i, c_f],
@@ -199,6 +204,7 @@ def load():
     lib.bmv_mvs_mlp_train_scratch_floats.restype = C.c_long
     lib.bmv_conv_wgrad_workspace.restype = C.c_long
     lib.bmv_group_norm_workspace.restype = C.c_long
+    lib.bmv_newton_schulz_workspace.restype = C.c_long
     lib.bmv_last_error.argtypes = []
     lib.bmv_last_error.restype = C.c_char_p
     lib.bmv_tuning_name.restype = C.c_char_p

@@ -15,7 +15,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libbmv.so")
-SOURCES = ["sweep.hip", "sweep_win.hip", "sweep_quad.hip", "tuning.hip", "sample.hip", "render.hip", "mvs.hip", "mvs_mlp_train.hip", "backward.hip", "sweep_bwd_cl.hip", "mlp_bwd.hip", "conv.hip", "conv_c4.hip", "conv_c4s.hip", "fpn_s.hip", "conv2d_s.hip", "conv_split.hip", "conv_wgrad.hip", "bn.hip", "group_norm.hip", "rays.hip", "timing.hip"]
+SOURCES = ["sweep.hip", "sweep_win.hip", "sweep_quad.hip", "tuning.hip", "sample.hip", "render.hip", "mvs.hip", "mvs_mlp_train.hip", "backward.hip", "sweep_bwd_cl.hip", "mlp_bwd.hip", "conv.hip", "conv_c4.hip", "conv_c4s.hip", "fpn_s.hip", "conv2d_s.hip", "conv_split.hip", "conv_wgrad.hip", "bn.hip", "group_norm.hip", "newton_schulz.hip", "rays.hip", "timing.hip"]
 HEADERS = ["bmv_common.hpp", "scatter.hpp", "sweep_util.hpp", "render_geom.hpp", "mlp.hpp", os.path.join("..", "..", "include", "bmv.h")]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function"]
 EXTRA_FLAGS = {}    # per-file flags
@@ -24,7 +24,7 @@ EXTRA_FLAGS = {}    # per-file flags
 EXTRA_FLAGS["sweep_quad.hip"] = ["-fno-slp-vectorize"]
 # no packed fp32 arithmetic (v_pk_add / mul / fma_f32) out of ordinary float code (the host pass warns that it does not know the feature)
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-EXTRA_FLAGS["group_norm.hip"] = list(NO_PACKED_FP32)
+EXTRA_FLAGS["group_norm.hip"] = EXTRA_FLAGS["newton_schulz.hip"] = NO_PACKED_FP32
 if os.environ.get("BMV_QUAD_DEFS"):
     EXTRA_FLAGS["sweep_quad.hip"] += os.environ["BMV_QUAD_DEFS"].split()
 if os.environ.get("BMV_RENDER_DEFS"):   # e.g. "-DBMV_RENDER_STAMPS" for scripts/stamps_render.py

@@ -1487,6 +1487,130 @@ def group_norm_bwd(x, dy, groups, weight, bias, mean, rstd, relu=False, want_par
     return dx, dw, db
 
 
+NS_COEFFS = (3.4445, -4.7750, 2.0315)      # the quintic a s + b s^3 + c s^5 of a Newton-Schulz step
+NS_EPS = 1e-7
+
+
+def _matrix(t, name):
+    """(rows, cols) of a weight as a matrix: everything behind the first dimension is its columns."""
+    _gpu_float(t, name)
+    if t.dim() < 2:
+        raise ValueError(f"{name}: expected a matrix (at least 2 dimensions), got {tuple(t.shape)}")
+    rows = t.shape[0]
+    cols = t.numel() // rows if rows else 0
+    if rows > 65536 or cols > 65536:
+        raise ValueError(f"{name}: sides of up to 65536, got {rows} x {cols}")
+    return rows, cols
+
+
+def _ns_args(steps, coeffs, eps):
+    if int(steps) < 1:
+        raise ValueError(f"steps: expected at least 1, got {steps}")
+    a, b, c = (float(v) for v in coeffs)
+    if not eps >= 1e-12:
+        raise ValueError(f"eps: expected at least 1e-12, got {eps}")
+    return int(steps), a, b, c, float(eps)
+
+
+def _by_kind(tensors):
+    """Indices of the non-empty tensors, by (device, dtype): a launch has one of each."""
+    kinds = {}
+    for i, t in enumerate(tensors):
+        if t.numel():
+            kinds.setdefault((t.device, t.dtype), []).append(i)
+    return kinds.items()
+
+
+def _pointers(tensors):
+    return (C.c_void_p * len(tensors))(*[_addr(t) for t in tensors])
+
+
+def _ns_workspace(lib, count, rows, cols, device):
+    n = lib.bmv_newton_schulz_workspace(count, rows, cols)
+    if n < 0:
+        _lib.check(int(n), "newton_schulz_workspace")
+    return torch.empty(n, device=device, dtype=torch.uint8)
+
+
+def newton_schulz(mats, steps=5, coeffs=NS_COEFFS, eps=NS_EPS):
+    """Orthogonalise matrices: X = M / max(|M|_F, eps), then `steps` times A = X X^T, X = a X + (b A + c A A) X with
+    `coeffs` = (a, b, c) -- singular values towards 1, singular vectors kept.  `mats`: a tensor, or a list of tensors (one set
+    of launches for all), of 2 dimensions or more (what is behind the first is flattened: convolution kernels), fp32, bf16 or
+    fp16.  Computed at fp32 accuracy whatever the type.  -> new tensors of the same shapes and types."""
+    if torch.is_tensor(mats):
+        return newton_schulz([mats], steps, coeffs, eps)[0]
+    mats = list(mats)
+    steps, a, b, c, eps = _ns_args(steps, coeffs, eps)
+    sizes = [_matrix(t, f"mats[{i}]") for i, t in enumerate(mats)]
+    out = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in mats]
+    lib = _lib.load()
+    for (device, dtype), idx in _by_kind(mats):
+        with _on_device_of(mats[idx[0]]):
+            n = len(idx)
+            rows, cols = (C.c_int * n)(*[sizes[i][0] for i in idx]), (C.c_int * n)(*[sizes[i][1] for i in idx])
+            ws = _ns_workspace(lib, n, rows, cols, device)
+            with ktimer.region("newton_schulz"):
+                rc = lib.bmv_newton_schulz(n, _pointers([_c(mats[i]) for i in idx]), _pointers([out[i] for i in idx]), rows, cols,
+                                           _FLOAT_CODES[dtype], steps, a, b, c, eps, _addr(ws), stream())
+            _lib.check(rc, "newton_schulz")
+    return out
+
+
+MUON_SCALES = {
+    "shape": lambda rows, cols: max(1.0, rows / cols) ** 0.5,      # an update of unit spectral norm per output
+    "rms": lambda rows, cols: 0.2 * max(rows, cols) ** 0.5,        # an update of an Adam step's root mean square
+    "none": lambda rows, cols: 1.0,
+}
+
+
+def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale="shape", steps=5, coeffs=NS_COEFFS,
+              eps=NS_EPS):
+    """One optimiser step over a list of weight matrices, IN PLACE:
+        buf = momentum buf + (1 - momentum) grad;  U = (1 - momentum) grad + momentum buf  (nesterov) or buf
+        param = param (1 - lr weight_decay) - lr s newton_schulz(U)
+    with s by `scale`: "shape" sqrt(max(1, rows / cols)), "rms" 0.2 sqrt(max(rows, cols)), "none" 1.  params and grads: fp32, bf16
+    or fp16, 2 dimensions or more; momenta: fp32, of the params' shapes.  A tensor listed twice is refused."""
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError(f"{len(params)} params, {len(grads)} grads, {len(momenta)} momenta")
+    if scale not in MUON_SCALES:
+        raise ValueError(f"scale: expected one of {sorted(MUON_SCALES)}, got {scale!r}")
+    steps, a, b, c, eps = _ns_args(steps, coeffs, eps)
+    if not 0 <= momentum < 1:
+        raise ValueError(f"momentum: expected 0 <= momentum < 1, got {momentum}")
+    lr, keep = float(lr), 1.0 - float(lr) * float(weight_decay)
+    sizes = []
+    for i, (p, g, m) in enumerate(zip(params, grads, momenta)):
+        sizes.append(_matrix(p, f"params[{i}]"))
+        _gpu_float(g, f"grads[{i}]", p), _gpu_float(m, f"momenta[{i}]", p)
+        if g.shape != p.shape or g.dtype != p.dtype:
+            raise ValueError(f"grads[{i}]: expected {tuple(p.shape)} {p.dtype}, got {tuple(g.shape)} {g.dtype}")
+        if m.shape != p.shape or m.dtype != torch.float32:
+            raise ValueError(f"momenta[{i}]: expected {tuple(p.shape)} float32, got {tuple(m.shape)} {m.dtype}")
+    lib = _lib.load()
+    for (device, dtype), idx in _by_kind(params):
+        with torch.no_grad(), _on_device_of(params[idx[0]]):
+            n = len(idx)
+            rows, cols = (C.c_int * n)(*[sizes[i][0] for i in idx]), (C.c_int * n)(*[sizes[i][1] for i in idx])
+            scales = (C.c_float * n)(*[lr * MUON_SCALES[scale](*sizes[i]) for i in idx])
+            p, m = [_c(params[i]) for i in idx], [_c(momenta[i]) for i in idx]
+            ws = _ns_workspace(lib, n, rows, cols, device)
+            with ktimer.region("muon_step"):
+                rc = lib.bmv_muon_step(n, _pointers(p), _pointers([_c(grads[i]) for i in idx]), _pointers(m), rows, cols, scales,
+                                       _FLOAT_CODES[dtype], float(momentum), int(bool(nesterov)), keep, steps, a, b, c, eps,
+                                       _addr(ws), stream())
+            _lib.check(rc, "muon_step")
+            for i, new in zip(idx, p):             # (weights of other strides went through a copy)
+                if new is not params[i]:
+                    params[i].copy_(new)
+            for i, new in zip(idx, m):
+                if new is not momenta[i]:
+                    momenta[i].copy_(new)
+            # the kernels wrote through raw addresses: caches keyed by a weight's version (packed weights) have to see it,
+            # and autograd that a saved weight is not what it was
+            torch.autograd.graph.increment_version([params[i] for i in idx] + [momenta[i] for i in idx])
+
+
 def mvs_sweep_bwd(feats, proj, depth_values, d_volume, pad):
     """d_volume (B, 3S+C, D, hp, wp) -> d_feats (B,S,C,h,w)."""
     B, S, C_, h, w = feats.shape

@@ -1,0 +1,305 @@
+"""Newton-Schulz orthogonalisation and the optimiser step around it (csrc/newton_schulz.hip) against the formula in 64 bits on
+the CPU, and their refusals.
+
+Tolerance of an iterate, in the Frobenius norm: a product L R^T over k terms in fp32 (three-piece operands: dropped products
+below 3 x 2^-24 of a term, then fp32 sums) is off by at most eps_k |L|_F |R|_F with eps_k = 2^-24 (4 + 2 sqrt(k)) -- one
+rounding of each operand, of the result, and k roundings of partial sums of random sign.  A step turns errors of its three products
+into at most (|b| + 2 |c| |A|) dA |X| + |c| d(AA) |X| + d(QX) of X, and an error of X into at most L of it, L = max |p'| of the
+polynomial p = a s + b s^3 + c s^5 over the iterate's singular values (of the divided differences as well, which p' bounds).
+That sum is computed along the 64-bit iteration; bf16 and fp16 results add half a step of their rounding."""
+import math
+
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+def _iterate(u, steps=5, coeffs=COEFFS, eps=1e-7):
+    """(the iterate, its tolerance in the Frobenius norm) of u, in 64 bits."""
+    a, b, c = coeffs
+    u = u.double()
+    x = u / max(float(u.norm()), eps)
+    tall = x.shape[0] > x.shape[1]
+    x = x.mT if tall else x
+    m, n = x.shape
+    unit = 2.0 ** -24
+    ek = lambda k: unit * (4 + 2 * math.sqrt(k))       # noqa: E731
+    tol = 2 * unit * float(x.norm())
+    for _ in range(steps):
+        A = x @ x.mT
+        Q = a * torch.eye(m, dtype=torch.float64) + b * A + c * (A @ A)
+        s = max(float(torch.linalg.matrix_norm(x, 2)), 1e-300)
+        grid = torch.linspace(0, s, 200, dtype=torch.float64)
+        lip = float((a + 3 * b * grid ** 2 + 5 * c * grid ** 4).abs().max())
+        dA, dAA = ek(n) * float(x.norm()) ** 2, ek(m) * float(A.norm()) ** 2
+        local = ((abs(b) + 2 * abs(c) * s * s) * dA + abs(c) * dAA) * s + ek(m) * float(Q.norm()) * float(x.norm())
+        tol = lip * tol + local
+        x = Q @ x
+    return (x.mT if tall else x), tol
+
+
+def _grad(m, n, seed=0, rank=3, noise=0.1):
+    g = torch.Generator().manual_seed(seed)
+    return 1e-2 * (noise * torch.randn(m, n, generator=g) + torch.randn(m, rank, generator=g) @ torch.randn(rank, n, generator=g))
+
+
+def _check(got, u, steps=5, coeffs=COEFFS, eps=1e-7):
+    want, tol = _iterate(u, steps, coeffs, eps)
+    u_out = torch.finfo(got.dtype).eps / 2
+    err = float((got.double().cpu() - want).norm())
+    small = 2.0 ** -25 * math.sqrt(want.numel()) if got.dtype == torch.float16 else 0.0      # half a step of fp16's subnormals
+    assert err <= tol + u_out * float(want.norm()) + small, (tuple(u.shape), err, tol)
+    return err, tol
+
+
+SHAPES = [(1, 1), (1, 7), (9, 1), (2, 2), (3, 64), (8, 27), (16, 200), (35, 4), (64, 24), (33, 32), (63, 65), (64, 64), (64, 1728),
+          (65, 40), (127, 129), (128, 63), (128, 128), (128, 515), (129, 129), (130, 1000), (333, 257), (256, 384), (700, 90)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_newton_schulz_matches_the_formula(dtype):
+    from boostmvsnerfs_amd import ops
+    mats = [_grad(m, n, seed=i).to(dtype) for i, (m, n) in enumerate(SHAPES)]
+    on_gpu = [v.cuda() for v in mats]
+    before = [v.clone() for v in on_gpu]
+    out = ops.newton_schulz(on_gpu)
+    for got, u, src, keep in zip(out, mats, on_gpu, before):
+        assert got.shape == u.shape and got.dtype == dtype and torch.equal(src, keep)
+        _check(got, u)
+    # one call for the list, one call each: the same
+    for got, src in zip(out, on_gpu):
+        assert torch.equal(ops.newton_schulz(src), got), src.shape
+
+
+@gpu
+def test_newton_schulz_is_as_exact_as_the_iteration_in_fp32():
+    """Within four times the error of the same iteration in fp32 products (four: two roundings for its one at the operands'
+    pieces, and the spread of one random error against another), on flat and on decaying spectra."""
+    from boostmvsnerfs_amd import ops
+
+    def fp32(u):
+        a, b, c = COEFFS
+        x = u / u.norm()
+        for _ in range(5):
+            A = x @ x.mT
+            x = a * x + (b * A + c * (A @ A)) @ x
+        return x
+    for k, (m, n, rank, noise) in enumerate([(64, 200, 3, 0.1), (128, 128, 3, 0.1), (128, 1000, 128, 1.0), (256, 300, 5, 0.01), (200, 200, 200, 1.0)]):
+        u = _grad(m, n, k, rank, noise)
+        want, _ = _iterate(u)
+        base = float((fp32(u).double() - want).norm() / want.norm())
+        err = float((ops.newton_schulz(u.cuda()).double().cpu() - want).norm() / want.norm())
+        assert err <= 4 * base + 2.0 ** -24, (m, n, err, base)
+
+
+@gpu
+def test_newton_schulz_large_matrices():
+    from boostmvsnerfs_amd import ops
+    for m, n in ((1024, 1100), (1500, 520)):
+        u = _grad(m, n, 7)
+        _check(ops.newton_schulz(u.cuda()), u)
+
+
+@gpu
+def test_newton_schulz_orthogonalises():
+    """After enough steps of the classical cubic (1.5, -0.5, 0) the result is the orthogonal factor itself."""
+    from boostmvsnerfs_amd import ops
+    for m, n in ((24, 40), (40, 24), (140, 150)):
+        u = _grad(m, n, 3, rank=min(m, n), noise=1.0)
+        got = ops.newton_schulz(u.cuda(), steps=30, coeffs=(1.5, -0.5, 0.0)).double().cpu()
+        U, _, V = torch.linalg.svd(u.double(), full_matrices=False)
+        # the fixed point is stable (p'(1) = 0): what stays is one step's own error
+        eps = 2.0 ** -24 * (4 + 2 * math.sqrt(max(m, n)))
+        assert float((got - U @ V).norm()) <= 8 * eps * min(m, n), (m, n)
+
+
+@gpu
+def test_newton_schulz_steps_coefficients_and_lists():
+    from boostmvsnerfs_amd import ops
+    u = _grad(20, 30, 1)
+    for steps in (1, 2, 3, 8):
+        _check(ops.newton_schulz(u.cuda(), steps=steps), u, steps)
+    _check(ops.newton_schulz(u.cuda(), coeffs=(2.0, -1.5, 0.5)), u, coeffs=(2.0, -1.5, 0.5))
+    # a large eps damps: the norm does not count below it
+    _check(ops.newton_schulz(u.cuda(), eps=10.0), u, eps=10.0)
+    # more matrices than a launch's table holds, of mixed types, one of them a convolution kernel of other strides, one empty
+    g = torch.Generator().manual_seed(4)
+    mats = [torch.randn(1 + i % 9, 3 + 5 * (i % 7), generator=g).to((torch.float32, torch.bfloat16)[i % 2]) for i in range(90)]
+    conv = torch.randn(16, 8, 3, 3, generator=g)
+    on_gpu = [v.cuda() for v in mats] + [conv.cuda().to(memory_format=torch.channels_last), torch.empty(3, 0, device="cuda"),
+                                         torch.randn(40, 50, generator=g).cuda().t()]
+    out = ops.newton_schulz(on_gpu)
+    for got, v in zip(out, mats):
+        _check(got, v)
+    _check(out[90].flatten(1), conv.flatten(1))
+    assert out[91].shape == (3, 0)
+    _check(out[92], on_gpu[92].cpu())
+    assert ops.newton_schulz([]) == []
+
+
+@gpu
+def test_newton_schulz_zero_tiny_and_non_finite():
+    from boostmvsnerfs_amd import ops
+    u = _grad(24, 40, 2)
+    mats = [u * 0, u * 1e-12, u * 1e-30, u * 1e12, u.clone(), u.clone(), u]
+    mats[4][3, 5] = float("nan")
+    mats[5][0, 0] = float("inf")
+    out = ops.newton_schulz([v.cuda() for v in mats])
+    assert not out[0].any()
+    for k in (1, 2, 3, 6):
+        _check(out[k], mats[k])
+    assert out[4].isnan().all() and out[5].isnan().any()
+    # (what is below eps is divided by eps: 1e-30 stays tiny, and finite)
+    assert float(out[2].abs().max()) < 1e-18
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nesterov,scale,decay", [(True, "shape", 0.0), (False, "rms", 0.1), (True, "none", 0.01)])
+def test_muon_step_matches_the_formula(dtype, nesterov, scale, decay):
+    from boostmvsnerfs_amd import ops
+    shapes = [(8, 27), (64, 24), (1, 12), (128, 63), (130, 140), (16, 8, 3, 3), (200, 40)]
+    g = torch.Generator().manual_seed(11)
+    lr, mu = 0.02, 0.9
+    params = [torch.randn(s, generator=g).to(dtype) for s in shapes]
+    momenta = [torch.zeros(s) for s in shapes]
+    pg, mg = [p.cuda() for p in params], [m.cuda() for m in momenta]
+    for it in range(3):
+        grads = [torch.randn(s, generator=g).mul(0.1).to(dtype) for s in shapes]
+        params, momenta = [p.cpu() for p in pg], [m.cpu() for m in mg]        # (every step from the state that is there)
+        ops.muon_step(pg, [v.cuda() for v in grads], mg, lr, mu, nesterov, decay, scale)
+        for p, gr, m, pn, mn in zip(params, grads, momenta, pg, mg):
+            gd, md = gr.double(), m.double()
+            moved = mu * md + (1 - mu) * gd
+            # two products and a sum, with mu and 1 - mu rounded to fp32
+            off = (mn.double().cpu() - moved).abs() - 4 * 2.0 ** -24 * ((mu * md).abs() + ((1 - mu) * gd).abs()) - 1e-40
+            assert float(off.max()) <= 0, (tuple(p.shape), float(off.max()))
+            u = ((1 - mu) * gd + mu * moved if nesterov else moved).flatten(1)
+            o, tol = _iterate(u)
+            rows, cols = u.shape
+            s = {"shape": math.sqrt(max(1, rows / cols)), "rms": 0.2 * math.sqrt(max(rows, cols)), "none": 1.0}[scale]
+            want = p.double().flatten(1) * (1 - lr * decay) - lr * s * o
+            # the iterate's tolerance, its input's (U is off by a few 2^-24 of |U|, which the steps can amplify as they do X's own
+            # error: the tolerance begins with 2 x 2^-24 |X|, so four times as much again), and the roundings of the update
+            u_out = torch.finfo(dtype).eps / 2
+            lim = lr * s * 5 * tol + (u_out + 4 * 2.0 ** -24) * float(want.norm()) + 4 * 2.0 ** -24 * float(p.double().norm())
+            if dtype == torch.float16:
+                lim += 2.0 ** -25 * math.sqrt(want.numel())
+            err = float((pn.double().cpu().flatten(1) - want).norm())
+            assert err <= lim, (tuple(p.shape), err, lim)
+
+
+@gpu
+def test_muon_step_bumps_versions_and_takes_other_strides():
+    from boostmvsnerfs_amd import ops
+    g = torch.Generator().manual_seed(1)
+    p0, gr = torch.randn(16, 8, 3, 3, generator=g).cuda(), torch.randn(16, 8, 3, 3, generator=g).cuda()
+    pa, ma = p0.clone(), torch.zeros_like(p0)
+    pb = p0.to(memory_format=torch.channels_last)
+    mb = torch.zeros_like(pb)
+    va, vb = pa._version, pb._version
+    ops.muon_step([pa], [gr], [ma], 0.1)
+    ops.muon_step([pb], [gr.to(memory_format=torch.channels_last)], [mb], 0.1)
+    assert torch.equal(pa, pb) and torch.equal(ma, mb) and pa._version > va and pb._version > vb
+    assert pb.is_contiguous(memory_format=torch.channels_last)
+    # a saved weight that a step changed is noticed
+    w = torch.nn.Parameter(p0[:, :, 0, 0].clone())
+    y = (torch.randn(3, 8, device="cuda", requires_grad=True) @ w.t())
+    ops.muon_step([w], [gr[:, :, 0, 0]], [torch.zeros_like(w)], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@gpu
+def test_iterates_on_another_stream_and_in_a_graph():
+    from boostmvsnerfs_amd import ops
+    mats = [_grad(m, n, i).cuda() for i, (m, n) in enumerate([(8, 27), (128, 128), (140, 300)])]
+    params, momenta = [torch.randn_like(v) for v in mats], [torch.zeros_like(v) for v in mats]
+    want = [v.clone() for v in ops.newton_schulz(mats)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.newton_schulz(mats)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        out = ops.newton_schulz(mats)
+    with torch.cuda.graph(g2):
+        ops.muon_step(params, mats, momenta, 0.1, weight_decay=0.01)
+    for k in range(3):
+        for v in mats:
+            v.mul_(1 + k).add_(1e-3)
+        pe, me = [p.clone() for p in params], [m.clone() for m in momenta]
+        want = [v.clone() for v in ops.newton_schulz(mats)]
+        ops.muon_step(pe, mats, me, 0.1, weight_decay=0.01)
+        torch.cuda.synchronize()
+        g1.replay(), g2.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+        assert all(torch.equal(a, b) for a, b in zip(params + momenta, pe + me)), k
+
+
+def test_refusals():
+    from boostmvsnerfs_amd import ops
+    m = torch.zeros(4, 4)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.newton_schulz(m)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.muon_step([m], [m], [m], 0.1)
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        ops.newton_schulz([m.double()])
+    with pytest.raises(TypeError, match="expected a tensor"):
+        ops.newton_schulz([3.0])
+    with pytest.raises(ValueError, match="steps"):
+        ops.newton_schulz(m, steps=0)
+    with pytest.raises(ValueError, match="eps"):
+        ops.newton_schulz(m, eps=0.0)
+    with pytest.raises(ValueError, match="1 params, 2 grads"):
+        ops.muon_step([m], [m, m], [m], 0.1)
+    with pytest.raises(ValueError, match="scale"):
+        ops.muon_step([m], [m], [m], 0.1, scale="other")
+    with pytest.raises(ValueError, match="momentum"):
+        ops.muon_step([m], [m], [m], 0.1, momentum=1.0)
+
+
+def test_overlaps_are_refused_by_the_entry_points():
+    """Checked on the host, in front of any launch: addresses that are never read."""
+    import ctypes as C
+
+    from boostmvsnerfs_amd import _lib
+    lib = _lib.load()
+
+    def ptrs(*v):
+        return (C.c_void_p * len(v))(*v)
+    rows, cols, one = (C.c_int * 2)(4, 4), (C.c_int * 2)(8, 8), (C.c_float * 2)(1, 1)
+    A, B, G, M, N, W = 0x1000000, 0x2000000, 0x3000000, 0x4000000, 0x5000000, 0x6000000
+
+    def step(p, g, m):
+        return lib.bmv_muon_step(2, ptrs(*p), ptrs(*g), ptrs(*m), rows, cols, one, 0, 0.9, 1, 1.0, 5, *COEFFS, 1e-7, C.c_void_p(W), None)
+    for p, g, m in (((A, A), (G, G), (M, N)), ((A, A + 64), (G, G), (M, N)), ((A, B), (A, G), (M, N)), ((A, B), (G, G), (M, M)),
+                    ((A, B), (G, G), (M, B)), ((A, B), (G, M + 4), (M, N))):
+        assert step(p, g, m) == -1 and b"overlaps" in lib.bmv_last_error()
+    assert lib.bmv_newton_schulz(2, ptrs(A, B), ptrs(G, A), rows, cols, 0, 5, *COEFFS, 1e-7, C.c_void_p(W), None) == -1
+    assert b"overlaps" in lib.bmv_last_error()
+    assert lib.bmv_newton_schulz_workspace(1, (C.c_int * 1)(0), (C.c_int * 1)(4)) == -1
+    assert lib.bmv_newton_schulz(1, ptrs(A), ptrs(G), rows, cols, 7, 5, *COEFFS, 1e-7, C.c_void_p(W), None) == -1
+
+
+@gpu
+def test_refusals_on_the_gpu():
+    from boostmvsnerfs_amd import ops
+    m = torch.zeros(4, 4, device="cuda")
+    with pytest.raises(ValueError, match="matrix"):
+        ops.newton_schulz(m[0])
+    with pytest.raises(ValueError, match=r"grads\[0\]"):
+        ops.muon_step([m], [m.half()], [m], 0.1)
+    with pytest.raises(ValueError, match=r"momenta\[0\]"):
+        ops.muon_step([m], [m], [m.half()], 0.1)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ops.muon_step([m, m], [m.clone(), m.clone()], [m.clone(), m.clone()], 0.1)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ops.muon_step([m], [m], [m.clone()], 0.1)
