@@ -144,7 +144,7 @@ SIGNATURES = {
     "bmv_group_norm_workspace": [c_i, c_i, c_l, c_i, c_i, c_i, c_i],
     "bmv_group_norm_fwd": [c_f, c_f, c_f, c_i, c_i, c_l, c_i, c_i, c_i, c_i, C.c_double, c_i, c_fl, c_f, c_f, c_f, c_f, c_f],
     "bmv_group_norm_bwd": [c_f, c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_l, c_i, c_i, c_i, c_i, c_i, c_fl, c_f, c_f, c_f, c_f, c_f],
-    "bmv_newton_schulz_workspace": [c_i, C.POINTER(C.c_int), C.POINTER(C.c_int)],
+    "bmv_newton_schulz_workspace": [c_i, C.POINTER(C.c_int), C.POINTER(C.c_int), c_i],
     "bmv_newton_schulz": [c_i, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_int), C.POINTER(C.c_int), c_i, c_i, c_fl, c_fl,
                           c_fl, c_fl, c_f, c_f],
     "bmv_muon_step": [c_i, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_int), C.POINTER(C.c_int),

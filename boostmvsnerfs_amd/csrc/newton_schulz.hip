@@ -6,16 +6,24 @@
 //   Step: buf <- mu buf + (1 - mu) g,  U = (1 - mu) g + mu buf (Nesterov) or buf,  w <- w (1 - lr decay) - lr scale X.
 //
 // Numbers.  A near-zero singular value grows by a = 3.4 a step, and with it whatever error X carried in its direction: the
-// products need fp32 accuracy, whatever type the matrices have.  They run on the bf16 matrix cores with every fp32 operand as
+// products need more accuracy than the result's type has.  They run on the bf16 matrix cores with every fp32 operand as
 // three bf16 pieces (hi + mid + lo: its 24 significand bits exactly) and the six products that are not below 2^-25, sums in
 // fp32: 2.5 PFLOP/s / 6 against the 0.157 of the fp32 matrix instructions.  |U|_F is a 64-bit sum.
 //
-// Every operand is kept as its three pieces from the moment it is computed (one split per value, not one per use), in the
-// orientation in which its k axis is contiguous, so all three products are L R^T of row-major operands and LDS tiles are
-// filled by 16-byte DMA with no registers in between: A from X (k = n), A A from the symmetric A (k = m), Q X from Q and X^T
-// (k = m); X is therefore written in both orientations.  A and Q are symmetric: only tiles on and below the diagonal are
-// computed, the others are written as their transposes.
-// One launch per stage for the whole list: a workgroup finds its matrix and tile in a table of the kernel arguments.
+// bf16 matrices (half a step of a result: 2^-9) get two pieces (2^-17) and three products, half the work: what the steps make
+// of that error is a few 1e-4 of the result at most, beside 1.7e-3 that its one rounding costs.  fp16 (2^-12) keeps three.
+//
+// Layout.  Every operand is kept as its pieces from the moment it is computed (one split per value, not one per use), in the
+// orientation in which its k axis is contiguous, so all three products are L R^T: A from X (k = n), A A from the symmetric A
+// (k = m), Q X from Q and X^T (k = m); X is therefore written in both orientations.  And it is kept in the order in which the
+// products stage it: panels of 128 rows, in them blocks of 16 k-values, in a block piece after piece, 128 rows of 32 bytes.
+// What a stage of a product loads is one run of memory per operand, moved to LDS by 16-byte DMA with no registers and next to
+// no address arithmetic.  A and Q are symmetric: only tiles on and below the diagonal are computed.
+//
+// Work.  A product's tiles of 128 x 128 are as many workgroups while they fill the card; the rest (all of them, for matrices
+// of a few hundred) is cut along k into equal runs of stages over all compute units, whose partial tiles the joining launch
+// adds in a fixed order.  That launch also applies the polynomial, splits the values and writes both orientations.
+// A stage of the whole list is one launch: a workgroup finds its matrix in a table of the kernel arguments.
 #include <algorithm>
 #include <vector>
 
@@ -24,12 +32,16 @@
 namespace bmv {
 
 using nsb8 = __attribute__((ext_vector_type(8))) __bf16;
+using nsf4 = __attribute__((ext_vector_type(4))) float;
 using nsf16 = __attribute__((ext_vector_type(16))) float;
-using nsi4 = __attribute__((ext_vector_type(4))) int;
 
 constexpr int kNsList = 40;      // matrices per launch (the table travels in the kernel arguments)
 constexpr int kNsTile = 128;     // output tile of a workgroup; matrices are padded to it with zeros
-constexpr int kNsStrip = 512;    // columns of a preparing workgroup's strip of 64 rows
+constexpr int kNsK = 16;         // k-values of a stage
+constexpr int kNsCell = 2048;    // elements of a piece of a block: 128 rows of 16 k-values
+constexpr int kNsChunk = 8192;   // elements of a workgroup of the norm
+constexpr int kNsSlots = 512;    // workgroups that run at once: two on each of 256 compute units
+constexpr int kNsRun = 4;        // stages of the shortest run that a workgroup is started for
 
 struct NsItem {
   const void* src;      // U, or the gradient
@@ -38,13 +50,15 @@ struct NsItem {
   long ws;              // byte offset of this matrix' pieces in the workspace
   int rows, cols;       // of src / dst
   float scale;          // step: lr * scale of this matrix
-  int wg0;              // first workgroup of this matrix in the launch
+  int at;               // first workgroup / tile of this matrix in the launch
 };
 struct NsArgs {
   NsItem it[kNsList];
   char* ws;
-  double* sq;           // partial sums of squares: [item][strip], kNsList * sqn of them
-  int count, sqn, dtype, muon, nesterov, first, last, flip;
+  double* sq;           // partial sums of squares: [item][chunk], kNsList * sqn of them
+  float* part;          // partial tiles
+  int count, sqn, dtype, muon, nesterov, last, flip;
+  int full, run;        // a product's tiles that are a workgroup each; stages of a run of the others
   float a, b, c, eps, mu, nu, keep;      // nu: 1 - mu, rounded once
 };
 
@@ -59,20 +73,32 @@ struct NsShape {
   }
   __host__ __device__ long big() const { return (long)mp * np; }
   __host__ __device__ long sym() const { return (long)mp * mp; }
+  __host__ __device__ int mt() const { return mp / kNsTile; }
+  __host__ __device__ int nt() const { return np / kNsTile; }
+  __host__ __device__ long triangle() const { return (long)mt() * (mt() + 1) / 2; }
 };
-// the pieces of a matrix: plane p of an operand begins p * (elements of a plane) behind its first
+// the operands of a matrix, P pieces each
+template <int P>
 struct NsPlanes {
   __bf16 *x, *xt, *xt1, *a, *q;      // xt, xt1: X^T before and after a step, in turn
   __device__ NsPlanes(char* ws, const NsShape& s) {
     x = reinterpret_cast<__bf16*>(ws);
-    xt = x + 3 * s.big(), xt1 = xt + 3 * s.big(), a = xt1 + 3 * s.big(), q = a + 3 * s.sym();
+    xt = x + P * s.big(), xt1 = xt + P * s.big(), a = xt1 + P * s.big(), q = a + P * s.sym();
   }
 };
-static long ns_bytes(const NsShape& s) { return (9 * s.big() + 6 * s.sym()) * 2; }
+static long ns_bytes(const NsShape& s, int pieces) { return (3 * s.big() + 2 * s.sym()) * 2 * pieces; }
 
-__device__ __forceinline__ int ns_find(const NsArgs& g, int wg) {
+// the 8 k-values k ... k + 7 (k % 8 == 0) of row r, piece 0, of an operand with K k-values; piece q is kNsCell * q behind.
+// The two 16-byte cells of a row in a block are in turn swapped every 8 rows: the 16 lanes of a phase of ds_read_b128 (rows at
+// one k) then touch all 64 banks once.
+template <int P>
+__device__ __forceinline__ long ns_cell(int r, int k, int K) {
+  return ((long)(r >> 7) * (K / kNsK) + k / kNsK) * (P * kNsCell) + (r & 127) * kNsK + (((k >> 3) ^ (r >> 3)) & 1) * 8;
+}
+
+__device__ __forceinline__ int ns_find(const NsArgs& g, int at) {
   int i = 0;
-  while (i + 1 < g.count && g.it[i + 1].wg0 <= wg) ++i;
+  while (i + 1 < g.count && g.it[i + 1].at <= at) ++i;
   return __builtin_amdgcn_readfirstlane(i);
 }
 
@@ -99,40 +125,60 @@ __device__ __forceinline__ void ns_result(const NsArgs& g, const NsItem& it, lon
 }
 
 // x = p[0] + p[1] + p[2], exactly: every piece is the nearest bf16 to what the pieces before it leave (to nearest, not
-// truncated: what the dropped products of the pieces amount to is then below 2^-25 and of either sign, not 2^-21 of one)
-__device__ __forceinline__ void ns_split(float x, __bf16 p[3]) {
-  p[0] = (__bf16)x;
-  const float r = x - (float)p[0];
-  p[1] = (__bf16)r;
-  p[2] = (__bf16)(r - (float)p[1]);
-}
-// eight consecutive values as three 16-byte stores
-__device__ __forceinline__ void ns_store8(__bf16* p, long plane, const float* v) {
-  nsb8 o[3];
+// truncated: what the dropped products of the pieces amount to is then below 2^-25 and of either sign, not 2^-21 of one);
+// two pieces leave 2^-17 out.  Eight consecutive values as P 16-byte stores.
+template <int P>
+__device__ __forceinline__ void ns_store8(__bf16* p, const float* v) {
+  nsb8 o[P];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    __bf16 q[3];
-    ns_split(v[j], q);
+    float r = v[j];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) o[k][j] = q[k];
+    for (int q = 0; q < P; ++q) o[q][j] = (__bf16)r, r -= (float)o[q][j];
   }
 #pragma unroll
-  for (int k = 0; k < 3; ++k) *reinterpret_cast<nsb8*>(p + k * plane) = o[k];
+  for (int q = 0; q < P; ++q) *reinterpret_cast<nsb8*>(p + q * kNsCell) = o[q];
+}
+
+// A 64 x 64 block of values in LDS, rows r0 ..., columns c0 ... of a matrix, as cells of the operand whose k axis is the
+// columns (out, K = its columns) and of its transpose (outt, Kt); either may be null.
+constexpr int kNsPitch = 65;
+template <int P>
+__device__ __forceinline__ void ns_store_block(const float* t, int r0, int c0, __bf16* out, int K, __bf16* outt, int Kt) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int i = threadIdx.x + 256 * e, line = i >> 1 & 63, k = (i >> 7) * 16 + (i & 1) * 8;     // lanes along a block's run
+    float v[8];
+    if (out) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = t[line * kNsPitch + k + j];
+      ns_store8<P>(out + ns_cell<P>(r0 + line, c0 + k, K), v);
+    }
+    if (outt) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = t[(k + j) * kNsPitch + line];
+      ns_store8<P>(outt + ns_cell<P>(c0 + line, r0 + k, Kt), v);
+    }
+  }
 }
 
 // ---- the start: momentum and sum of squares; then scaled, split, both orientations --------------------------------------
 __global__ void __launch_bounds__(256) ns_norm_kernel(NsArgs g) {
   const int i = ns_find(g, blockIdx.x);
   const NsItem it = g.it[i];
-  const int wg = blockIdx.x - it.wg0, nc = (it.cols + kNsStrip - 1) / kNsStrip;
-  const int r0 = wg / nc * 64, c0 = wg % nc * kNsStrip;
-  const int r1 = min(r0 + 64, it.rows), c1 = min(c0 + kNsStrip, it.cols);
+  const int wg = blockIdx.x - it.at;
+  const long numel = (long)it.rows * it.cols, base = (long)wg * kNsChunk;
   double s = 0.;
-  for (int r = r0 + (threadIdx.x >> 6); r < r1; r += 4)
-    for (int c = c0 + (threadIdx.x & 63); c < c1; c += 64) {
-      const double v = (double)ns_start(g, it, (long)r * it.cols + c, true);
-      s += v * v;
+  for (int k = 0; k < kNsChunk / 256; k += 8) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const long at = base + (k + j) * 256 + threadIdx.x;
+      v[j] = at < numel ? ns_start(g, it, at, true) : 0.f;
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += (double)v[j] * (double)v[j];
+  }
   __shared__ double sh[4];
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
@@ -141,127 +187,133 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(NsArgs g) {
   if (threadIdx.x == 0) g.sq[(long)i * g.sqn + wg] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
 }
 
+template <int P>
 __global__ void __launch_bounds__(256) ns_split_kernel(NsArgs g) {
   const int i = ns_find(g, blockIdx.x);
   const NsItem it = g.it[i];
   const NsShape s(it.rows, it.cols);
-  const NsPlanes p(g.ws + it.ws, s);
-  const int wg = blockIdx.x - it.wg0, nt = s.np / 64;
+  const NsPlanes<P> p(g.ws + it.ws, s);
+  const int wg = blockIdx.x - it.at, nt = s.np / 64;
   const int k0 = wg / nt * 64, j0 = wg % nt * 64;       // rows and columns of X
-  __shared__ float tile[64][65];                         // [row of X][column of X]
+  __shared__ float tile[64 * kNsPitch];                  // [row of X][column of X]
   __shared__ double sh[4];
   double sq = 0.;
-  const int strips = ((it.rows + 63) / 64) * ((it.cols + kNsStrip - 1) / kNsStrip);
-  for (int k = threadIdx.x; k < strips; k += 256) sq += g.sq[(long)i * g.sqn + k];
+  const int chunks = (int)(((long)it.rows * it.cols + kNsChunk - 1) / kNsChunk);
+  for (int k = threadIdx.x; k < chunks; k += 256) sq += g.sq[(long)i * g.sqn + k];
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) sq += __shfl_xor(sq, m, 64);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = sq;
   __syncthreads();
   const double norm = sqrt((sh[0] + sh[1]) + (sh[2] + sh[3]));
   const float scale = (float)(1. / (norm > (double)g.eps || norm != norm ? norm : (double)g.eps));
+#pragma unroll 8
   for (int e = threadIdx.x; e < 64 * 64; e += 256) {
     const int hi = e >> 6, lo = e & 63;                  // the source's row and column inside the tile
     const int r = (s.tall ? j0 : k0) + hi, c = (s.tall ? k0 : j0) + lo;
     const float v = r < it.rows && c < it.cols ? ns_start(g, it, (long)r * it.cols + c, false) * scale : 0.f;
-    if (s.tall) tile[lo][hi] = v;
-    else tile[hi][lo] = v;
+    tile[s.tall ? lo * kNsPitch + hi : hi * kNsPitch + lo] = v;
   }
   __syncthreads();
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {                          // 64 lines of 8 pieces of 8 values, each way
-    const int line = (threadIdx.x >> 3) + 32 * e, at = (threadIdx.x & 7) * 8;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = tile[line][at + j];
-    ns_store8(p.x + (long)(k0 + line) * s.np + j0 + at, s.big(), v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = tile[at + j][line];
-    ns_store8(p.xt + (long)(j0 + line) * s.mp + k0 + at, s.big(), v);
-  }
+  ns_store_block<P>(tile, k0, j0, p.x, s.np, p.xt, s.mp);
 }
 
 // ---- the products --------------------------------------------------------------------------------------------------------
 enum { kNsGram = 0, kNsPoly = 1, kNsApply = 2 };
 
-// tile t of the lower triangle, row by row
-__device__ __forceinline__ void ns_triangle(int t, int& i, int& j) {
-  i = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-  while ((long)(i + 1) * (i + 2) / 2 <= t) ++i;
-  while ((long)i * (i + 1) / 2 > t) --i;
-  j = t - (int)((long)i * (i + 1) / 2);
+// Tile t of a product: super-rows of 8 tile rows, in them column by column, so that neighbouring workgroups (the 64 of an XCD
+// at a time) share 8 + 8 panels of operands in its L2.  Symmetric products: only columns up to the row.
+__device__ __forceinline__ void ns_tile(int t, const NsShape& s, bool symmetric, int& i, int& j) {
+  const int mt = s.mt();
+  if (!symmetric) {
+    const int per = 8 * s.nt(), sr = t / per, h = min(8, mt - 8 * sr);
+    t -= sr * per;
+    i = 8 * sr + t % h, j = t / h;
+    return;
+  }
+  int sr = 0;
+  while (32 * (sr + 1) * (sr + 1) + 4 * (sr + 1) <= t) ++sr;      // (tiles above super-row sr: 32 sr^2 + 4 sr)
+  t -= 32 * sr * sr + 4 * sr;
+  const int h = min(8, mt - 8 * sr);
+  if (t < 8 * sr * h) {
+    i = 8 * sr + t % h, j = t / h;
+    return;
+  }
+  t -= 8 * sr * h;
+  int col = 0;
+  while (t >= h - col) t -= h - col, ++col;
+  i = 8 * sr + col + t, j = 8 * sr + col;
 }
+__device__ __forceinline__ int ns_tiles(const NsShape& s, int stage) { return stage == kNsApply ? s.mt() * s.nt() : (int)s.triangle(); }
+__host__ __device__ __forceinline__ int ns_stages(const NsShape& s, int stage) { return (stage == kNsGram ? s.np : s.mp) / kNsK; }
 
-// A workgroup = 128 x 128 of L R^T, four waves of 64 x 64 (2 x 2 accumulators of v_mfma_f32_32x32x16_bf16); 32 k-values a
-// stage, two stages in LDS.  LDS tile of one operand piece: 128 rows of 64 bytes = 4 x 16-byte cells; the cell of k-octet o
-// of row r is o ^ (r >> 2 & 3), so that the 16 lanes of a phase of ds_read_b128 (16 rows, one octet) touch all 64 banks once.
-// The DMA writes lane l's 16 bytes at cell l: the swizzle is applied to the address that the lane reads from.
-constexpr int kNsPiece = kNsTile * 64;                    // bytes of one piece's tile
-constexpr int kNsStage = 6 * kNsPiece;                    // L and R, three pieces each
-constexpr int kNsPitch = kNsTile + 4;                     // floats: the finished tile in LDS
-constexpr int kNsLds = 2 * kNsStage > kNsTile * kNsPitch * 4 ? 2 * kNsStage : kNsTile * kNsPitch * 4;
-
-template <int STAGE>
-__global__ void __launch_bounds__(256, 1) ns_product_kernel(NsArgs g) {
-  extern __shared__ __align__(16) char lds[];
-  const int i = ns_find(g, blockIdx.x);
-  const NsItem it = g.it[i];
-  const NsShape s(it.rows, it.cols);
-  const NsPlanes p(g.ws + it.ws, s);
-  const int t = blockIdx.x - it.wg0;
-  int ti, tj;
-  if (STAGE == kNsApply) ti = t / (s.np / kNsTile), tj = t % (s.np / kNsTile);
-  else ns_triangle(t, ti, tj);
-  const int K = STAGE == kNsGram ? s.np : s.mp;
-  const __bf16* L = STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : p.q;
-  const __bf16* R = STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : (g.flip ? p.xt1 : p.xt);
-  const long lplane = STAGE == kNsGram ? s.big() : s.sym(), rplane = STAGE == kNsApply ? s.big() : lplane;
-  L += (long)ti * kNsTile * K, R += (long)tj * kNsTile * K;
-
+// A workgroup = 128 x 128 of L R^T, four waves of 64 x 64 (2 x 2 accumulators of v_mfma_f32_32x32x16_bf16, twice: hi hi goes to
+// accumulators of its own, because the other products are 2^-8 of it and adding them into the large sums would round those
+// once more for each).  Three stages of 16 k-values in LDS: one being multiplied, two on their way.  The finished tile leaves
+// in the order of the accumulators, 16 bytes a lane; the joining launch knows that order.
+template <int P, int STAGE>
+__global__ void __launch_bounds__(256, 2) ns_product_kernel(NsArgs g) {
+  constexpr int kStage = 2 * P * kNsCell;                 // elements: L's block, then R's
+  constexpr int kLoads = 2 * P * kNsCell * 2 / 1024 / 4;  // 1 KB DMAs of a wave for a stage
+  __shared__ __align__(16) __bf16 lds[3 * kStage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // DMA: wave w fills rows 16 (w + 4 h) .. + 15 (h = 0, 1) of each of the six tiles: lane -> row lane >> 2, cell lane & 3
-  const int drow = wave * 16 + (lane >> 2), dcell = (lane & 3) ^ (drow >> 2 & 3);
-  const long doff = (long)drow * K + dcell * 8;           // (row + 64: r >> 2 & 3 is the same)
-  auto fill = [&](int buf, int k) {
-#pragma unroll
-    for (int q = 0; q < 3; ++q)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        char* to = lds + buf * kNsStage + q * kNsPiece + (wave * 16 + h * 64) * 64;
-        const long off = doff + (long)h * 64 * K + k;
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(L + q * lplane + off),
-                                         (__attribute__((address_space(3))) void*)to, 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(R + q * rplane + off),
-                                         (__attribute__((address_space(3))) void*)(to + 3 * kNsPiece), 16, 0, 0);
+  const bool whole = (int)blockIdx.x < g.full;
+  // the unit range of this workgroup: unit = stage of a tile behind the whole ones
+  int t = whole ? xcd_contiguous(blockIdx.x, g.full) : g.full;
+  long skip = whole ? 0 : (long)(blockIdx.x - g.full) * g.run, left = whole ? 1l << 40 : g.run;
+  int i = ns_find(g, t);
+  while (left > 0) {
+    const NsItem it = g.it[i];
+    const NsShape s(it.rows, it.cols);
+    const int stages = ns_stages(s, STAGE), tiles = ns_tiles(s, STAGE);
+    if (!whole) {                                         // go to the tile that holds the next unit
+      const long jump = min(skip / stages, (long)(it.at + tiles - t));
+      t += (int)jump, skip -= jump * stages;
+      if (t >= it.at + tiles) {
+        if (++i >= g.count) return;
+        continue;
       }
-  };
-  const int lr = (wave >> 1) * 64 + (lane & 31), rr = (wave & 1) * 64 + (lane & 31), oct = lane >> 5;
-  auto read = [&](int buf, int operand, int q, int row, int o) {
-    return *reinterpret_cast<const nsb8*>(lds + buf * kNsStage + (operand * 3 + q) * kNsPiece + row * 64 + ((o ^ (row >> 2 & 3)) * 16));
-  };
-  // hi hi goes to accumulators of its own: the other five products are 2^-8 of it, and adding them into the large sums would
-  // round those six times instead of once per 16 k-values
-  nsf16 acc[2][2] = {}, low[2][2] = {};
-  fill(0, 0);
-  const int stages = K / 32;
-  for (int k = 0; k < stages; ++k) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this wave's part of stage k is in LDS
-    __syncthreads();                                      // everybody's, and nobody reads the other buffer any more
-    if (k + 1 < stages) fill((k + 1) & 1, (k + 1) * 32);
+    }
+    const int first = (int)skip, count = (int)min(left, (long)stages - first);
+    skip = 0, left -= whole ? left : count;
+    int ti, tj;
+    ns_tile(t - it.at, s, STAGE != kNsApply, ti, tj);
+    const NsPlanes<P> p(g.ws + it.ws, s);
+    const __bf16* L = STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : p.q;
+    const __bf16* R = STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : (g.flip ? p.xt1 : p.xt);
+    L += ((long)ti * stages + first) * (P * kNsCell), R += ((long)tj * stages + first) * (P * kNsCell);
+    auto fill = [&](int k) {                              // stage k into buffer k % 3
+      __bf16* to = lds + k % 3 * kStage;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      nsb8 lf[2][3], rf[2][3];
+      for (int h = 0; h < kLoads; ++h) {
+        const int c = wave + 4 * h, off = c % (kLoads * 2) * 512;      // (1 KB = 512 elements; L's first, then R's)
+        const __bf16* from = (c < kLoads * 2 ? L : R) + (long)k * (P * kNsCell) + off;
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + lane * 8),
+                                         (__attribute__((address_space(3))) void*)(to + c * 512), 16, 0, 0);
+      }
+    };
+    const int lr = (wave >> 1) * 64 + (lane & 31), rr = (wave & 1) * 64 + (lane & 31), oct = lane >> 5;
+    auto read = [&](int k, int operand, int q, int row) {
+      return *reinterpret_cast<const nsb8*>(lds + k % 3 * kStage + (operand * P + q) * kNsCell + row * kNsK + ((oct ^ row >> 3) & 1) * 8);
+    };
+    nsf16 acc[2][2] = {}, low[2][2] = {};
+    fill(0);
+    if (count > 1) fill(1);
+    for (int k = 0; k < count; ++k) {
+      // this wave's part of stage k is in LDS (of the newer loads only those of stage k + 1 may be on their way), then
+      // everybody's, and nobody reads stage k - 1 any more
+      if (k + 1 < count) asm volatile("s_waitcnt vmcnt(%0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (k + 2 < count) fill(k + 2);
+      nsb8 lf[2][P], rf[2][P];
 #pragma unroll
-      for (int q = 0; q < 3; ++q)
+      for (int q = P - 1; q >= 0; --q)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          lf[e][q] = read(k & 1, 0, q, lr + 32 * e, half * 2 + oct);
-          rf[e][q] = read(k & 1, 1, q, rr + 32 * e, half * 2 + oct);
-        }
-      // the six products, small ones first
+        for (int e = 0; e < 2; ++e) lf[e][q] = read(k, 0, q, lr + 32 * e), rf[e][P - 1 - q] = read(k, 1, P - 1 - q, rr + 32 * e);
+      // the products of pieces whose numbers add up to at most P - 1, small ones first
 #pragma unroll
-      for (int sum = 2; sum >= 0; --sum)
+      for (int sum = P - 1; sum >= 0; --sum)
 #pragma unroll
-        for (int q = 0; q <= sum; ++q)
+        for (int q = sum; q >= 0; --q)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -269,65 +321,102 @@ __global__ void __launch_bounds__(256, 1) ns_product_kernel(NsArgs g) {
               if (sum) low[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[e][q], rf[f][sum - q], low[e][f], 0, 0, 0);
               else acc[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[e][q], rf[f][sum - q], acc[e][f], 0, 0, 0);
     }
+    // slot: a whole tile's number; behind those, run + tile, which grows by one from each run's piece of a tile to the next
+    const long slot = whole ? t : t + (long)(blockIdx.x - g.full);
+    nsf4* out = reinterpret_cast<nsf4*>(g.part) + slot * (kNsTile * kNsTile / 4) + threadIdx.x;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int f = 0; f < 2; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          nsf4 v;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = acc[e][f][4 * r + j] + low[e][f][4 * r + j];
+          out[((e * 2 + f) * 4 + r) * 256] = v;
+        }
+    if (whole) return;
+    // (the next tile's first stages go over this one's, and its waits count loads alone)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (++t >= it.at + tiles) {
+      if (++i >= g.count) return;
+    }
   }
+}
+
+// A workgroup = a wave's 64 x 64 quarter of a tile: its partial sums in the order of the runs, then the polynomial
+// (kNsPoly), then both orientations as pieces, or the result.
+template <int P, int STAGE>
+__global__ void __launch_bounds__(256) ns_join_kernel(NsArgs g) {
+  __shared__ float tile[64 * kNsPitch];
+  const int t = blockIdx.x >> 2, quarter = blockIdx.x & 3, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int i = ns_find(g, t);
+  const NsItem it = g.it[i];
+  const NsShape s(it.rows, it.cols);
+  const NsPlanes<P> p(g.ws + it.ws, s);
+  int ti, tj;
+  ns_tile(t - it.at, s, STAGE != kNsApply, ti, tj);
+  // the slots that hold this tile: its own number, or one for each run that has stages of it
+  long lo = t, hi = t;
+  if (t >= g.full) {
+    long unit = 0;                                        // the tile's first unit
+    for (int k = 0; k < i; ++k) {
+      const NsShape o(g.it[k].rows, g.it[k].cols);
+      const int begin = max(g.it[k].at, g.full), end = g.it[k].at + ns_tiles(o, STAGE);
+      if (end > begin) unit += (long)(end - begin) * ns_stages(o, STAGE);
+    }
+    const int stages = ns_stages(s, STAGE);
+    unit += (long)(t - max(it.at, g.full)) * stages;
+    lo = t + unit / g.run, hi = t + (unit + stages - 1) / g.run;
+  }
+  const nsf4* part = reinterpret_cast<const nsf4*>(g.part) + quarter * 64 + lane;
+  nsf4 v[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = part[lo * (kNsTile * kNsTile / 4) + (wave * 4 + r) * 256];
+  for (long k = lo + 1; k <= hi; ++k)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] += part[k * (kNsTile * kNsTile / 4) + (wave * 4 + r) * 256];
+  // accumulator register 4 r + j of lane l: row 8 r + 4 (l >> 5) + j, column l & 31 of the 32 x 32 block (wave >> 1, wave & 1)
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      tile[((wave >> 1) * 32 + 8 * r + 4 * (lane >> 5) + j) * kNsPitch + (wave & 1) * 32 + (lane & 31)] = v[r][j];
   __syncthreads();
-  // the tile into LDS (accumulator register r of lane l: row 8 (r >> 2) + 4 (l >> 5) + (r & 3), column l & 31)
-  float* tile = reinterpret_cast<float*>(lds);
-#pragma unroll
-  for (int e = 0; e < 2; ++e)
-#pragma unroll
-    for (int f = 0; f < 2; ++f)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int row = (wave >> 1) * 64 + e * 32 + 8 * (r >> 2) + 4 * oct + (r & 3);
-        tile[row * kNsPitch + (wave & 1) * 64 + f * 32 + (lane & 31)] = acc[e][f][r] + low[e][f][r];
-      }
-  __syncthreads();
-  const int row0 = ti * kNsTile, col0 = tj * kNsTile;
+  const int row0 = ti * kNsTile + (quarter >> 1) * 64, col0 = tj * kNsTile + (quarter & 1) * 64;
   if (STAGE == kNsPoly) {                                 // a I + b A + c A A, in place
-    for (int e = threadIdx.x; e < kNsTile * kNsTile / 8; e += 256) {
-      const int r = e >> 4, c = (e & 15) * 8;
-      const __bf16* ap = p.a + (long)(row0 + r) * s.mp + col0 + c;
-      const nsb8 h = *reinterpret_cast<const nsb8*>(ap), m = *reinterpret_cast<const nsb8*>(ap + s.sym()),
-                 l = *reinterpret_cast<const nsb8*>(ap + 2 * s.sym());
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int k = threadIdx.x + 256 * e, r = k >> 1 & 63, c = (k >> 7) * 16 + (k & 1) * 8;
+      const __bf16* ap = p.a + ns_cell<P>(row0 + r, col0 + c, s.mp);
+      float av[8] = {};
+#pragma unroll
+      for (int q = P - 1; q >= 0; --q) {
+        const nsb8 piece = *reinterpret_cast<const nsb8*>(ap + q * kNsCell);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) av[j] += (float)piece[j];
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float av = ((float)h[j] + (float)m[j]) + (float)l[j];
-        float v = g.b * av + g.c * tile[r * kNsPitch + c + j];
-        if (row0 + r == col0 + c + j && row0 + r < s.m) v += g.a;
-        tile[r * kNsPitch + c + j] = v;
+        float* to = tile + r * kNsPitch + c + j;
+        *to = g.b * av[j] + g.c * *to + (row0 + r == col0 + c + j && row0 + r < s.m ? g.a : 0.f);
       }
     }
     __syncthreads();
   }
   if (STAGE == kNsApply && g.last) {
-    for (int e = threadIdx.x; e < kNsTile * kNsTile; e += 256) {
-      const int hi = e >> 7, lo = e & 127;                // row and column of the source inside the tile
-      const int r = (s.tall ? col0 : row0) + hi, c = (s.tall ? row0 : col0) + lo;
-      if (r < it.rows && c < it.cols) ns_result(g, it, (long)r * it.cols + c, s.tall ? tile[lo * kNsPitch + hi] : tile[hi * kNsPitch + lo]);
+#pragma unroll 4
+    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+      const int hi_ = e >> 6, lo_ = e & 63;               // row and column of the source inside the block
+      const int r = (s.tall ? col0 : row0) + hi_, c = (s.tall ? row0 : col0) + lo_;
+      if (r < it.rows && c < it.cols)
+        ns_result(g, it, (long)r * it.cols + c, tile[s.tall ? lo_ * kNsPitch + hi_ : hi_ * kNsPitch + lo_]);
     }
     return;
   }
-  // both orientations, as pieces
   __bf16* out = STAGE == kNsGram ? p.a : STAGE == kNsPoly ? p.q : p.x;
-  __bf16* outt = STAGE == kNsApply ? (g.flip ? p.xt : p.xt1) : out;
-  const int pitch = STAGE == kNsApply ? s.np : s.mp;
-  const long plane = STAGE == kNsApply ? s.big() : s.sym();
-  for (int e = threadIdx.x; e < kNsTile * kNsTile / 8; e += 256) {
-    const int r = e >> 4, c = (e & 15) * 8;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = tile[r * kNsPitch + c + j];
-    ns_store8(out + (long)(row0 + r) * pitch + col0 + c, plane, v);
-  }
-  if (STAGE != kNsApply && ti == tj) return;
-  for (int e = threadIdx.x; e < kNsTile * kNsTile / 8; e += 256) {
-    const int c = e >> 4, r = (e & 15) * 8;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = tile[(r + j) * kNsPitch + c];
-    ns_store8(outt + (long)(col0 + c) * s.mp + row0 + r, plane, v);
-  }
+  if (STAGE == kNsApply) ns_store_block<P>(tile, row0, col0, out, s.np, g.flip ? p.xt : p.xt1, s.mp);
+  else ns_store_block<P>(tile, row0, col0, out, s.mp, ti == tj ? nullptr : out, s.mp);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -360,65 +449,74 @@ static bool ns_apart(int count, const int* rows, const int* cols, int size, cons
   }
   return true;
 }
-static int ns_strips(int rows, int cols) { return ((rows + 63) / 64) * ((cols + kNsStrip - 1) / kNsStrip); }
+static int ns_chunks(int rows, int cols) { return (int)(((long)rows * cols + kNsChunk - 1) / kNsChunk); }
 
-// the list in runs of kNsList; a run's pieces share the workspace with the next run's
-static long ns_workspace(int count, const int* rows, const int* cols) {
-  long most = 0;
-  for (int b = 0; b < count; b += kNsList) {
-    long bytes = 0;
-    int sqn = 1;
-    for (int i = b; i < count && i < b + kNsList; ++i) {
-      bytes += ns_bytes(NsShape(rows[i], cols[i]));
-      if (ns_strips(rows[i], cols[i]) > sqn) sqn = ns_strips(rows[i], cols[i]);
+// workspace of matrices b ... e - 1: pieces, then the norm's partial sums, then partial tiles
+struct NsRoom {
+  long pieces = 0, tiles = 0;
+  int sqn = 1;
+  NsRoom(const int* rows, const int* cols, int b, int e, int p) {
+    for (int i = b; i < e; ++i) {
+      const NsShape s(rows[i], cols[i]);
+      pieces += ns_bytes(s, p), tiles += (long)s.mt() * s.nt();      // (no fewer than the symmetric products')
+      sqn = std::max(sqn, ns_chunks(rows[i], cols[i]));
     }
-    bytes += (long)kNsList * sqn * sizeof(double);
-    if (bytes > most) most = bytes;
   }
+  long bytes() const { return pieces + (long)kNsList * sqn * sizeof(double) + (tiles + kNsSlots) * (kNsTile * kNsTile * 4l); }
+};
+// a list is done in parts of kNsList, which share the workspace
+static long ns_workspace(int count, const int* rows, const int* cols, int dtype) {
+  long most = 0;
+  for (int b = 0; b < count; b += kNsList)
+    most = std::max(most, NsRoom(rows, cols, b, std::min(count, b + kNsList), dtype == 1 ? 2 : 3).bytes());
   return most;
 }
 
-static int ns_run(NsArgs g, int count, const void* const* src, void* const* dst, float* const* buf, const int* rows,
-                  const int* cols, const float* scales, int steps, char* ws, hipStream_t st) {
-  static const bool ready = [] {      // (96 KB of LDS: above what a kernel gets without asking)
-    const void* k[3] = {(const void*)ns_product_kernel<kNsGram>, (const void*)ns_product_kernel<kNsPoly>, (const void*)ns_product_kernel<kNsApply>};
-    for (const void* f : k)
-      if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kNsLds) != hipSuccess) return false;
-    return true;
-  }();
-  if (!ready) return -1;
+template <int P, int STAGE>
+static void ns_product(NsArgs& g, hipStream_t st) {
+  long tiles = 0, units = 0;
+  for (int i = 0; i < g.count; ++i) {
+    const NsShape s(g.it[i].rows, g.it[i].cols);
+    g.it[i].at = (int)tiles;
+    tiles += STAGE == kNsApply ? (long)s.mt() * s.nt() : s.triangle();
+  }
+  g.full = (int)(tiles / kNsSlots * kNsSlots);
+  for (int i = 0; i < g.count; ++i) {
+    const NsShape s(g.it[i].rows, g.it[i].cols);
+    const long end = i + 1 < g.count ? g.it[i + 1].at : tiles, begin = std::max<long>(g.it[i].at, g.full);
+    if (end > begin) units += (end - begin) * ns_stages(s, STAGE);
+  }
+  g.run = std::max<long>((units + kNsSlots - 1) / kNsSlots, kNsRun);
+  hipLaunchKernelGGL((ns_product_kernel<P, STAGE>), dim3((unsigned)(g.full + (units + g.run - 1) / g.run)), dim3(256), 0, st, g);
+  hipLaunchKernelGGL((ns_join_kernel<P, STAGE>), dim3((unsigned)(4 * tiles)), dim3(256), 0, st, g);
+}
+
+template <int P>
+static void ns_run(NsArgs g, int count, const void* const* src, void* const* dst, float* const* buf, const int* rows,
+                   const int* cols, const float* scales, int steps, char* ws, hipStream_t st) {
   for (int b = 0; b < count; b += kNsList) {
-    g.count = count - b < kNsList ? count - b : kNsList;
-    long off = 0;
-    g.sqn = 1;
+    g.count = std::min(count - b, kNsList);
+    const NsRoom room(rows, cols, b, b + g.count, P);
+    g.ws = ws, g.sqn = room.sqn, g.sq = reinterpret_cast<double*>(ws + room.pieces);
+    g.part = reinterpret_cast<float*>(g.sq + (long)kNsList * g.sqn);
+    long off = 0, chunks = 0;
     for (int i = 0; i < g.count; ++i) {
       NsItem& it = g.it[i];
       it.src = src[b + i], it.dst = dst[b + i], it.buf = buf ? buf[b + i] : nullptr, it.rows = rows[b + i], it.cols = cols[b + i];
-      it.scale = scales ? scales[b + i] : 1.f, it.ws = off;
-      off += ns_bytes(NsShape(it.rows, it.cols));
-      if (ns_strips(it.rows, it.cols) > g.sqn) g.sqn = ns_strips(it.rows, it.cols);
+      it.scale = scales ? scales[b + i] : 1.f, it.ws = off, it.at = (int)chunks;
+      off += ns_bytes(NsShape(it.rows, it.cols), P), chunks += ns_chunks(it.rows, it.cols);
     }
-    g.ws = ws, g.sq = reinterpret_cast<double*>(ws + off);
-    // workgroups of the launch: fills wg0
-    auto table = [&](auto&& wgs) {
-      long n = 0;
-      for (int i = 0; i < g.count; ++i) g.it[i].wg0 = (int)n, n += wgs(g.it[i], NsShape(g.it[i].rows, g.it[i].cols));
-      return dim3((unsigned)n);
-    };
-    const dim3 block(256);
-    hipLaunchKernelGGL(ns_norm_kernel, table([](const NsItem& it, const NsShape&) { return (long)ns_strips(it.rows, it.cols); }), block, 0, st, g);
-    hipLaunchKernelGGL(ns_split_kernel, table([](const NsItem&, const NsShape& s) { return s.big() / (64 * 64); }), block, 0, st, g);
-    auto triangle = [](const NsItem&, const NsShape& s) { return (long)(s.mp / kNsTile) * (s.mp / kNsTile + 1) / 2; };
+    hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)chunks), dim3(256), 0, st, g);
+    long blocks = 0;
+    for (int i = 0; i < g.count; ++i) g.it[i].at = (int)blocks, blocks += NsShape(g.it[i].rows, g.it[i].cols).big() / (64 * 64);
+    hipLaunchKernelGGL(ns_split_kernel<P>, dim3((unsigned)blocks), dim3(256), 0, st, g);
     for (int k = 0; k < steps; ++k) {
       g.last = k + 1 == steps, g.flip = k & 1;
-      dim3 grid = table(triangle);
-      hipLaunchKernelGGL(ns_product_kernel<kNsGram>, grid, block, kNsLds, st, g);
-      hipLaunchKernelGGL(ns_product_kernel<kNsPoly>, grid, block, kNsLds, st, g);
-      grid = table([](const NsItem&, const NsShape& s) { return s.big() / (kNsTile * kNsTile); });
-      hipLaunchKernelGGL(ns_product_kernel<kNsApply>, grid, block, kNsLds, st, g);
+      ns_product<P, kNsGram>(g, st);
+      ns_product<P, kNsPoly>(g, st);
+      ns_product<P, kNsApply>(g, st);
     }
   }
-  return 0;
 }
 
 }  // namespace bmv
@@ -427,10 +525,11 @@ using namespace bmv;
 
 extern "C" {
 
-long bmv_newton_schulz_workspace(int count, const int* rows, const int* cols) {
+long bmv_newton_schulz_workspace(int count, const int* rows, const int* cols, int dtype) {
   const char* bad = ns_bad(count, rows, cols);
   BMV_REQUIRE(!bad, "bmv_newton_schulz_workspace: %s", bad);
-  return ns_workspace(count, rows, cols);
+  BMV_REQUIRE(dtype >= 0 && dtype <= 2, "bmv_newton_schulz_workspace: unknown type %d", dtype);
+  return ns_workspace(count, rows, cols, dtype);
 }
 
 int bmv_newton_schulz(int count, const void* const* src, void* const* dst, const int* rows, const int* cols, int dtype, int steps,
@@ -445,8 +544,8 @@ int bmv_newton_schulz(int count, const void* const* src, void* const* dst, const
   BMV_REQUIRE(ns_apart(count, rows, cols, dtype == 0 ? 4 : 2, src, dst, nullptr), "bmv_newton_schulz: a result overlaps another matrix");
   NsArgs g{};
   g.dtype = dtype, g.a = a, g.b = b, g.c = c, g.eps = eps;
-  BMV_REQUIRE(ns_run(g, count, src, dst, nullptr, rows, cols, nullptr, steps, static_cast<char*>(workspace), as_stream(stream)) == 0,
-              "bmv_newton_schulz: %d bytes of LDS refused", kNsLds);
+  if (dtype != 1) ns_run<3>(g, count, src, dst, nullptr, rows, cols, nullptr, steps, static_cast<char*>(workspace), as_stream(stream));
+  else ns_run<2>(g, count, src, dst, nullptr, rows, cols, nullptr, steps, static_cast<char*>(workspace), as_stream(stream));
   BMV_LAUNCH_END("bmv_newton_schulz");
 }
 
@@ -465,8 +564,8 @@ int bmv_muon_step(int count, void* const* params, const void* const* grads, floa
               "bmv_muon_step: a weight or a momentum overlaps another tensor (is one listed twice?)");
   NsArgs g{};
   g.dtype = dtype, g.a = a, g.b = b, g.c = c, g.eps = eps, g.muon = 1, g.nesterov = nesterov, g.mu = (float)momentum, g.nu = (float)(1. - momentum), g.keep = (float)keep;
-  BMV_REQUIRE(ns_run(g, count, grads, params, momenta, rows, cols, scales, steps, static_cast<char*>(workspace), as_stream(stream)) == 0,
-              "bmv_muon_step: %d bytes of LDS refused", kNsLds);
+  if (dtype != 1) ns_run<3>(g, count, grads, params, momenta, rows, cols, scales, steps, static_cast<char*>(workspace), as_stream(stream));
+  else ns_run<2>(g, count, grads, params, momenta, rows, cols, scales, steps, static_cast<char*>(workspace), as_stream(stream));
   BMV_LAUNCH_END("bmv_muon_step");
 }
 

@@ -1525,8 +1525,8 @@ def _pointers(tensors):
     return (C.c_void_p * len(tensors))(*[_addr(t) for t in tensors])
 
 
-def _ns_workspace(lib, count, rows, cols, device):
-    n = lib.bmv_newton_schulz_workspace(count, rows, cols)
+def _ns_workspace(lib, count, rows, cols, dtype, device):
+    n = lib.bmv_newton_schulz_workspace(count, rows, cols, _FLOAT_CODES[dtype])
     if n < 0:
         _lib.check(int(n), "newton_schulz_workspace")
     return torch.empty(n, device=device, dtype=torch.uint8)
@@ -1536,7 +1536,7 @@ def newton_schulz(mats, steps=5, coeffs=NS_COEFFS, eps=NS_EPS):
     """Orthogonalise matrices: X = M / max(|M|_F, eps), then `steps` times A = X X^T, X = a X + (b A + c A A) X with
     `coeffs` = (a, b, c) -- singular values towards 1, singular vectors kept.  `mats`: a tensor, or a list of tensors (one set
     of launches for all), of 2 dimensions or more (what is behind the first is flattened: convolution kernels), fp32, bf16 or
-    fp16.  Computed at fp32 accuracy whatever the type.  -> new tensors of the same shapes and types."""
+    fp16.  Computed at fp32 accuracy (bf16: with 17-bit operands).  -> new tensors of the same shapes and types."""
     if torch.is_tensor(mats):
         return newton_schulz([mats], steps, coeffs, eps)[0]
     mats = list(mats)
@@ -1548,7 +1548,7 @@ def newton_schulz(mats, steps=5, coeffs=NS_COEFFS, eps=NS_EPS):
         with _on_device_of(mats[idx[0]]):
             n = len(idx)
             rows, cols = (C.c_int * n)(*[sizes[i][0] for i in idx]), (C.c_int * n)(*[sizes[i][1] for i in idx])
-            ws = _ns_workspace(lib, n, rows, cols, device)
+            ws = _ns_workspace(lib, n, rows, cols, dtype, device)
             with ktimer.region("newton_schulz"):
                 rc = lib.bmv_newton_schulz(n, _pointers([_c(mats[i]) for i in idx]), _pointers([out[i] for i in idx]), rows, cols,
                                            _FLOAT_CODES[dtype], steps, a, b, c, eps, _addr(ws), stream())
@@ -1594,7 +1594,7 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
             rows, cols = (C.c_int * n)(*[sizes[i][0] for i in idx]), (C.c_int * n)(*[sizes[i][1] for i in idx])
             scales = (C.c_float * n)(*[lr * MUON_SCALES[scale](*sizes[i]) for i in idx])
             p, m = [_c(params[i]) for i in idx], [_c(momenta[i]) for i in idx]
-            ws = _ns_workspace(lib, n, rows, cols, device)
+            ws = _ns_workspace(lib, n, rows, cols, dtype, device)
             with ktimer.region("muon_step"):
                 rc = lib.bmv_muon_step(n, _pointers(p), _pointers([_c(grads[i]) for i in idx]), _pointers(m), rows, cols, scales,
                                        _FLOAT_CODES[dtype], float(momentum), int(bool(nesterov)), keep, steps, a, b, c, eps,

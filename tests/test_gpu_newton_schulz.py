@@ -6,7 +6,11 @@ below 3 x 2^-24 of a term, then fp32 sums) is off by at most eps_k |L|_F |R|_F w
 rounding of each operand, of the result, and k roundings of partial sums of random sign.  A step turns errors of its three products
 into at most (|b| + 2 |c| |A|) dA |X| + |c| d(AA) |X| + d(QX) of X, and an error of X into at most L of it, L = max |p'| of the
 polynomial p = a s + b s^3 + c s^5 over the iterate's singular values (of the divided differences as well, which p' bounds).
-That sum is computed along the 64-bit iteration; bf16 and fp16 results add half a step of their rounding."""
+That sum is computed along the 64-bit iteration; bf16 and fp16 results add half a step of their rounding.
+
+For bf16 matrices the operands have two pieces: each is off by at most 2^-18 of itself, and mid mid (2^-18) is dropped, so a term
+l r is off by at most 3 x 2^-18 of itself, of random sign: a product by 3 x 2^-18 sqrt(sum_k |l_k|^2 |r_k|^2) over the columns
+l_k, r_k (twice that is allowed: in X X^T the same rounding stands on both sides)."""
 import math
 
 import pytest
@@ -16,16 +20,21 @@ gpu = pytest.mark.gpu
 COEFFS = (3.4445, -4.7750, 2.0315)
 
 
-def _iterate(u, steps=5, coeffs=COEFFS, eps=1e-7):
-    """(the iterate, its tolerance in the Frobenius norm) of u, in 64 bits."""
+def _iterate(u, steps=5, coeffs=COEFFS, eps=1e-7, two=False):
+    """(the iterate, its tolerance in the Frobenius norm) of u, in 64 bits; `two`: with operands of two pieces."""
     a, b, c = coeffs
+    two = two or u.dtype == torch.bfloat16
     u = u.double()
     x = u / max(float(u.norm()), eps)
     tall = x.shape[0] > x.shape[1]
     x = x.mT if tall else x
     m, n = x.shape
     unit = 2.0 ** -24
-    ek = lambda k: unit * (4 + 2 * math.sqrt(k))       # noqa: E731
+
+    def off(l, r):                                     # of l r, the columns of l against the rows of r
+        k = l.shape[1]
+        d = unit * (4 + 2 * math.sqrt(k)) * float(l.norm()) * float(r.norm())
+        return d + (6 * 2.0 ** -18 * float((l.norm(dim=0) * r.norm(dim=1)).norm()) if two else 0.0)
     tol = 2 * unit * float(x.norm())
     for _ in range(steps):
         A = x @ x.mT
@@ -33,8 +42,8 @@ def _iterate(u, steps=5, coeffs=COEFFS, eps=1e-7):
         s = max(float(torch.linalg.matrix_norm(x, 2)), 1e-300)
         grid = torch.linspace(0, s, 200, dtype=torch.float64)
         lip = float((a + 3 * b * grid ** 2 + 5 * c * grid ** 4).abs().max())
-        dA, dAA = ek(n) * float(x.norm()) ** 2, ek(m) * float(A.norm()) ** 2
-        local = ((abs(b) + 2 * abs(c) * s * s) * dA + abs(c) * dAA) * s + ek(m) * float(Q.norm()) * float(x.norm())
+        dA, dAA = off(x, x.mT), off(A, A)
+        local = ((abs(b) + 2 * abs(c) * s * s) * dA + abs(c) * dAA) * s + off(Q, x)
         tol = lip * tol + local
         x = Q @ x
     return (x.mT if tall else x), tol
@@ -178,7 +187,7 @@ def test_muon_step_matches_the_formula(dtype, nesterov, scale, decay):
             off = (mn.double().cpu() - moved).abs() - 4 * 2.0 ** -24 * ((mu * md).abs() + ((1 - mu) * gd).abs()) - 1e-40
             assert float(off.max()) <= 0, (tuple(p.shape), float(off.max()))
             u = ((1 - mu) * gd + mu * moved if nesterov else moved).flatten(1)
-            o, tol = _iterate(u)
+            o, tol = _iterate(u, two=dtype == torch.bfloat16)
             rows, cols = u.shape
             s = {"shape": math.sqrt(max(1, rows / cols)), "rms": 0.2 * math.sqrt(max(rows, cols)), "none": 1.0}[scale]
             want = p.double().flatten(1) * (1 - lr * decay) - lr * s * o
@@ -285,7 +294,7 @@ def test_overlaps_are_refused_by_the_entry_points():
         assert step(p, g, m) == -1 and b"overlaps" in lib.bmv_last_error()
     assert lib.bmv_newton_schulz(2, ptrs(A, B), ptrs(G, A), rows, cols, 0, 5, *COEFFS, 1e-7, C.c_void_p(W), None) == -1
     assert b"overlaps" in lib.bmv_last_error()
-    assert lib.bmv_newton_schulz_workspace(1, (C.c_int * 1)(0), (C.c_int * 1)(4)) == -1
+    assert lib.bmv_newton_schulz_workspace(1, (C.c_int * 1)(0), (C.c_int * 1)(4), 0) == -1
     assert lib.bmv_newton_schulz(1, ptrs(A), ptrs(G), rows, cols, 7, 5, *COEFFS, 1e-7, C.c_void_p(W), None) == -1
 
 
