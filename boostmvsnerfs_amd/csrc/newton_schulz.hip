@@ -24,7 +24,10 @@
 // of a few hundred) is cut along k into equal runs of stages over all compute units, whose partial tiles the joining launch
 // adds in a fixed order.  That launch also applies the polynomial, splits the values and writes both orientations.
 // A stage of the whole list is one launch: a workgroup finds its matrix in a table of the kernel arguments.
+//
+// Matrices with a short side of up to 128 (every layer of the networks here) go another way, one launch a step: see below.
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "bmv_common.hpp"
@@ -57,7 +60,7 @@ struct NsArgs {
   char* ws;
   double* sq;           // partial sums of squares: [item][chunk], kNsList * sqn of them
   float* part;          // partial tiles
-  int count, sqn, dtype, muon, nesterov, last, flip;
+  int count, sqn, dtype, muon, nesterov, first, last, flip;
   int full, run;        // a product's tiles that are a workgroup each; stages of a run of the others
   float a, b, c, eps, mu, nu, keep;      // nu: 1 - mu, rounded once
 };
@@ -96,10 +99,11 @@ __device__ __forceinline__ long ns_cell(int r, int k, int K) {
   return ((long)(r >> 7) * (K / kNsK) + k / kNsK) * (P * kNsCell) + (r & 127) * kNsK + (((k >> 3) ^ (r >> 3)) & 1) * 8;
 }
 
+// the matrix that holds `at`: the last whose first is not behind it (one load a lane instead of a chain of them)
 __device__ __forceinline__ int ns_find(const NsArgs& g, int at) {
-  int i = 0;
-  while (i + 1 < g.count && g.it[i + 1].at <= at) ++i;
-  return __builtin_amdgcn_readfirstlane(i);
+  static_assert(kNsList <= 64, "a lane each");
+  const int lane = threadIdx.x & 63;
+  return __popcll(__ballot(lane < g.count && g.it[min(lane, kNsList - 1)].at <= at)) - 1;
 }
 
 __device__ __forceinline__ float ns_read(const void* p, long i, int dtype) {
@@ -419,6 +423,194 @@ __global__ void __launch_bounds__(256) ns_join_kernel(NsArgs g) {
   else ns_store_block<P>(tile, row0, col0, out, s.mp, ti == tj ? nullptr : out, s.mp);
 }
 
+// ---- short sides of up to 128 ------------------------------------------------------------------------------------------------
+// A step of such a matrix is launches, not work: the three products and their joins are six launches of 3 to 6 us each that
+// leave the card nearly empty.  Here a workgroup owns T columns of X for all steps (X^T and A in LDS, fp32) and a step is ONE
+// launch: it adds up the other workgroups' shares of A = X X^T, takes Y = A X and X <- a X + b Y + c A Y of its columns
+// (2 m^2 T operations twice instead of m^3 and 2 m^2 T: A A would be computed by every workgroup again), and leaves its
+// share of the next A.  |U|_F^2 is the trace of the first A: no launch of its own.  fp32 matrix instructions (16x16x4): the
+// products are too small for the split of the operands to pay.
+// LDS rows are m + 4 floats (m a multiple of 16): rows 4 apart are 16 banks apart, which keeps both the 16-byte reads along k
+// (16 rows, one k) and the 4-byte reads across rows (16 values of rows 4 apart) free of conflicts.
+constexpr int kNsShort = 128, kNsShortLong = 4096;      // short and long side up to which this way is taken
+struct NsShort {
+  int m, n, mp, mb, T, parts, blocks, pitch;            // m in 16s: mp = 16 mb; columns of a workgroup; workgroups; 16 x 16 blocks of A's lower triangle
+  __host__ __device__ NsShort(const NsShape& s) {
+    m = s.m, n = s.n, mp = (m + 15) & ~15, mb = mp / 16, T = mp <= 64 ? 64 : 32;
+    parts = (n + T - 1) / T, blocks = mb * (mb + 1) / 2, pitch = mp + 4;
+  }
+  __host__ __device__ long x() const { return (long)n * mp; }                     // floats of X^T
+  __host__ __device__ long share() const { return (long)parts * blocks * 256; }   // floats of A's shares
+  __host__ __device__ long bytes() const { return (x() + 2 * share()) * 4; }
+  __host__ __device__ int lds() const { return (2 * T + mp) * pitch * 4; }
+};
+
+// block b of the lower triangle of at most 8 x 8, row by row
+__device__ __forceinline__ void ns_triangle(int b, int& i, int& j) {
+  i = (b >= 1) + (b >= 3) + (b >= 6) + (b >= 10) + (b >= 15) + (b >= 21) + (b >= 28);
+  j = b - i * (i + 1) / 2;
+}
+
+template <bool START>
+__global__ void __launch_bounds__(512) ns_short_kernel(NsArgs g) {
+  extern __shared__ __align__(16) float sm[];
+  const int i = ns_find(g, blockIdx.x);
+  const NsItem it = g.it[i];
+  const NsShape shape(it.rows, it.cols);
+  const NsShort s(shape);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, c16 = lane & 15;
+  const int wg = blockIdx.x - it.at, j0 = wg * s.T, nj = min(s.T, s.n - j0);
+  float *xs = sm, *ys = xs + s.T * s.pitch, *as = ys + s.T * s.pitch;      // [column][row], [column][row], [row][row]
+  float* x = reinterpret_cast<float*>(g.ws + it.ws);
+  nsf4* in = reinterpret_cast<nsf4*>(x + s.x() + (g.flip ? s.share() : 0));
+  nsf4* out = reinterpret_cast<nsf4*>(x + s.x() + (g.flip ? 0 : s.share()));
+  // columns of the tile as rows of m values, 16 bytes a lane, two columns a wave
+  const int k4 = lane & 31, jw = wave * 2 + (lane >> 5);
+  if (START) {
+    if (shape.tall) {
+#pragma unroll 8
+      for (int j = wave; j < s.T; j += 8)
+        for (int k = lane; k < s.mp; k += 64) xs[j * s.pitch + k] = j < nj && k < s.m ? ns_start(g, it, (long)(j0 + j) * it.cols + k, true) : 0.f;
+    } else {
+      const int sh = s.T == 64 ? 6 : 5;
+#pragma unroll 8
+      for (int e = threadIdx.x; e < s.mp << sh; e += 512) {
+        const int k = e >> sh, j = e & (s.T - 1);
+        xs[j * s.pitch + k] = j < nj && k < s.m ? ns_start(g, it, (long)k * it.cols + j0 + j, true) : 0.f;
+      }
+    }
+    __syncthreads();
+  } else {
+    // all of the wave's loads in flight at once: its columns of X, then its (at most five) blocks of the shares
+    nsf4 xv[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int j = jw + 16 * e;
+      xv[e] = j < nj && k4 < s.mp / 4 ? *reinterpret_cast<const nsf4*>(x + (long)(j0 + j) * s.mp + 4 * k4) : nsf4{};
+    }
+    auto gather = [&](auto nb) {                          // blocks wave, wave + 8, ...: nb of them (the last one again where there are fewer)
+      constexpr int NB = decltype(nb)::value;
+      nsf4 v[NB] = {};
+      const nsf4* from[NB];
+#pragma unroll
+      for (int e = 0; e < NB; ++e) from[e] = in + min(wave + 8 * e, s.blocks - 1) * 64 + lane;
+      const int step = s.blocks * 64;
+      int p = 0;
+      for (; p + 4 <= s.parts; p += 4) {
+        nsf4 w[NB][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int e = 0; e < NB; ++e) w[e][u] = from[e][(p + u) * step];
+#pragma unroll
+        for (int e = 0; e < NB; ++e) v[e] += (w[e][0] + w[e][1]) + (w[e][2] + w[e][3]);
+      }
+      for (; p < s.parts; ++p)
+#pragma unroll
+        for (int e = 0; e < NB; ++e) v[e] += from[e][p * step];
+#pragma unroll
+      for (int e = 0; e < NB; ++e) {
+        int bi, bj;
+        ns_triangle(min(wave + 8 * e, s.blocks - 1), bi, bj);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) as[(16 * bi + 4 * q + r) * s.pitch + 16 * bj + c16] = v[e][r];
+        *reinterpret_cast<nsf4*>(as + (16 * bj + c16) * s.pitch + 16 * bi + 4 * q) = v[e];
+      }
+    };
+    if (s.blocks <= 8) gather(std::integral_constant<int, 1>{});
+    else if (s.blocks <= 16) gather(std::integral_constant<int, 2>{});
+    else gather(std::integral_constant<int, 5>{});
+    if (k4 < s.mp / 4) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (jw + 16 * e < s.T) *reinterpret_cast<nsf4*>(xs + (jw + 16 * e) * s.pitch + 4 * k4) = xv[e];
+      for (int j = jw + 32; j < s.T; j += 16)             // (64 columns)
+        *reinterpret_cast<nsf4*>(xs + j * s.pitch + 4 * k4) = j < nj ? *reinterpret_cast<const nsf4*>(x + (long)(j0 + j) * s.mp + 4 * k4) : nsf4{};
+    }
+    __syncthreads();
+    if (g.first) {                                        // X = U / max(|U|, eps), A = (X X^T) / the same squared
+      float tr = 0.f;
+      for (int k = lane; k < s.mp; k += 64) tr += as[k * s.pitch + k];
+#pragma unroll
+      for (int m = 32; m >= 1; m >>= 1) tr += __shfl_xor(tr, m, 64);
+      const float norm = sqrtf(tr), f = 1.f / (norm > g.eps || norm != norm ? norm : g.eps);
+      __syncthreads();
+      for (int e = threadIdx.x; e < s.mp * s.pitch; e += 512) as[e] = as[e] * f * f;
+      for (int e = threadIdx.x; e < s.T * s.pitch; e += 512) xs[e] *= f;
+      __syncthreads();
+    }
+    // block e of the wave: rows 16 rb ..., columns 16 cb ...; at most two of the at most 16 blocks of a tile
+    const int tiles = s.mb * (s.T / 16);
+    int at[2];
+    nsf4 acc[2];
+    // A v: the lane's four k-values are 4 q ... 4 q + 3 of every 16, each summed on its own (a chain of m / 4 roundings, not m)
+    auto product = [&](const float* v) {
+      nsf4 sum[2][4] = {};
+      for (int k = 0; k < s.mp; k += 16)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int b = min(wave + 8 * e, tiles - 1), rb = b % s.mb, cb = b / s.mb;
+          const nsf4 av = *reinterpret_cast<const nsf4*>(as + (16 * rb + c16) * s.pitch + k + 4 * q);
+          const nsf4 bv = *reinterpret_cast<const nsf4*>(v + (16 * cb + c16) * s.pitch + k + 4 * q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum[e][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[j], bv[j], sum[e][j], 0, 0, 0);
+        }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) acc[e] = (sum[e][0] + sum[e][1]) + (sum[e][2] + sum[e][3]);
+    };
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int b = min(wave + 8 * e, tiles - 1);
+      at[e] = (16 * (b / s.mb) + c16) * s.pitch + 16 * (b % s.mb) + 4 * q;      // the lane's four rows of its column
+    }
+    product(xs);
+    // (a wave without a block of its own computes the last one again and writes the same values)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) *reinterpret_cast<nsf4*>(ys + at[e]) = acc[e];
+    __syncthreads();
+    product(ys);
+    nsf4 next[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const nsf4 xv = *reinterpret_cast<const nsf4*>(xs + at[e]), yv = *reinterpret_cast<const nsf4*>(ys + at[e]);
+      next[e] = g.a * xv + (g.b * yv + g.c * acc[e]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; ++e) *reinterpret_cast<nsf4*>(xs + at[e]) = next[e];
+    __syncthreads();
+    if (g.last) {
+      if (shape.tall) {
+        for (int j = wave; j < nj; j += 8)
+          for (int k = lane; k < s.m; k += 64) ns_result(g, it, (long)(j0 + j) * it.cols + k, xs[j * s.pitch + k]);
+      } else {
+        const int sh = s.T == 64 ? 6 : 5;
+        for (int e = threadIdx.x; e < s.m << sh; e += 512) {
+          const int k = e >> sh, j = e & (s.T - 1);
+          if (j < nj) ns_result(g, it, (long)k * it.cols + j0 + j, xs[j * s.pitch + k]);
+        }
+      }
+      return;
+    }
+  }
+  if (k4 < s.mp / 4)
+    for (int j = jw; j < nj; j += 16)
+      *reinterpret_cast<nsf4*>(x + (long)(j0 + j) * s.mp + 4 * k4) = *reinterpret_cast<const nsf4*>(xs + j * s.pitch + 4 * k4);
+  // this tile's share of X X^T, blocks of the lower triangle in the order of the accumulators
+  for (int b = wave; b < s.blocks; b += 8) {
+    int bi, bj;
+    ns_triangle(b, bi, bj);
+    nsf4 sum[4] = {};
+    for (int j = 0; j < s.T; j += 16)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float* col = xs + (j + e + 4 * q) * s.pitch + c16;
+        sum[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(col[16 * bi], col[16 * bj], sum[e], 0, 0, 0);
+      }
+    out[((long)wg * s.blocks + b) * 64 + lane] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------
 static const char* ns_bad(int count, const int* rows, const int* cols) {
   if (count < 0 || (count > 0 && (!rows || !cols))) return "bad list";
@@ -451,12 +643,22 @@ static bool ns_apart(int count, const int* rows, const int* cols, int size, cons
 }
 static int ns_chunks(int rows, int cols) { return (int)(((long)rows * cols + kNsChunk - 1) / kNsChunk); }
 
-// workspace of matrices b ... e - 1: pieces, then the norm's partial sums, then partial tiles
+static bool ns_is_short(int rows, int cols) {
+  return std::min(rows, cols) <= std::min(kNsShort, tuning("BMV_NS_SHORT", kNsShort)) && std::max(rows, cols) <= kNsShortLong;
+}
+// Workspace of a part of the list (indices): the short ones' X and shares, or the others' pieces, then the norm's partial
+// sums, then partial tiles
+static long ns_short_room(const int* rows, const int* cols, const int* idx, int n) {
+  long bytes = 0;
+  for (int k = 0; k < n; ++k) bytes += NsShort(NsShape(rows[idx[k]], cols[idx[k]])).bytes();
+  return bytes;
+}
 struct NsRoom {
   long pieces = 0, tiles = 0;
   int sqn = 1;
-  NsRoom(const int* rows, const int* cols, int b, int e, int p) {
-    for (int i = b; i < e; ++i) {
+  NsRoom(const int* rows, const int* cols, const int* idx, int n, int p) {
+    for (int k = 0; k < n; ++k) {
+      const int i = idx[k];
       const NsShape s(rows[i], cols[i]);
       pieces += ns_bytes(s, p), tiles += (long)s.mt() * s.nt();      // (no fewer than the symmetric products')
       sqn = std::max(sqn, ns_chunks(rows[i], cols[i]));
@@ -464,11 +666,25 @@ struct NsRoom {
   }
   long bytes() const { return pieces + (long)kNsList * sqn * sizeof(double) + (tiles + kNsSlots) * (kNsTile * kNsTile * 4l); }
 };
+// the list's indices: the short ones, then the others
+static std::vector<int> ns_order(int count, const int* rows, const int* cols, int& shorts) {
+  std::vector<int> v;
+  v.reserve(count);
+  for (int i = 0; i < count; ++i)
+    if (ns_is_short(rows[i], cols[i])) v.push_back(i);
+  shorts = (int)v.size();
+  for (int i = 0; i < count; ++i)
+    if (!ns_is_short(rows[i], cols[i])) v.push_back(i);
+  return v;
+}
 // a list is done in parts of kNsList, which share the workspace
 static long ns_workspace(int count, const int* rows, const int* cols, int dtype) {
   long most = 0;
-  for (int b = 0; b < count; b += kNsList)
-    most = std::max(most, NsRoom(rows, cols, b, std::min(count, b + kNsList), dtype == 1 ? 2 : 3).bytes());
+  int shorts;
+  const std::vector<int> v = ns_order(count, rows, cols, shorts);
+  for (int b = 0; b < shorts; b += kNsList) most = std::max(most, ns_short_room(rows, cols, &v[b], std::min(shorts - b, kNsList)));
+  for (int b = shorts; b < count; b += kNsList)
+    most = std::max(most, NsRoom(rows, cols, &v[b], std::min(count - b, kNsList), dtype == 1 ? 2 : 3).bytes());
   return most;
 }
 
@@ -491,32 +707,79 @@ static void ns_product(NsArgs& g, hipStream_t st) {
   hipLaunchKernelGGL((ns_join_kernel<P, STAGE>), dim3((unsigned)(4 * tiles)), dim3(256), 0, st, g);
 }
 
-template <int P>
-static void ns_run(NsArgs g, int count, const void* const* src, void* const* dst, float* const* buf, const int* rows,
-                   const int* cols, const float* scales, int steps, char* ws, hipStream_t st) {
-  for (int b = 0; b < count; b += kNsList) {
-    g.count = std::min(count - b, kNsList);
-    const NsRoom room(rows, cols, b, b + g.count, P);
-    g.ws = ws, g.sqn = room.sqn, g.sq = reinterpret_cast<double*>(ws + room.pieces);
-    g.part = reinterpret_cast<float*>(g.sq + (long)kNsList * g.sqn);
-    long off = 0, chunks = 0;
-    for (int i = 0; i < g.count; ++i) {
-      NsItem& it = g.it[i];
-      it.src = src[b + i], it.dst = dst[b + i], it.buf = buf ? buf[b + i] : nullptr, it.rows = rows[b + i], it.cols = cols[b + i];
-      it.scale = scales ? scales[b + i] : 1.f, it.ws = off, it.at = (int)chunks;
-      off += ns_bytes(NsShape(it.rows, it.cols), P), chunks += ns_chunks(it.rows, it.cols);
-    }
-    hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)chunks), dim3(256), 0, st, g);
-    long blocks = 0;
-    for (int i = 0; i < g.count; ++i) g.it[i].at = (int)blocks, blocks += NsShape(g.it[i].rows, g.it[i].cols).big() / (64 * 64);
-    hipLaunchKernelGGL(ns_split_kernel<P>, dim3((unsigned)blocks), dim3(256), 0, st, g);
-    for (int k = 0; k < steps; ++k) {
-      g.last = k + 1 == steps, g.flip = k & 1;
-      ns_product<P, kNsGram>(g, st);
-      ns_product<P, kNsPoly>(g, st);
-      ns_product<P, kNsApply>(g, st);
-    }
+struct NsLists {
+  const void* const* src;
+  void* const* dst;
+  float* const* buf;
+  const int *rows, *cols;
+  const float* scales;
+};
+static void ns_fill(NsArgs& g, const NsLists& l, const int* idx, int n) {
+  g.count = n;
+  for (int k = 0; k < n; ++k) {
+    NsItem& it = g.it[k];
+    const int i = idx[k];
+    it.src = l.src[i], it.dst = l.dst[i], it.buf = l.buf ? l.buf[i] : nullptr, it.rows = l.rows[i], it.cols = l.cols[i];
+    it.scale = l.scales ? l.scales[i] : 1.f;
   }
+}
+
+static void ns_run_short(NsArgs& g, int steps, char* ws, hipStream_t st) {
+  long off = 0, wgs = 0;
+  int lds = 0;
+  g.ws = ws;
+  for (int i = 0; i < g.count; ++i) {
+    const NsShort s(NsShape(g.it[i].rows, g.it[i].cols));
+    g.it[i].ws = off, g.it[i].at = (int)wgs, off += s.bytes(), wgs += s.parts, lds = std::max(lds, s.lds());
+  }
+  g.flip = 1;                                             // (the first shares go to where step 0 reads)
+  hipLaunchKernelGGL(ns_short_kernel<true>, dim3((unsigned)wgs), dim3(512), lds, st, g);
+  for (int k = 0; k < steps; ++k) {
+    g.first = k == 0, g.last = k + 1 == steps, g.flip = k & 1;
+    hipLaunchKernelGGL(ns_short_kernel<false>, dim3((unsigned)wgs), dim3(512), lds, st, g);
+  }
+}
+
+template <int P>
+static void ns_run_long(NsArgs& g, const NsRoom& room, int steps, char* ws, hipStream_t st) {
+  g.ws = ws, g.sqn = room.sqn, g.sq = reinterpret_cast<double*>(ws + room.pieces);
+  g.part = reinterpret_cast<float*>(g.sq + (long)kNsList * g.sqn);
+  long off = 0, chunks = 0, blocks = 0;
+  for (int i = 0; i < g.count; ++i) {
+    NsItem& it = g.it[i];
+    it.ws = off, it.at = (int)chunks;
+    off += ns_bytes(NsShape(it.rows, it.cols), P), chunks += ns_chunks(it.rows, it.cols);
+  }
+  hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)chunks), dim3(256), 0, st, g);
+  for (int i = 0; i < g.count; ++i) g.it[i].at = (int)blocks, blocks += NsShape(g.it[i].rows, g.it[i].cols).big() / (64 * 64);
+  hipLaunchKernelGGL(ns_split_kernel<P>, dim3((unsigned)blocks), dim3(256), 0, st, g);
+  for (int k = 0; k < steps; ++k) {
+    g.last = k + 1 == steps, g.flip = k & 1;
+    ns_product<P, kNsGram>(g, st);
+    ns_product<P, kNsPoly>(g, st);
+    ns_product<P, kNsApply>(g, st);
+  }
+}
+
+static int ns_run(NsArgs g, int count, const NsLists& l, int dtype, int steps, void* workspace, hipStream_t st) {
+  constexpr int kLds = (2 * 32 + 128) * (128 + 4) * 4;    // the largest NsShort::lds(): above what a kernel gets without asking
+  static const bool ready = hipFuncSetAttribute((const void*)ns_short_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess &&
+                            hipFuncSetAttribute((const void*)ns_short_kernel<false>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess;
+  if (!ready) return -1;
+  char* ws = static_cast<char*>(workspace);
+  int shorts;
+  const std::vector<int> v = ns_order(count, l.rows, l.cols, shorts);
+  for (int b = 0; b < shorts; b += kNsList) {
+    ns_fill(g, l, &v[b], std::min(shorts - b, kNsList));
+    ns_run_short(g, steps, ws, st);
+  }
+  for (int b = shorts; b < count; b += kNsList) {
+    const int n = std::min(count - b, kNsList);
+    ns_fill(g, l, &v[b], n);
+    if (dtype == 1) ns_run_long<2>(g, NsRoom(l.rows, l.cols, &v[b], n, 2), steps, ws, st);
+    else ns_run_long<3>(g, NsRoom(l.rows, l.cols, &v[b], n, 3), steps, ws, st);
+  }
+  return 0;
 }
 
 }  // namespace bmv
@@ -544,8 +807,8 @@ int bmv_newton_schulz(int count, const void* const* src, void* const* dst, const
   BMV_REQUIRE(ns_apart(count, rows, cols, dtype == 0 ? 4 : 2, src, dst, nullptr), "bmv_newton_schulz: a result overlaps another matrix");
   NsArgs g{};
   g.dtype = dtype, g.a = a, g.b = b, g.c = c, g.eps = eps;
-  if (dtype != 1) ns_run<3>(g, count, src, dst, nullptr, rows, cols, nullptr, steps, static_cast<char*>(workspace), as_stream(stream));
-  else ns_run<2>(g, count, src, dst, nullptr, rows, cols, nullptr, steps, static_cast<char*>(workspace), as_stream(stream));
+  const NsLists l{src, dst, nullptr, rows, cols, nullptr};
+  BMV_REQUIRE(ns_run(g, count, l, dtype, steps, workspace, as_stream(stream)) == 0, "bmv_newton_schulz: LDS refused");
   BMV_LAUNCH_END("bmv_newton_schulz");
 }
 
@@ -564,8 +827,8 @@ int bmv_muon_step(int count, void* const* params, const void* const* grads, floa
               "bmv_muon_step: a weight or a momentum overlaps another tensor (is one listed twice?)");
   NsArgs g{};
   g.dtype = dtype, g.a = a, g.b = b, g.c = c, g.eps = eps, g.muon = 1, g.nesterov = nesterov, g.mu = (float)momentum, g.nu = (float)(1. - momentum), g.keep = (float)keep;
-  if (dtype != 1) ns_run<3>(g, count, grads, params, momenta, rows, cols, scales, steps, static_cast<char*>(workspace), as_stream(stream));
-  else ns_run<2>(g, count, grads, params, momenta, rows, cols, scales, steps, static_cast<char*>(workspace), as_stream(stream));
+  const NsLists l{grads, params, momenta, rows, cols, scales};
+  BMV_REQUIRE(ns_run(g, count, l, dtype, steps, workspace, as_stream(stream)) == 0, "bmv_muon_step: LDS refused");
   BMV_LAUNCH_END("bmv_muon_step");
 }
 

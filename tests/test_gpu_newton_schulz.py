@@ -64,12 +64,21 @@ def _check(got, u, steps=5, coeffs=COEFFS, eps=1e-7):
 
 
 SHAPES = [(1, 1), (1, 7), (9, 1), (2, 2), (3, 64), (8, 27), (16, 200), (35, 4), (64, 24), (33, 32), (63, 65), (64, 64), (64, 1728),
-          (65, 40), (127, 129), (128, 63), (128, 128), (128, 515), (129, 129), (130, 1000), (333, 257), (256, 384), (700, 90)]
+          (65, 40), (80, 100), (127, 129), (128, 63), (8, 4000), (128, 4096), (128, 4097), (33, 1000), (128, 128), (128, 515), (129, 129), (130, 1000), (333, 257), (256, 384), (700, 90)]
+
+
+@pytest.fixture(params=["short", "long"])
+def way(request):
+    """Short sides of up to 128 one launch a step (default), and through the tiles of the large ones."""
+    from boostmvsnerfs_amd import _lib
+    _lib.set_tuning("BMV_NS_SHORT", None if request.param == "short" else 0)
+    yield request.param
+    _lib.set_tuning("BMV_NS_SHORT", None)
 
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-def test_newton_schulz_matches_the_formula(dtype):
+def test_newton_schulz_matches_the_formula(dtype, way):
     from boostmvsnerfs_amd import ops
     mats = [_grad(m, n, seed=i).to(dtype) for i, (m, n) in enumerate(SHAPES)]
     on_gpu = [v.cuda() for v in mats]
@@ -84,7 +93,7 @@ def test_newton_schulz_matches_the_formula(dtype):
 
 
 @gpu
-def test_newton_schulz_is_as_exact_as_the_iteration_in_fp32():
+def test_newton_schulz_is_as_exact_as_the_iteration_in_fp32(way):
     """Within four times the error of the same iteration in fp32 products (four: two roundings for its one at the operands'
     pieces, and the spread of one random error against another), on flat and on decaying spectra."""
     from boostmvsnerfs_amd import ops
@@ -150,7 +159,7 @@ def test_newton_schulz_steps_coefficients_and_lists():
 
 
 @gpu
-def test_newton_schulz_zero_tiny_and_non_finite():
+def test_newton_schulz_zero_tiny_and_non_finite(way):
     from boostmvsnerfs_amd import ops
     u = _grad(24, 40, 2)
     mats = [u * 0, u * 1e-12, u * 1e-30, u * 1e12, u.clone(), u.clone(), u]
@@ -168,7 +177,7 @@ def test_newton_schulz_zero_tiny_and_non_finite():
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("nesterov,scale,decay", [(True, "shape", 0.0), (False, "rms", 0.1), (True, "none", 0.01)])
-def test_muon_step_matches_the_formula(dtype, nesterov, scale, decay):
+def test_muon_step_matches_the_formula(dtype, nesterov, scale, decay, way):
     from boostmvsnerfs_amd import ops
     shapes = [(8, 27), (64, 24), (1, 12), (128, 63), (130, 140), (16, 8, 3, 3), (200, 40)]
     g = torch.Generator().manual_seed(11)
