@@ -1491,16 +1491,22 @@ NS_COEFFS = (3.4445, -4.7750, 2.0315)      # the quintic a s + b s^3 + c s^5 of 
 NS_EPS = 1e-7
 
 
-def _matrix(t, name):
-    """(rows, cols) of a weight as a matrix: everything behind the first dimension is its columns."""
-    _gpu_float(t, name)
-    if t.dim() < 2:
-        raise ValueError(f"{name}: expected a matrix (at least 2 dimensions), got {tuple(t.shape)}")
-    rows = t.shape[0]
-    cols = t.numel() // rows if rows else 0
-    if rows > 65536 or cols > 65536:
-        raise ValueError(f"{name}: sides of up to 65536, got {rows} x {cols}")
-    return rows, cols
+def _matrices(tensors, name):
+    """(rows, cols) of each weight as a matrix: everything behind the first dimension is its columns.  (Lists of a network's
+    weights come here every step: one pass, names only for errors.)"""
+    sizes = []
+    for i, t in enumerate(tensors):
+        if not (isinstance(t, torch.Tensor) and t.dtype in _FLOAT_CODES and t.is_cuda):
+            _gpu_float(t, f"{name}[{i}]")           # raises
+        shape = t.shape
+        if len(shape) < 2:
+            raise ValueError(f"{name}[{i}]: expected a matrix (at least 2 dimensions), got {tuple(shape)}")
+        rows = shape[0]
+        cols = shape[1] if len(shape) == 2 else t.numel() // rows if rows else 0
+        if rows > 65536 or cols > 65536:
+            raise ValueError(f"{name}[{i}]: sides of up to 65536, got {rows} x {cols}")
+        sizes.append((rows, cols))
+    return sizes
 
 
 def _ns_args(steps, coeffs, eps):
@@ -1512,17 +1518,24 @@ def _ns_args(steps, coeffs, eps):
     return int(steps), a, b, c, float(eps)
 
 
-def _by_kind(tensors):
+def _by_kind(tensors, sizes):
     """Indices of the non-empty tensors, by (device, dtype): a launch has one of each."""
     kinds = {}
     for i, t in enumerate(tensors):
-        if t.numel():
+        if sizes[i][0] and sizes[i][1]:
             kinds.setdefault((t.device, t.dtype), []).append(i)
     return kinds.items()
 
 
 def _pointers(tensors):
-    return (C.c_void_p * len(tensors))(*[_addr(t) for t in tensors])
+    """Host array of the tensors' addresses; they stay referenced until the launch is enqueued (see _lib.dptr)."""
+    _lib._held_list().extend(tensors)
+    return (C.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def _sides(sizes, idx):
+    n = C.c_int * len(idx)
+    return n(*[sizes[i][0] for i in idx]), n(*[sizes[i][1] for i in idx])
 
 
 def _ns_workspace(lib, count, rows, cols, dtype, device):
@@ -1541,16 +1554,17 @@ def newton_schulz(mats, steps=5, coeffs=NS_COEFFS, eps=NS_EPS):
         return newton_schulz([mats], steps, coeffs, eps)[0]
     mats = list(mats)
     steps, a, b, c, eps = _ns_args(steps, coeffs, eps)
-    sizes = [_matrix(t, f"mats[{i}]") for i, t in enumerate(mats)]
-    out = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in mats]
+    sizes = _matrices(mats, "mats")
+    mats = [t if t.is_contiguous() else t.contiguous() for t in mats]
+    out = [torch.empty_like(t) for t in mats]
     lib = _lib.load()
-    for (device, dtype), idx in _by_kind(mats):
+    for (device, dtype), idx in _by_kind(mats, sizes):
         with _on_device_of(mats[idx[0]]):
             n = len(idx)
-            rows, cols = (C.c_int * n)(*[sizes[i][0] for i in idx]), (C.c_int * n)(*[sizes[i][1] for i in idx])
+            rows, cols = _sides(sizes, idx)
             ws = _ns_workspace(lib, n, rows, cols, dtype, device)
             with ktimer.region("newton_schulz"):
-                rc = lib.bmv_newton_schulz(n, _pointers([_c(mats[i]) for i in idx]), _pointers([out[i] for i in idx]), rows, cols,
+                rc = lib.bmv_newton_schulz(n, _pointers([mats[i] for i in idx]), _pointers([out[i] for i in idx]), rows, cols,
                                            _FLOAT_CODES[dtype], steps, a, b, c, eps, _addr(ws), stream())
             _lib.check(rc, "newton_schulz")
     return out
@@ -1579,19 +1593,19 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
     if not 0 <= momentum < 1:
         raise ValueError(f"momentum: expected 0 <= momentum < 1, got {momentum}")
     lr, keep = float(lr), 1.0 - float(lr) * float(weight_decay)
-    sizes = []
+    sizes = _matrices(params, "params")
     for i, (p, g, m) in enumerate(zip(params, grads, momenta)):
-        sizes.append(_matrix(p, f"params[{i}]"))
-        _gpu_float(g, f"grads[{i}]", p), _gpu_float(m, f"momenta[{i}]", p)
-        if g.shape != p.shape or g.dtype != p.dtype:
+        if not (isinstance(g, torch.Tensor) and g.shape == p.shape and g.dtype == p.dtype and g.device == p.device):
+            _gpu_float(g, f"grads[{i}]", p)
             raise ValueError(f"grads[{i}]: expected {tuple(p.shape)} {p.dtype}, got {tuple(g.shape)} {g.dtype}")
-        if m.shape != p.shape or m.dtype != torch.float32:
+        if not (isinstance(m, torch.Tensor) and m.shape == p.shape and m.dtype == torch.float32 and m.device == p.device):
+            _gpu_float(m, f"momenta[{i}]", p)
             raise ValueError(f"momenta[{i}]: expected {tuple(p.shape)} float32, got {tuple(m.shape)} {m.dtype}")
     lib = _lib.load()
-    for (device, dtype), idx in _by_kind(params):
+    for (device, dtype), idx in _by_kind(params, sizes):
         with torch.no_grad(), _on_device_of(params[idx[0]]):
             n = len(idx)
-            rows, cols = (C.c_int * n)(*[sizes[i][0] for i in idx]), (C.c_int * n)(*[sizes[i][1] for i in idx])
+            rows, cols = _sides(sizes, idx)
             scales = (C.c_float * n)(*[lr * MUON_SCALES[scale](*sizes[i]) for i in idx])
             p, m = [_c(params[i]) for i in idx], [_c(momenta[i]) for i in idx]
             ws = _ns_workspace(lib, n, rows, cols, dtype, device)
