@@ -17,6 +17,7 @@ import torch.nn.functional as F
 
 from ... import autograd as A
 from ... import convnet, ops, switches
+from ..norm import GroupNorm
 from .conv_train import Conv2d, Conv3d, ConvTranspose3d, _Conv3dFn   # engine forward / data gradients, MFMA weight gradients
 
 
@@ -32,7 +33,7 @@ def _engine_ok(module, x):
         raise RuntimeError(f"{type(module).__name__}: the BoostMVSNeRFs hot path runs on the GPU only (input is on "
                            f"{x.device}); there is no CPU fallback")
     return (not module.training and not torch.is_grad_enabled() and x.is_cuda and x.dtype == torch.float32
-            and switches.get("BMV_CNN") != "torch")
+            and switches.get("BMV_CNN") != "torch" and not getattr(module, "group_norm", False))
 
 
 # (BMV_FPN_FUSE / BMV_CONV0_FUSE / BMV_TOP_FUSE are read where FeatureNet's engine path runs: `switches.set()` /
@@ -70,7 +71,10 @@ def _pack_cbr(m):
 def _bn_forward(bn, x, relu):
     """bn(x) [+ ReLU].  A plain nn.BatchNorm{2,3}d in training mode on the GPU runs on csrc/bn.hip (statistics pass +
     apply pass, ReLU fused; MIOpen's spatial batch norm costs ~73 us per call whatever the size); everything else --
-    eval mode, SyncBatchNorm under DDP, BMV_BN=torch -- stays on torch."""
+    eval mode, SyncBatchNorm under DDP, BMV_BN=torch -- stays on torch.  A converted network's group norm
+    (networks/norm.py) takes its activation from here."""
+    if isinstance(bn, GroupNorm):
+        return bn(x, relu)
     if (type(bn) in (nn.BatchNorm2d, nn.BatchNorm3d) and bn.training and bn.track_running_stats and bn.affine
             and bn.momentum is not None and x.is_cuda and x.dtype == torch.float32
             and switches.get("BMV_BN") != "torch"):
@@ -284,7 +288,7 @@ class _CostReg(nn.Module):
     def takes_quad_volume(self):
         """True: hand forward() the cost volume as ops.QuadVolume (the sweep's quad-record output) -- the first layer runs
         on the 4-row-block kernel, which stages such an input with one 16-byte load per position."""
-        return (self.quad_volume and self.conv_c4 and not self.training and not torch.is_grad_enabled()
+        return (self.quad_volume and self.conv_c4 and not self.training and not torch.is_grad_enabled() and not getattr(self, "group_norm", False)
                 and switches.get("BMV_CNN") != "torch" and not convnet.split_parts(self.split_bf16, "conv0", self.conv0.conv.weight.shape[1]))
 
     def _apply(self, fn, *args, **kwargs):
@@ -294,6 +298,8 @@ class _CostReg(nn.Module):
     def prepack(self):
         """Folded + packed weights (cached).  Callers that run this module on several streams call it once on the
         stream they fork from: the pack kernels must not race with a side stream's first use of the blobs."""
+        if getattr(self, "group_norm", False):
+            return None
         def build():
             P = {f"conv{i}": _pack_cbr(getattr(self, f"conv{i}")) for i in range(5 + 2 * (self.depth == 3))}
             for name in ("conv7", "conv9", "conv11")[3 - self.depth:]:

@@ -150,9 +150,11 @@ class _Conv2dFn(torch.autograd.Function):
 
 
 class Conv2d(nn.Conv2d):
+    engine_always = False     # True: the engine without autograd as well (networks/norm.py: blocks that are not folded)
+
     def forward(self, x):
         k = self.kernel_size[0]
-        if (torch.is_grad_enabled() and _engine_forward(x) and self.kernel_size == (k, k) and (k, self.stride) in
+        if ((torch.is_grad_enabled() or self.engine_always) and _engine_forward(x) and self.kernel_size == (k, k) and (k, self.stride) in
                 ((1, (1, 1)), (3, (1, 1)), (5, (2, 2))) and self.padding == (k // 2, k // 2) and self.dilation == (1, 1)
                 and self.groups == 1 and self.padding_mode == "zeros"):
             return _Conv2dFn.apply(x, self.weight, self.bias, self.stride[0])
@@ -160,8 +162,10 @@ class Conv2d(nn.Conv2d):
 
 
 class Conv3d(nn.Conv3d):
+    engine_always = False
+
     def forward(self, x):
-        if (torch.is_grad_enabled() and self.weight.requires_grad and self.bias is None and self.kernel_size == (3, 3, 3)
+        if ((torch.is_grad_enabled() and self.weight.requires_grad or self.engine_always) and self.bias is None and self.kernel_size == (3, 3, 3)
                 and self.padding == (1, 1, 1) and self.dilation == (1, 1, 1) and self.groups == 1
                 and self.stride[0] == self.stride[1] == self.stride[2]):
             return _Conv3dFn.apply(x, self.weight, self.stride[0])
@@ -169,8 +173,10 @@ class Conv3d(nn.Conv3d):
 
 
 class ConvTranspose3d(nn.ConvTranspose3d):
+    engine_always = False
+
     def forward(self, x, output_size=None):
-        if (torch.is_grad_enabled() and self.weight.requires_grad and self.bias is None and output_size is None
+        if ((torch.is_grad_enabled() and self.weight.requires_grad or self.engine_always) and self.bias is None and output_size is None
                 and self.kernel_size == (3, 3, 3) and self.stride == (2, 2, 2) and self.padding == (1, 1, 1)
                 and self.output_padding == (1, 1, 1) and self.groups == 1):
             return _ConvT3dFn.apply(x, self.weight)

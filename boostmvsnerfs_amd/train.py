@@ -10,7 +10,7 @@ import torch
 import torch.nn as nn
 from torch.optim._functional import adam as _adam_update
 
-from . import convnet
+from . import convnet, ops
 from .config import cfg
 
 
@@ -108,9 +108,96 @@ class GroupedAdam(torch.optim.Adam):
         return loss
 
 
-def make_optimizer(net, lr=5e-4, weight_decay=0.0, eps=1e-8):
+class MuonAdam(torch.optim.Optimizer):
+    """Orthogonalised momentum for weight matrices, Adam for the rest: the matrices' updates are the Newton-Schulz iterate of
+    their (Nesterov) momentum, ONE list of launches for all of them (ops.muon_step, csrc/newton_schulz.hip), the other
+    parameters step as GroupedAdam's.
+
+    `matrices` / `others`: parameters, or param groups (the reference's one-group-per-parameter layout works for both).  A
+    matrix has 2 dimensions or more (convolution kernels are flattened behind the first) and is fp32, bf16 or fp16, contiguous
+    or not; its state is `momentum_buffer`, fp32.  Groups of matrices carry lr, momentum, nesterov, weight_decay (decoupled),
+    scale (ops.muon_step) and steps; schedulers see all groups.  Learning rates are plain numbers."""
+
+    def __init__(self, matrices, others=(), lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, scale="shape", steps=5,
+                 adam_lr=5e-4, adam_weight_decay=0.0, adam_eps=1e-8):
+        if scale not in ops.MUON_SCALES:
+            raise ValueError(f"scale: expected one of {sorted(ops.MUON_SCALES)}, got {scale!r}")
+        super().__init__(list(matrices), dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, scale=scale,
+                                              steps=steps, muon=True))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() < 2:
+                    raise ValueError(f"a matrix has at least 2 dimensions, got {tuple(p.shape)}")
+        others = list(others)
+        self._adam = None
+        if others:
+            self._adam = GroupedAdam(others, lr=adam_lr, weight_decay=adam_weight_decay, eps=adam_eps)
+            for group in self._adam.param_groups:
+                group["muon"] = False
+            both = {id(p) for g in self.param_groups for p in g["params"]}
+            if any(id(p) in both for g in self._adam.param_groups for p in g["params"]):
+                raise ValueError("a parameter is listed among the matrices and among the others")
+            self.param_groups += self._adam.param_groups
+        self._share()
+
+    def _share(self):
+        """Adam works on this optimiser's own state and groups."""
+        if self._adam is not None:
+            self._adam.state = self.state
+            self._adam.param_groups = [g for g in self.param_groups if not g["muon"]]
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # (torch casts a state to its parameter's type: a 16-bit weight's momentum is fp32)
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, [p for g in self.param_groups for p in g["params"]]):
+            saved = state_dict["state"].get(i, {}).get("momentum_buffer")
+            if saved is not None:
+                self.state[p]["momentum_buffer"] = saved.detach().to(device=p.device, dtype=torch.float32, copy=True)
+        self._share()
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if self._adam is not None:
+            self._adam.step()
+        buckets = {}
+        for group in self.param_groups:
+            if not group["muon"]:
+                continue
+            key = (group["lr"], group["momentum"], group["nesterov"], group["weight_decay"], group["scale"], group["steps"])
+            if any(torch.is_tensor(k) for k in key):
+                raise TypeError("MuonAdam: hyper-parameters are plain numbers")
+            params, grads, momenta = buckets.setdefault(key, ([], [], []))
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("MuonAdam: sparse gradients are not supported")
+                state = self.state[p]
+                if not state:
+                    state["momentum_buffer"] = torch.zeros(p.shape, device=p.device, dtype=torch.float32)
+                params.append(p), grads.append(p.grad), momenta.append(state["momentum_buffer"])
+        for (lr, momentum, nesterov, decay, scale, steps), lists in buckets.items():
+            if lists[0]:
+                ops.muon_step(*lists, lr, momentum, nesterov, decay, scale, steps)
+        return loss
+
+
+def make_optimizer(net, lr=5e-4, weight_decay=0.0, eps=1e-8, optim="adam", muon_lr=0.02):
     """lib/train/optimizer.py:12-28 with cfg.train.optim = 'adam' (every shipped config): one param group per
-    parameter, in named_parameters() order."""
+    parameter, in named_parameters() order.  optim = 'muon': the matrices with more than one row step as MuonAdam's with
+    `muon_lr`, all other parameters (biases, normalisations, one-row heads) as before."""
+    if optim not in ("adam", "muon"):
+        raise ValueError(f"optim: expected 'adam' or 'muon', got {optim!r}")
+    if optim == "muon":
+        named = [p for _, p in net.named_parameters() if p.requires_grad]
+        muon = [p.dim() >= 2 and p.shape[0] > 1 for p in named]
+        return MuonAdam([{"params": [p]} for p, m in zip(named, muon) if m], [{"params": [p]} for p, m in zip(named, muon) if not m],
+                        lr=muon_lr, weight_decay=weight_decay, adam_lr=lr, adam_weight_decay=weight_decay, adam_eps=eps)
     params = [{"params": [p], "lr": lr, "weight_decay": weight_decay, "eps": eps} for _, p in net.named_parameters() if p.requires_grad]
     return GroupedAdam(params, lr=lr, weight_decay=weight_decay, eps=eps)
 
