@@ -230,19 +230,32 @@ class GroupNormAct(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, groups, weight, bias, eps=1e-5, relu=False):
-        y, mean, rstd = ops.group_norm_fwd(x, groups, weight, bias, eps, relu)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        y, stats = ops.group_norm_stats_fwd(x, groups, weight, bias, eps, relu)
+        ctx.save_for_backward(x, weight, bias, stats)
         ctx.cfg = (groups, relu)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
+        x, weight, bias, stats = ctx.saved_tensors
         groups, relu = ctx.cfg
         _, _, want_w, want_b, _, _ = ctx.needs_input_grad
-        dx, dw, db = ops.group_norm_bwd(x, dy, groups, weight, bias, mean, rstd, relu, want_params=want_w or want_b)
+        dx, dw, db = ops.group_norm_stats_bwd(x, dy, groups, weight, bias, stats, relu, want_w or want_b)
+        if torch.is_grad_enabled():          # create_graph: the gradients depend on all of these
+            dx, dw, db = _NotAgain.apply(dx, dw, db, x, weight, bias, dy)
         return dx, None, dw if want_w else None, db if want_b else None, None, None
+
+
+class _NotAgain(torch.autograd.Function):
+    """GroupNormAct's gradients where autograd records them: a second differentiation is refused, not silently left out."""
+
+    @staticmethod
+    def forward(ctx, dx, dw, db, *_inputs):
+        return dx.view_as(dx), None if dw is None else dw.view_as(dw), None if db is None else db.view_as(db)
+
+    @staticmethod
+    def backward(ctx, *_grads):
+        raise RuntimeError("GroupNormAct: a second differentiation is not supported")
 
 
 class MvsSweep(torch.autograd.Function):

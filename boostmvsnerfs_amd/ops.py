@@ -1370,54 +1370,105 @@ def _gpu_float(t, name, like=None):
     return t
 
 
-def _addr(t):
-    """Address of a dense tensor of any layout, kept referenced until the launch is enqueued (see _lib.dptr)."""
-    if t is None:
-        return None
-    _lib._held_list().append(t)
-    return t.data_ptr()
-
-
 def _gn_dense(x):
     """(x dense in one of the two layouts, 1 for channel-last / 0 for planar)."""
-    last = x.dim() > 2 and ((x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last))
-                            or (x.dim() == 5 and x.is_contiguous(memory_format=torch.channels_last_3d))
-                            or (x.dim() == 3 and x.transpose(1, 2).is_contiguous()))
-    if not (last or x.is_contiguous()):
-        x = x.contiguous()
+    last = 0
+    if not x.is_contiguous():
+        d = x.dim()
+        last = int((d == 4 and x.is_contiguous(memory_format=torch.channels_last))
+                   or (d == 5 and x.is_contiguous(memory_format=torch.channels_last_3d))
+                   or (d == 3 and x.transpose(1, 2).is_contiguous()))
+        if not last:
+            x = x.contiguous()
     if x.data_ptr() & 15:           # (a view that begins inside a 16-byte piece)
         x = x.clone(memory_format=torch.preserve_format)
-    # (where both layouts are one -- a single position -- the channel axis is the contiguous one)
-    return x, int(last and x.shape[1] > 1 or x.numel() == x.shape[0] * x.shape[1])
+    return x, last
 
 
 def _gn_check(x, groups, weight, bias, relu):
-    _gpu_float(x, "x")
-    if x.dim() < 2:
-        raise ValueError(f"x: expected (N, C, *spatial), got {tuple(x.shape)}")
+    """-> groups, activation code, slope, the parameters' type code."""
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in _FLOAT_CODES):
+        _gpu_float(x, "x")           # raises
+    shape = x.shape
+    if len(shape) < 2:
+        raise ValueError(f"x: expected (N, C, *spatial), got {tuple(shape)}")
+    C_ = shape[1]
     groups = int(groups)
-    if groups <= 0 or x.shape[1] == 0 or x.shape[1] % groups:
-        raise ValueError(f"groups: {groups} do not divide {x.shape[1]} channels")
+    if groups <= 0 or C_ == 0 or C_ % groups:
+        raise ValueError(f"groups: {groups} do not divide {C_} channels")
+    code = None
     for t, name in ((weight, "weight"), (bias, "bias")):
         if t is None:
             continue
-        _gpu_float(t, name, x)
-        if tuple(t.shape) != (x.shape[1],):
-            raise ValueError(f"{name}: expected ({x.shape[1]},), got {tuple(t.shape)}")
-        if t.dtype not in (torch.float32, x.dtype):
+        if not (isinstance(t, torch.Tensor) and t.device == x.device and t.dtype in _FLOAT_CODES):
+            _gpu_float(t, name, x)
+        if t.shape != (C_,):
+            raise ValueError(f"{name}: expected ({C_},), got {tuple(t.shape)}")
+        if t.dtype is not torch.float32 and t.dtype is not x.dtype:
             raise TypeError(f"{name}: expected float32 or {x.dtype}, got {t.dtype}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError(f"weight and bias: {weight.dtype} and {bias.dtype}, expected one type")
+        mine = _FLOAT_CODES[t.dtype]
+        if code is not None and code != mine:
+            raise TypeError(f"weight and bias: {weight.dtype} and {bias.dtype}, expected one type")
+        code = mine
     if isinstance(relu, str):
         if relu != "silu":
             raise ValueError(f"relu: expected False, True, a slope or 'silu', got {relu!r}")
-        return groups, 1, 0.0
-    return groups, 0, _act_slope(relu)
+        return groups, 1, 0.0, code or 0
+    return groups, 0, _act_slope(relu), code or 0
 
 
-def _gn_param_code(x, weight, bias):
-    p = weight if weight is not None else bias
-    return 0 if p is None else _FLOAT_CODES[p.dtype]
+_GN_WORKSPACE = {}      # bmv_group_norm_workspace by its arguments (a few shapes a network; asked once each)
+
+
+def _gn_workspace(lib, key, device):
+    n = _GN_WORKSPACE.get(key)
+    if n is None:
+        n = lib.bmv_group_norm_workspace(*key)
+        if n < 0:
+            _lib.check(int(n), "group_norm_workspace")
+        if len(_GN_WORKSPACE) >= 4096:
+            _GN_WORKSPACE.clear()
+        _GN_WORKSPACE[key] = n
+    return torch.empty(n, device=device, dtype=torch.float64)
+
+
+def _region(name):
+    return ktimer.region(name) if ktimer.enabled else _NO_REGION
+
+
+_NO_REGION = contextlib.nullcontext()
+
+
+def group_norm_stats_fwd(x, groups, weight=None, bias=None, eps=1e-5, relu=False):
+    """`group_norm_fwd` with its statistics as one tensor: -> y, (2, N, groups) float64 (mean, rstd)."""
+    groups, act, slope, pcode = _gn_check(x, groups, weight, bias, relu)
+    if not eps >= 0:
+        raise ValueError(f"eps: {eps} is negative")
+    device = x.device
+    if device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return group_norm_stats_fwd(x, groups, weight, bias, eps, relu)
+    x, last = _gn_dense(x)
+    shape = x.shape
+    N, C_ = shape[0], shape[1]
+    y = torch.empty_like(x)
+    stats = torch.empty((2, N, groups), device=device, dtype=torch.float64)
+    numel = x.numel()
+    if numel == 0:
+        return y, stats.zero_()
+    S = numel // (N * C_)
+    last = 1 if S == 1 else last        # (a single position: both layouts are one, the channel axis the contiguous one)
+    weight, bias = weight if weight is None else _c(weight), bias if bias is None else _c(bias)
+    lib = _lib.load()
+    code = _FLOAT_CODES[x.dtype]
+    ws = _gn_workspace(lib, (N, C_, S, groups, code, last, 0), device)
+    mean = stats.data_ptr()
+    with _region("group_norm_fwd"):
+        rc = lib.bmv_group_norm_fwd(x.data_ptr(), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
+                                    N, C_, S, groups, code, pcode, last, float(eps), act, slope, ws.data_ptr(), mean,
+                                    mean + 8 * N * groups, y.data_ptr(), stream())
+    _lib.check(rc, "group_norm_fwd")
+    return y, stats
 
 
 def group_norm_fwd(x, groups, weight=None, bias=None, eps=1e-5, relu=False):
@@ -1425,66 +1476,53 @@ def group_norm_fwd(x, groups, weight=None, bias=None, eps=1e-5, relu=False):
     copied to planar): y = act((x - mean) / sqrt(var + eps) * weight + bias), statistics over a sample's C / groups channels.
     `relu`: False, True, a leaky slope, or "silu".  weight / bias (C): fp32 or x's type, or None.
     -> y (x's layout and type), mean, rstd (N, groups; float64, what `group_norm_bwd` reads)."""
-    groups, act, slope = _gn_check(x, groups, weight, bias, relu)
-    if not eps >= 0:
-        raise ValueError(f"eps: {eps} is negative")
-    with _on_device_of(x):
-        x, last = _gn_dense(x)
-        N, C_ = x.shape[:2]
-        S = x.numel() // max(1, N * C_)
-        y = torch.empty_like(x)
-        stats = torch.empty(2, N, groups, device=x.device, dtype=torch.float64)
-        mean, rstd = stats[0], stats[1]
-        if x.numel() == 0:
-            mean.zero_(), rstd.zero_()
-            return y, mean, rstd
-        lib = _lib.load()
-        code = _FLOAT_CODES[x.dtype]
-        n_ws = lib.bmv_group_norm_workspace(N, C_, S, groups, code, last, 0)
-        if n_ws < 0:
-            _lib.check(int(n_ws), "group_norm_workspace")
-        ws = torch.empty(n_ws, device=x.device, dtype=torch.float64)
-        with ktimer.region("group_norm_fwd"):
-            rc = lib.bmv_group_norm_fwd(_addr(x), _addr(weight if weight is None else _c(weight)), _addr(bias if bias is None else _c(bias)),
-                                        N, C_, S, groups, code, _gn_param_code(x, weight, bias), last, float(eps), act, slope,
-                                        _addr(ws), _addr(mean), _addr(rstd), _addr(y), stream())
-        _lib.check(rc, "group_norm_fwd")
-    return y, mean, rstd
+    y, stats = group_norm_stats_fwd(x, groups, weight, bias, eps, relu)
+    return (y, *stats.unbind())
+
+
+def group_norm_stats_bwd(x, dy, groups, weight, bias, stats, relu=False, want_params=True):
+    """`group_norm_bwd` with the statistics as `group_norm_stats_fwd` returns them."""
+    groups, act, slope, pcode = _gn_check(x, groups, weight, bias, relu)
+    if not (isinstance(dy, torch.Tensor) and dy.shape == x.shape and dy.dtype == x.dtype and dy.device == x.device):
+        _gpu_float(dy, "dy", x)
+        raise ValueError(f"dy: expected {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
+    device = x.device
+    if device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return group_norm_stats_bwd(x, dy, groups, weight, bias, stats, relu, want_params)
+    x, last = _gn_dense(x)
+    if dy.stride() != x.stride() or dy.data_ptr() & 15:
+        dy = torch.empty_like(x).copy_(dy)
+    shape = x.shape
+    N, C_ = shape[0], shape[1]
+    dx = torch.empty_like(x)
+    weight, bias = weight if weight is None else _c(weight), bias if bias is None else _c(bias)
+    dw = torch.empty_like(weight) if weight is not None and want_params else None
+    db = torch.empty_like(bias) if bias is not None and want_params else None
+    numel = x.numel()
+    if numel == 0:
+        return dx, dw if dw is None else dw.zero_(), db if db is None else db.zero_()
+    S = numel // (N * C_)
+    last = 1 if S == 1 else last
+    lib = _lib.load()
+    code = _FLOAT_CODES[x.dtype]
+    ws = _gn_workspace(lib, (N, C_, S, groups, code, last, 1), device)
+    mean = stats.data_ptr()
+    with _region("group_norm_bwd"):
+        rc = lib.bmv_group_norm_bwd(x.data_ptr(), dy.data_ptr(), None if weight is None else weight.data_ptr(),
+                                    None if bias is None else bias.data_ptr(), mean, mean + 8 * N * groups, N, C_, S, groups, code, pcode,
+                                    last, act, slope, ws.data_ptr(), dx.data_ptr(), None if dw is None else dw.data_ptr(),
+                                    None if db is None else db.data_ptr(), stream())
+    _lib.check(rc, "group_norm_bwd")
+    return dx, dw, db
 
 
 def group_norm_bwd(x, dy, groups, weight, bias, mean, rstd, relu=False, want_params=True):
     """-> dx (x's layout and type), dweight, dbias (C; None where weight / bias is None or not `want_params`)."""
-    groups, act, slope = _gn_check(x, groups, weight, bias, relu)
-    _gpu_float(dy, "dy", x)
-    if dy.shape != x.shape or dy.dtype != x.dtype:
-        raise ValueError(f"dy: expected {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
     for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if tuple(t.shape) != (x.shape[0], groups) or t.dtype != torch.float64 or t.device != x.device:
+        if not torch.is_tensor(t) or tuple(t.shape) != (x.shape[0], int(groups)) or t.dtype != torch.float64 or t.device != x.device:
             raise ValueError(f"{name}: expected ({x.shape[0]}, {groups}) float64 on {x.device}")
-    with _on_device_of(x):
-        x, last = _gn_dense(x)
-        if dy.stride() != x.stride() or dy.data_ptr() & 15:
-            dy = torch.empty_like(x).copy_(dy)
-        N, C_ = x.shape[:2]
-        S = x.numel() // max(1, N * C_)
-        dx = torch.empty_like(x)
-        dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if weight is not None and want_params else None
-        db = torch.empty_like(bias, memory_format=torch.contiguous_format) if bias is not None and want_params else None
-        if x.numel() == 0:
-            return dx, dw if dw is None else dw.zero_(), db if db is None else db.zero_()
-        lib = _lib.load()
-        code = _FLOAT_CODES[x.dtype]
-        n_ws = lib.bmv_group_norm_workspace(N, C_, S, groups, code, last, 1)
-        if n_ws < 0:
-            _lib.check(int(n_ws), "group_norm_workspace")
-        ws = torch.empty(n_ws, device=x.device, dtype=torch.float64)
-        with ktimer.region("group_norm_bwd"):
-            rc = lib.bmv_group_norm_bwd(_addr(x), _addr(dy), _addr(weight if weight is None else _c(weight)),
-                                        _addr(bias if bias is None else _c(bias)), _addr(_c(mean)), _addr(_c(rstd)), N, C_, S, groups, code,
-                                        _gn_param_code(x, weight, bias), last, act, slope, _addr(ws), _addr(dx), _addr(dw),
-                                        _addr(db), stream())
-        _lib.check(rc, "group_norm_bwd")
-    return dx, dw, db
+    return group_norm_stats_bwd(x, dy, groups, weight, bias, torch.stack((mean, rstd)), relu, want_params)
 
 
 NS_COEFFS = (3.4445, -4.7750, 2.0315)      # the quintic a s + b s^3 + c s^5 of a Newton-Schulz step
@@ -1563,9 +1601,9 @@ def newton_schulz(mats, steps=5, coeffs=NS_COEFFS, eps=NS_EPS):
             n = len(idx)
             rows, cols = _sides(sizes, idx)
             ws = _ns_workspace(lib, n, rows, cols, dtype, device)
-            with ktimer.region("newton_schulz"):
+            with _region("newton_schulz"):
                 rc = lib.bmv_newton_schulz(n, _pointers([mats[i] for i in idx]), _pointers([out[i] for i in idx]), rows, cols,
-                                           _FLOAT_CODES[dtype], steps, a, b, c, eps, _addr(ws), stream())
+                                           _FLOAT_CODES[dtype], steps, a, b, c, eps, ws.data_ptr(), stream())
             _lib.check(rc, "newton_schulz")
     return out
 
@@ -1609,10 +1647,10 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
             scales = (C.c_float * n)(*[lr * MUON_SCALES[scale](*sizes[i]) for i in idx])
             p, m = [_c(params[i]) for i in idx], [_c(momenta[i]) for i in idx]
             ws = _ns_workspace(lib, n, rows, cols, dtype, device)
-            with ktimer.region("muon_step"):
+            with _region("muon_step"):
                 rc = lib.bmv_muon_step(n, _pointers(p), _pointers([_c(grads[i]) for i in idx]), _pointers(m), rows, cols, scales,
                                        _FLOAT_CODES[dtype], float(momentum), int(bool(nesterov)), keep, steps, a, b, c, eps,
-                                       _addr(ws), stream())
+                                       ws.data_ptr(), stream())
             _lib.check(rc, "muon_step")
             for i, new in zip(idx, p):             # (weights of other strides went through a copy)
                 if new is not params[i]:

@@ -278,6 +278,15 @@ def test_group_norm_gradients_against_differences():
         assert abs(got - want) <= scale * (2 ** -20 + 1e-8), (k, got, want)
 
 
+@gpu
+def test_group_norm_refuses_a_second_differentiation():
+    from boostmvsnerfs_amd import autograd as A
+    x = torch.randn(1, 4, 5, 5, device="cuda", requires_grad=True)
+    dx, = torch.autograd.grad(A.GroupNormAct.apply(x, 2, None, None, 1e-5, "silu").sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="second differentiation"):
+        dx.sum().backward()
+
+
 def test_group_norm_refusals():
     from boostmvsnerfs_amd import ops
     x, w = torch.zeros(1, 4, 2, 2), torch.ones(4)
