@@ -15,6 +15,8 @@
 // What bounds it: bytes.  Two launches each way: sums of a chunk per workgroup -> partials; then every workgroup joins the
 // partials of the groups it touches (always in the same order: bit-reproducible, no atomics) and writes its chunk, which it
 // finds in its XCD's L2 or the last-level cache because the chunk -> workgroup map of both launches is the same.
+#include <algorithm>
+
 #include "bmv_common.hpp"
 
 namespace bmv {
@@ -60,6 +62,7 @@ struct GnArgs {
   long pcn, pck, pcc;
   int N, C, G, cg, wdt;
   int chunks, slabs, width;      // channel-last: row chunks, channel slabs of `width` channels.  planar: chunks of a plane
+  long per;                      // rows (values of a plane) of a chunk
   int pieces, npc;               // pieces a (sample, group) is joined from; pieces per channel of partc
   int slab_pieces;               // channel-last: slabs that share a group (1 where slabs hold whole groups)
   int dwb;                       // backward: workgroups behind the map's that finish dw and db
@@ -96,7 +99,7 @@ __device__ __forceinline__ bool gn_positive(float z, float dsc, float b, float x
 
 template <bool SILU>
 __device__ __forceinline__ float gn_act(float z, float slope) {
-  if (SILU) return z / (1.f + __expf(-z));
+  if (SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));      // (1 ulp; a division is ten instructions)
   return z > 0.f ? z : (slope == 0.f ? (z != z ? z : 0.f) : slope * z);   // (0 * -inf would be NaN)
 }
 
@@ -106,7 +109,7 @@ __device__ __forceinline__ float gn_grad(float dy, float x, float d, float sc, f
                                          double rstd) {
   const float dsc = d * sc, z = dsc + b;
   if (SILU) {
-    const float s = 1.f / (1.f + __expf(-z));
+    const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
     return dy * s * (1.f + z * (1.f - s));
   }
   if (slope == 1.f) return dy;
@@ -132,84 +135,116 @@ __device__ __forceinline__ GnCl gn_cl(const GnArgs& a, int bid) {
   t.wv = t.nch / V, t.rpi = kGnThreads / t.wv;
   t.r0 = threadIdx.x / t.wv, t.cv = threadIdx.x - t.r0 * t.wv;
   t.on = t.r0 < t.rpi, t.c = t.c0 + t.cv * V;
-  const long per = (a.S + a.chunks - 1) / a.chunks;
-  t.begin = min((long)t.k * per, a.S), t.end = min(t.begin + per, a.S);
+  t.begin = min(t.k * a.per, a.S), t.end = min(t.begin + a.per, a.S);
   return t;
 }
 
-// The workgroup's sums of E values per thread (E = 1: the thread's V channels together; V: each) -> a piece of every group
-// of the slab.  sh: kGnThreads * E double2.
+// A thread's V channels as E sums: 1 where they always lie in one group (C / G a multiple of V), 2 where groups have V channels
+// or more (what is in front of a group border, what is behind it), else V.
+// (cut: channels of the first up to its group's border)
 template <int V, int E>
-__device__ __forceinline__ void gn_cl_pieces(const GnArgs& a, const GnCl& t, double2* sh, bool groups) {
-  const int ne = t.wv * E;                          // entries of a row of the table
+__device__ __forceinline__ int gn_entry(int cut, int j) {
+  return E == V ? j : E == 1 ? 0 : j >= cut;
+}
+// the groups of channels c ... c + V - 1, one division
+template <int V>
+__device__ __forceinline__ void gn_group_of(int c, int cg, int* g) {
+  int k = c / cg, left = (k + 1) * cg - c;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (j && left == 0) ++k, left = cg;
+    g[j] = k, --left;
+  }
+}
+
+// sh: [row of the workgroup][vector of the slab][E] -> row 0: the sum over the workgroup's rows
+template <int TH>
+__device__ __forceinline__ void gn_cl_rows(const GnCl& t, int ne, double2* sh) {
   __syncthreads();
   int half = 1;
   while (half < t.rpi) half <<= 1;
   for (half >>= 1; half >= 1; half >>= 1) {          // rows r0 + half onto r0
-    for (int i = threadIdx.x; i < half * ne; i += kGnThreads)
+    for (int i = threadIdx.x; i < half * ne; i += TH)
       if (i + half * ne < t.rpi * ne) sh[i].x += sh[i + half * ne].x, sh[i].y += sh[i + half * ne].y;
     __syncthreads();
   }
-  if (!groups) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int g0 = t.c0 / a.cg, g1 = (t.c0 + t.nch - 1) / a.cg;
-  for (int g = g0 + wave; g <= g1; g += kGnWaves) {
+}
+// ... and of it, group by group of the slab: lane 0 of a wave hands the group's two sums to `to`
+template <int V, int E, int TH, typename F>
+__device__ __forceinline__ void gn_cl_groups(const GnArgs& a, const GnCl& t, const double2* sh, F to) {
+  const int lane = threadIdx.x & 63, g0 = t.c0 / a.cg, g1 = (t.c0 + t.nch - 1) / a.cg;
+  for (int g = g0 + (int)(threadIdx.x >> 6); g <= g1; g += TH / 64) {
     const int lo = max(g * a.cg, t.c0) - t.c0, hi = min((g + 1) * a.cg, t.c0 + t.nch) - t.c0;   // channels of the slab
-    const int step = V / E;
     double x = 0., y = 0.;
-    for (int i = lo / step + lane; i < hi / step; i += 64) x += sh[i].x, y += sh[i].y;
+    if (E == V)
+      for (int i = lo + lane; i < hi; i += 64) x += sh[i].x, y += sh[i].y;
+    else
+      for (int i = lo / V + lane; i <= (hi - 1) / V; i += 64) {
+        const double2 v = sh[i * E + (E == 2 && (t.c0 + i * V) / a.cg != g)];
+        x += v.x, y += v.y;
+      }
     x = gn_wave_sum(x), y = gn_wave_sum(y);
-    if (lane == 0) {
-      const int first = g * a.cg / a.width;          // the group's first slab
-      a.part[((long)t.n * a.G + g) * a.pieces + (t.slab - first) * a.chunks + t.k] = {x, y};
-    }
-  }
-  // (a group that fewer slabs share than others: its missing pieces are zero)
-  for (int g = g0 + (int)threadIdx.x; g <= g1; g += kGnThreads) {
-    const int first = g * a.cg / a.width, last = ((g + 1) * a.cg - 1) / a.width;
-    if (t.slab == last)
-      for (int s = last - first + 1; s < a.slab_pieces; ++s)
-        a.part[((long)t.n * a.G + g) * a.pieces + s * a.chunks + t.k] = {0., 0.};
+    if (lane == 0) to(g, x, y);
   }
 }
+// the workgroup's piece of every group of its slab
+template <int V, int E>
+__device__ __forceinline__ void gn_cl_pieces(const GnArgs& a, const GnCl& t, const double2* sh) {
+  gn_cl_groups<V, E, kGnThreads>(a, t, sh, [&](int g, double x, double y) {
+    const int first = g * a.cg / a.width, last = ((g + 1) * a.cg - 1) / a.width;      // the slabs that share the group
+    double2* to = a.part + ((long)t.n * a.G + g) * a.pieces + t.k;
+    to[(t.slab - first) * a.chunks] = {x, y};
+    if (t.slab == last)                              // (fewer than others share: the missing pieces are zero)
+      for (int k = last - first + 1; k < a.slab_pieces; ++k) to[k * a.chunks] = {0., 0.};
+  });
+}
 
-template <int DT, int V, bool ONE>
+template <int V, int E>
+__device__ __forceinline__ void gn_fold(const GnArgs& a, const GnCl& t, const double* s, const double* q, double2* sh) {
+  double2 v[E];
+  const int cut = (t.c / a.cg + 1) * a.cg - t.c;
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = {0., 0.};
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int at = gn_entry<V, E>(cut, j);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e == at) v[e].x += s[j], v[e].y += q[j];
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) sh[threadIdx.x * E + e] = v[e];
+}
+
+template <int DT, int V, int E>
 __global__ void __launch_bounds__(kGnThreads) gn_cl_stats_kernel(GnArgs a) {
   using T = typename GnType<DT>::T;
-  constexpr int E = ONE ? 1 : V;
   __shared__ double2 sh[kGnThreads * E];
   const GnCl t = gn_cl<V>(a, blockIdx.x);
   if (t.on) {
-    double s[E], q[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) s[e] = q[e] = 0.;
+    constexpr int A = E == 1 ? 1 : V;                // accumulators
+    double s[V] = {}, q[V] = {};
     const T* p = static_cast<const T*>(a.x) + (long)t.n * a.S * a.C + t.c;
     constexpr int U = 4;
-    long r = t.begin + t.r0;
-    for (; r + (U - 1) * t.rpi < t.end; r += U * t.rpi) {
+    for (long r = t.begin + t.r0; r < t.end; r += U * t.rpi) {
       GnVec<T, V> v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = gn_load<T, V>(p + (r + u * t.rpi) * a.C);
+      for (int u = 0; u < U; ++u) v[u] = gn_load<T, V>(p + min(r + u * t.rpi, t.end - 1) * a.C);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        if (r + u * t.rpi >= t.end) break;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const double f = (double)(float)v[u].v[j];
-          s[ONE ? 0 : j] += f, q[ONE ? 0 : j] += f * f;
+          s[A == 1 ? 0 : j] += f, q[A == 1 ? 0 : j] += f * f;
         }
-    }
-    for (; r < t.end; r += t.rpi) {
-      const GnVec<T, V> v = gn_load<T, V>(p + r * a.C);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const double f = (double)(float)v.v[j];
-        s[ONE ? 0 : j] += f, q[ONE ? 0 : j] += f * f;
       }
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) sh[threadIdx.x * E + e] = {s[e], q[e]};
+    if (E == 1) sh[threadIdx.x] = {s[0], q[0]};
+    else gn_fold<V, E>(a, t, s, q, sh);
   }
-  gn_cl_pieces<V, E>(a, t, sh, true);
+  gn_cl_rows<kGnThreads>(t, t.wv * E, sh);
+  gn_cl_pieces<V, E>(a, t, sh);
 }
 
 // one piece per (sample, group) out of many: in front of the apply launch where its workgroups would join too many
@@ -225,7 +260,20 @@ template <int DT, int V, bool SILU>
 __global__ void __launch_bounds__(kGnThreads) gn_cl_apply_kernel(GnArgs a) {
   using T = typename GnType<DT>::T;
   extern __shared__ GnStat st[];                     // the slab's groups
+  constexpr int U = 4;
   const GnCl t = gn_cl<V>(a, blockIdx.x);
+  const long off = (long)t.n * a.S * a.C + t.c;
+  const T* p = static_cast<const T*>(a.x) + off;
+  T* o = static_cast<T*>(a.out) + off;
+  // the first rows and the parameters are on their way while the partials are joined
+  GnVec<T, V> v[U];
+  float sc[V], b[V];
+  if (t.on && t.begin < t.end) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = gn_load<T, V>(p + min(t.begin + t.r0 + u * t.rpi, t.end - 1) * a.C);
+#pragma unroll
+    for (int j = 0; j < V; ++j) sc[j] = gn_param<T>(a.w, t.c + j, a.wdt, 1.f), b[j] = gn_param<T>(a.b, t.c + j, a.wdt, 0.f);
+  }
   const int g0 = t.c0 / a.cg, g1 = (t.c0 + t.nch - 1) / a.cg;
   for (int g = g0 + (threadIdx.x >> 6); g <= g1; g += kGnWaves) {
     const long i = (long)t.n * a.G + g;
@@ -237,36 +285,101 @@ __global__ void __launch_bounds__(kGnThreads) gn_cl_apply_kernel(GnArgs a) {
   }
   __syncthreads();
   if (!t.on) return;
-  float mh[V], ml[V], sc[V], b[V];
+  float mh[V], ml[V];
+  int g[V];
+  gn_group_of<V>(t.c, a.cg, g);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const GnStat s = st[(t.c + j) / a.cg - g0];
-    mh[j] = (float)s.mean, ml[j] = (float)(s.mean - (double)mh[j]);
-    sc[j] = (float)(s.rstd * (double)gn_param<T>(a.w, t.c + j, a.wdt, 1.f)), b[j] = gn_param<T>(a.b, t.c + j, a.wdt, 0.f);
+    const GnStat s = st[g[j] - g0];
+    mh[j] = (float)s.mean, ml[j] = (float)(s.mean - (double)mh[j]), sc[j] = (float)(s.rstd * (double)sc[j]);
   }
-  const long off = (long)t.n * a.S * a.C + t.c;
-  const T* p = static_cast<const T*>(a.x) + off;
-  T* o = static_cast<T*>(a.out) + off;
-  constexpr int U = 4;
-  long r = t.begin + t.r0;
-  for (; r + (U - 1) * t.rpi < t.end; r += U * t.rpi) {
-    GnVec<T, V> v[U];
+  for (long r = t.begin + t.r0; r < t.end; r += U * t.rpi) {
+    GnVec<T, V> w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = gn_load<T, V>(p + (r + u * t.rpi) * a.C);
+    for (int u = 0; u < U; ++u) w[u] = v[u];
+    if (r + U * t.rpi < t.end) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = gn_load<T, V>(p + min(r + (U + u) * t.rpi, t.end - 1) * a.C);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (r + u * t.rpi >= t.end) break;
       float f[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) f[j] = gn_act<SILU>((((float)v[u].v[j] - mh[j]) - ml[j]) * sc[j] + b[j], a.slope);
+      for (int j = 0; j < V; ++j) f[j] = gn_act<SILU>((((float)w[u].v[j] - mh[j]) - ml[j]) * sc[j] + b[j], a.slope);
       gn_store<T, V>(o + (r + u * t.rpi) * a.C, f);
     }
   }
-  for (; r < t.end; r += t.rpi) {
-    const GnVec<T, V> v = gn_load<T, V>(p + r * a.C);
+}
+
+// A whole (sample, slab of groups) in the registers of one workgroup, R accesses a thread: one launch instead of two
+constexpr int kGnHold = 8;
+template <int DT, int V, int E, int TH, bool SILU>
+__global__ void __launch_bounds__(TH) gn_cl_whole_kernel(GnArgs a) {
+  using T = typename GnType<DT>::T;
+  constexpr int R = kGnHold;
+  __shared__ double2 sh[TH * E];
+  extern __shared__ GnStat st[];                     // the slab's groups
+  GnCl t = gn_cl<V>(a, blockIdx.x);
+  t.rpi = TH / t.wv, t.on = t.r0 < t.rpi;            // (gn_cl counts 256 threads)
+  const long off = (long)t.n * a.S * a.C + t.c;
+  const T* p = static_cast<const T*>(a.x) + off;
+  GnVec<T, V> v[R];
+  double s[V] = {}, q[V] = {};
+  if (t.on) {
+#pragma unroll
+    for (int u = 0; u < R; ++u) v[u] = gn_load<T, V>(p + min((long)t.r0 + u * t.rpi, a.S - 1) * a.C);
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      if (t.r0 + u * t.rpi >= a.S) break;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const double f = (double)(float)v[u].v[j];
+        s[E == 1 ? 0 : j] += f, q[E == 1 ? 0 : j] += f * f;
+      }
+    }
+  }
+  const int g0 = t.c0 / a.cg;
+  if (E == 1 && a.width == a.cg) {                   // one group: a sum over all threads
+    const double x = gn_wave_sum(s[0]), y = gn_wave_sum(q[0]);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = {x, y};
+    __syncthreads();
+    double2 sum = {0., 0.};
+#pragma unroll
+    for (int i = 0; i < TH / 64; ++i) sum.x += sh[i].x, sum.y += sh[i].y;
+    const GnStat m = gn_stat(sum, (double)a.M, a.eps);
+    if (threadIdx.x == 0) st[0] = m, a.mean[(long)t.n * a.G + g0] = m.mean, a.rstd[(long)t.n * a.G + g0] = m.rstd;
+  } else {
+    if (t.on) {
+      if (E == 1) sh[threadIdx.x] = {s[0], q[0]};
+      else gn_fold<V, E>(a, t, s, q, sh);
+    }
+    gn_cl_rows<TH>(t, t.wv * E, sh);
+    gn_cl_groups<V, E, TH>(a, t, sh, [&](int g, double x, double y) {
+      const GnStat m = gn_stat({x, y}, (double)a.M, a.eps);
+      st[g - g0] = m;
+      a.mean[(long)t.n * a.G + g] = m.mean, a.rstd[(long)t.n * a.G + g] = m.rstd;
+    });
+  }
+  __syncthreads();
+  if (!t.on) return;
+  float mh[V], ml[V], sc[V], b[V];
+  int gs[V];
+  gn_group_of<V>(t.c, a.cg, gs);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const GnStat m = st[gs[j] - g0];
+    mh[j] = (float)m.mean, ml[j] = (float)(m.mean - (double)mh[j]);
+    sc[j] = (float)(m.rstd * (double)gn_param<T>(a.w, t.c + j, a.wdt, 1.f)), b[j] = gn_param<T>(a.b, t.c + j, a.wdt, 0.f);
+  }
+  T* o = static_cast<T*>(a.out) + off;
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    if (t.r0 + u * t.rpi >= a.S) break;
     float f[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = gn_act<SILU>((((float)v.v[j] - mh[j]) - ml[j]) * sc[j] + b[j], a.slope);
-    gn_store<T, V>(o + r * a.C, f);
+    for (int j = 0; j < V; ++j) f[j] = gn_act<SILU>((((float)v[u].v[j] - mh[j]) - ml[j]) * sc[j] + b[j], a.slope);
+    gn_store<T, V>(o + ((long)t.r0 + u * t.rpi) * a.C, f);
   }
 }
 
@@ -278,9 +391,11 @@ __global__ void __launch_bounds__(kGnThreads) gn_cl_bwd_reduce_kernel(GnArgs a) 
   if (t.on) {
     float mh[V], ml[V], sc[V], b[V], w[V];
     double mean[V], rstd[V], s[V], q[V];
+    int gs[V];
+    gn_group_of<V>(t.c, a.cg, gs);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const long i = (long)t.n * a.G + (t.c + j) / a.cg;
+      const long i = (long)t.n * a.G + gs[j];
       mean[j] = a.mean[i], rstd[j] = a.rstd[i], s[j] = q[j] = 0.;
       mh[j] = (float)mean[j], ml[j] = (float)(mean[j] - (double)mh[j]);
       w[j] = gn_param<T>(a.w, t.c + j, a.wdt, 1.f), b[j] = gn_param<T>(a.b, t.c + j, a.wdt, 0.f);
@@ -312,7 +427,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_cl_bwd_reduce_kernel(GnArgs a) 
 #pragma unroll
     for (int j = 0; j < V; ++j) sh[threadIdx.x * V + j] = {s[j], q[j] * rstd[j]};
   }
-  gn_cl_pieces<V, V>(a, t, sh, false);
+  gn_cl_rows<kGnThreads>(t, t.nch, sh);
   for (int i = threadIdx.x; i < t.nch; i += kGnThreads) {
     const double2 v = sh[i];
     const int c = t.c0 + i;
@@ -320,9 +435,8 @@ __global__ void __launch_bounds__(kGnThreads) gn_cl_bwd_reduce_kernel(GnArgs a) 
     const double w = (double)gn_param<T>(a.w, c, a.wdt, 1.f);
     sh[i] = {v.x * w, v.y * w};
   }
-  GnCl one = t;
-  one.rpi = 1;
-  gn_cl_pieces<V, V>(a, one, sh, true);
+  __syncthreads();
+  gn_cl_pieces<V, V>(a, t, sh);
 }
 
 // dw and db out of the pieces: 8 channels a workgroup, 32 threads each, the samples and pieces of a channel in a fixed order
@@ -356,37 +470,54 @@ __global__ void __launch_bounds__(kGnThreads) gn_cl_bwd_apply_kernel(GnArgs a) {
   using T = typename GnType<DT>::T;
   extern __shared__ double2 sg[];                    // the slab's groups: the two sums over M
   if ((int)blockIdx.x < a.dwb) return gn_param_grads<DT>(a, blockIdx.x);
+  constexpr int U = 4;
   const GnCl t = gn_cl<V>(a, blockIdx.x - a.dwb);
+  const long off = (long)t.n * a.S * a.C + t.c;
+  const T *p = static_cast<const T*>(a.x) + off, *pd = static_cast<const T*>(a.dy) + off;
+  T* o = static_cast<T*>(a.out) + off;
+  // the first rows, the statistics and the parameters are on their way while the partials are joined
+  GnVec<T, V> v[U], e[U];
+  float w[V], b[V];
+  double mean[V], rstd[V];
+  int gs[V];
+  if (t.on && t.begin < t.end) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long at = min(t.begin + t.r0 + u * t.rpi, t.end - 1) * a.C;
+      v[u] = gn_load<T, V>(p + at), e[u] = gn_load<T, V>(pd + at);
+    }
+    gn_group_of<V>(t.c, a.cg, gs);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const long i = (long)t.n * a.G + gs[j];
+      mean[j] = a.mean[i], rstd[j] = a.rstd[i];
+      w[j] = gn_param<T>(a.w, t.c + j, a.wdt, 1.f), b[j] = gn_param<T>(a.b, t.c + j, a.wdt, 0.f);
+    }
+  }
   const int g0 = t.c0 / a.cg, g1 = (t.c0 + t.nch - 1) / a.cg;
   for (int g = g0 + (threadIdx.x >> 6); g <= g1; g += kGnWaves) {
     const double2 s = gn_join(a.part + ((long)t.n * a.G + g) * a.pieces, a.pieces);
     if ((threadIdx.x & 63) == 0) sg[g - g0] = {s.x / (double)a.M, s.y / (double)a.M};
   }
   __syncthreads();
-  if (!t.on) return;
+  if (!t.on || t.begin >= t.end) return;
   // dx = rstd w g - rstd m1 - (x - mean) rstd^2 m2
-  float mh[V], ml[V], sc[V], b[V], w[V], c1[V], c2[V];
-  double mean[V], rstd[V];
+  float mh[V], ml[V], sc[V], c1[V], c2[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int g = (t.c + j) / a.cg;
-    const long i = (long)t.n * a.G + g;
-    mean[j] = a.mean[i], rstd[j] = a.rstd[i];
+    const double2 m = sg[gs[j] - g0];
     mh[j] = (float)mean[j], ml[j] = (float)(mean[j] - (double)mh[j]);
-    w[j] = gn_param<T>(a.w, t.c + j, a.wdt, 1.f), b[j] = gn_param<T>(a.b, t.c + j, a.wdt, 0.f);
     sc[j] = (float)(rstd[j] * (double)w[j]);
-    c1[j] = (float)(rstd[j] * sg[g - g0].x), c2[j] = (float)(rstd[j] * rstd[j] * sg[g - g0].y);
+    c1[j] = (float)(rstd[j] * m.x), c2[j] = (float)(rstd[j] * rstd[j] * m.y);
   }
-  const long off = (long)t.n * a.S * a.C + t.c;
-  const T *p = static_cast<const T*>(a.x) + off, *pd = static_cast<const T*>(a.dy) + off;
-  T* o = static_cast<T*>(a.out) + off;
-  constexpr int U = 4;
   for (long r = t.begin + t.r0; r < t.end; r += U * t.rpi) {
-    GnVec<T, V> v[U], e[U];
+    GnVec<T, V> vn[U], en[U];
+    if (r + U * t.rpi < t.end) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long ru = min(r + u * t.rpi, t.end - 1);
-      v[u] = gn_load<T, V>(p + ru * a.C), e[u] = gn_load<T, V>(pd + ru * a.C);
+      for (int u = 0; u < U; ++u) {
+        const long at = min(r + (U + u) * t.rpi, t.end - 1) * a.C;
+        vn[u] = gn_load<T, V>(p + at), en[u] = gn_load<T, V>(pd + at);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -400,6 +531,8 @@ __global__ void __launch_bounds__(kGnThreads) gn_cl_bwd_apply_kernel(GnArgs a) {
       }
       gn_store<T, V>(o + (r + u * t.rpi) * a.C, f);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = vn[u], e[u] = en[u];
   }
 }
 
@@ -414,13 +547,13 @@ struct GnPl {
 template <int TPU>
 __device__ __forceinline__ GnPl gn_pl(const GnArgs& a, long bid) {
   GnPl p;
-  const long unit = bid * (kGnThreads / TPU) + (TPU == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
-  p.on = unit < (long)a.N * a.C * a.chunks;
+  const unsigned unit = (unsigned)bid * (kGnThreads / TPU) + (TPU == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  p.on = unit < (unsigned)a.N * a.C * a.chunks;           // (fewer than 2^32: gn_bad_shape)
   p.t = threadIdx.x & (TPU - 1);
-  p.k = (int)(unit % a.chunks), p.plane = unit / a.chunks;
-  p.c = (int)(p.plane % a.C), p.n = (int)(p.plane / a.C);
-  const long per = ((a.S + a.chunks - 1) / a.chunks + 15) & ~15l;      // chunks begin at 16-byte borders of the plane
-  p.begin = min((long)p.k * per, a.S), p.end = min(p.begin + per, a.S);
+  const unsigned plane = unit / a.chunks;
+  p.k = (int)(unit - plane * a.chunks), p.plane = plane;
+  p.n = (int)(plane / a.C), p.c = (int)(plane - (unsigned)p.n * a.C);
+  p.begin = min(p.k * a.per, a.S), p.end = min(p.begin + a.per, a.S);      // (chunks begin at 16-byte borders of the plane)
   return p;
 }
 // sum over the unit; every thread of a wave-unit, thread 0 of a workgroup-unit has it
@@ -493,6 +626,51 @@ __global__ void __launch_bounds__(kGnThreads) gn_pl_apply_kernel(GnArgs a) {
 #pragma unroll
     for (int j = 0; j < V; ++j) f[j] = gn_act<SILU>((((float)v.v[j] - mh) - ml) * sc + b, a.slope);
     gn_store<T, V>(o + i, f);
+  }
+}
+
+// A whole (sample, group) -- one run of C / G planes -- in the registers of one workgroup
+template <int DT, int V, int TH, bool SILU>
+__global__ void __launch_bounds__(TH) gn_pl_whole_kernel(GnArgs a) {
+  using T = typename GnType<DT>::T;
+  constexpr int R = kGnHold;
+  __shared__ double2 sh[TH / 64];
+  const int n = blockIdx.x / a.G, g = blockIdx.x - n * a.G, sv = (int)(a.S / V), nv = a.cg * sv;      // accesses of a plane, of the group
+  const long off = ((long)n * a.C + (long)g * a.cg) * a.S;
+  const T* p = static_cast<const T*>(a.x) + off;
+  GnVec<T, V> v[R];
+  double s = 0., q = 0.;
+#pragma unroll
+  for (int u = 0; u < R; ++u) v[u] = gn_load<T, V>(p + (long)min((int)threadIdx.x + u * TH, nv - 1) * V);
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    if ((int)threadIdx.x + u * TH >= nv) break;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const double f = (double)(float)v[u].v[j];
+      s += f, q += f * f;
+    }
+  }
+  s = gn_wave_sum(s), q = gn_wave_sum(q);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = {s, q};
+  __syncthreads();
+  s = q = 0.;
+#pragma unroll
+  for (int i = 0; i < TH / 64; ++i) s += sh[i].x, q += sh[i].y;
+  const GnStat m = gn_stat({s, q}, (double)a.M, a.eps);
+  if (threadIdx.x == 0) a.mean[blockIdx.x] = m.mean, a.rstd[blockIdx.x] = m.rstd;
+  const float mh = (float)m.mean, ml = (float)(m.mean - (double)mh);
+  T* o = static_cast<T*>(a.out) + off;
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    const int i = threadIdx.x + u * TH;
+    if (i >= nv) break;
+    const int c = g * a.cg + i / sv;
+    const float sc = (float)(m.rstd * (double)gn_param<T>(a.w, c, a.wdt, 1.f)), b = gn_param<T>(a.b, c, a.wdt, 0.f);
+    float f[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = gn_act<SILU>((((float)v[u].v[j] - mh) - ml) * sc + b, a.slope);
+    gn_store<T, V>(o + (long)i * V, f);
   }
 }
 
@@ -571,6 +749,7 @@ constexpr int kGnMaxJoin = 1024;      // double2 that a workgroup of the apply l
 struct GnPlan {
   GnArgs a;
   int V, tpu;
+  int whole, held;                     // forward in one launch: its workgroups' threads, or 0; channels that one holds
   bool last, finish;
   long wgs, part, partc, fin;          // workgroups of the map; double2 of the workspace's three parts
 };
@@ -580,6 +759,8 @@ static int gn_vec(long n, int size) {  // values per access: 16 bytes where the 
     if (n % v == 0) return v;
   return 1;
 }
+// threads of a workgroup that holds `accesses` of them, kGnHold a thread; 0: too many
+static int gn_whole(long accesses) { return accesses <= 256 * kGnHold ? 256 : accesses <= 1024 * kGnHold ? 1024 : 0; }
 
 static GnPlan gn_plan(int N, int C, long S, int G, int dtype, int last) {
   GnPlan p{};
@@ -590,54 +771,101 @@ static GnPlan gn_plan(int N, int C, long S, int G, int dtype, int last) {
   if (p.last) {
     p.V = gn_vec(C, size);
     const int cv = C / p.V;
-    // slabs: as many threads of the 256 at work as possible, whole groups where they fit
-    int best = 0, wv = cv;
-    for (int k = (cv + kGnThreads - 1) / kGnThreads; k <= (cv + kGnThreads - 1) / kGnThreads + 3; ++k) {
-      int w = (cv + k - 1) / k;
-      const int unit = a.cg % p.V == 0 ? a.cg / p.V : a.cg;        // vectors from one group border to the next on a vector border
-      if (unit <= kGnThreads && (w + unit - 1) / unit * unit <= kGnThreads) w = (w + unit - 1) / unit * unit;
-      if (w > cv) w = cv;
-      const int used = kGnThreads / w * w;
-      if (used > best + 16) best = used, wv = w;
+    // A slab is whole groups where 256 accesses hold one: the fewest that are 128 bytes of a row (a cache line), or the number
+    // among the next three that leaves the fewest of the 256 threads without a column.  Wide groups are cut in equal slabs.
+    int unit = a.cg / p.V;             // accesses from one group border that is an access border to the next
+    if (a.cg % p.V) {
+      int lcm = a.cg;
+      while (lcm % p.V) lcm += a.cg;
+      unit = lcm / p.V;
+    }
+    int wv;
+    if (unit > kGnThreads) {
+      const int k = (cv + kGnThreads - 1) / kGnThreads;
+      wv = (cv + k - 1) / k;
+    } else {
+      const int line = (128 / (p.V * size) + unit - 1) / unit;
+      int best = -1;
+      wv = unit;
+      for (int k = line; k < line + 4; ++k) {
+        const int w = std::min(unit * k, cv), used = w <= kGnThreads ? kGnThreads / w * w : 0;
+        if (used > best + 8) best = used, wv = w;
+      }
+      if (best <= 0) wv = unit;
     }
     a.width = wv * p.V, a.slabs = (C + a.width - 1) / a.width;
     a.slab_pieces = 1;
-    for (int g = 0; g < G; ++g) {
-      const int shared = ((g + 1) * a.cg - 1) / a.width - g * a.cg / a.width + 1;
-      if (shared > a.slab_pieces) a.slab_pieces = shared;
-    }
-    long chunks = (S * wv + kGnThreads * 8 - 1) / (kGnThreads * 8);
-    long cap = 2048 / ((long)N * a.slabs);
-    if (cap < 1) cap = 1;
-    if (chunks > cap) chunks = cap;
-    if (chunks < 1) chunks = 1;
+    if (a.width % a.cg)
+      for (int g = 0; g < G; ++g) {
+        const int shared = ((g + 1) * a.cg - 1) / a.width - g * a.cg / a.width + 1;
+        if (shared > a.slab_pieces) a.slab_pieces = shared;
+      }
+    // rows of a chunk: about 1024 workgroups (four on a compute unit), of at least 2 accesses a thread
+    const long rpi = kGnThreads / wv, wgs = std::max(1l, 1024 / ((long)N * a.slabs));
+    a.per = std::max(2 * rpi, ((S + wgs - 1) / wgs + rpi - 1) / rpi * rpi);
+    const long chunks = (S + a.per - 1) / a.per;
     a.chunks = (int)chunks, a.pieces = a.chunks * a.slab_pieces, a.npc = a.chunks;
     a.pcn = (long)a.chunks * C, a.pck = C, a.pcc = 1;
     p.wgs = (long)N * a.slabs * a.chunks;
     const long touched = (a.width + a.cg - 1) / a.cg + 1;
-    p.finish = (touched < G ? touched : G) * a.pieces > kGnMaxJoin;
+    p.finish = std::min<long>(touched, G) * a.pieces > kGnMaxJoin;
+    // (one launch: the fewest channels that are whole groups and whole accesses; kGnHold passes of threads / accesses rows)
+    if (unit <= kGnThreads) {
+      p.held = unit * p.V;
+      p.whole = S <= 256 / unit * kGnHold ? 256 : S <= 1024 / unit * kGnHold && (a.cg % p.V == 0 || a.cg >= p.V) ? 1024 : 0;
+    }
   } else {
     p.V = gn_vec(S, size);
     p.tpu = S >= 4096 ? 256 : 64;
-    long chunks = (S + p.tpu * p.V * 8 - 1) / (p.tpu * p.V * 8);
+    long chunks = (S + p.tpu * p.V * 4 - 1) / (p.tpu * p.V * 4);
     long cap = 2048 / ((long)N * C) * (256 / p.tpu);
     if (cap < 1) cap = 1;
     if (chunks > cap) chunks = cap;
+    a.per = ((S + chunks - 1) / chunks + 15) & ~15l;
     a.chunks = (int)chunks, a.pieces = a.cg * a.chunks, a.npc = a.chunks;
     a.pcn = (long)C * a.chunks, a.pck = 1, a.pcc = a.chunks;
     p.wgs = ((long)N * C * a.chunks * p.tpu + 255) / 256;
     p.finish = a.pieces > (p.tpu == 64 ? kGnMaxJoin / 4 : kGnMaxJoin);
+    p.whole = gn_whole(a.M / p.V);
   }
   p.part = (long)N * G * a.pieces, p.fin = p.finish ? (long)N * G : 0, p.partc = (long)N * C * a.npc;
   return p;
 }
 
+template <int DT, int V, bool SILU>
+static void gn_whole_launch(const GnPlan& p, const GnArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)((long)a.N * (p.last ? a.C / p.held : a.G)));
+  if (!p.last) {
+    if (p.whole == 256) hipLaunchKernelGGL((gn_pl_whole_kernel<DT, V, 256, SILU>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((gn_pl_whole_kernel<DT, V, 1024, SILU>), grid, dim3(1024), 0, st, a);
+    return;
+  }
+  GnArgs b = a;
+  b.chunks = 1, b.width = p.held, b.slabs = a.C / p.held;
+  const unsigned lds = (unsigned)(p.held / a.cg) * sizeof(GnStat);
+#define BMV_GN_WHOLE(E, TH) hipLaunchKernelGGL((gn_cl_whole_kernel<DT, V, E, TH, SILU>), grid, dim3(TH), lds, st, b)
+  if (a.cg % V == 0) {
+    if (p.whole == 256) BMV_GN_WHOLE(1, 256);
+    else BMV_GN_WHOLE(1, 1024);
+  } else if (a.cg >= V) {
+    if (p.whole == 256) BMV_GN_WHOLE((V < 2 ? 1 : 2), 256);
+    else BMV_GN_WHOLE((V < 2 ? 1 : 2), 1024);
+  } else BMV_GN_WHOLE(V, 256);
+#undef BMV_GN_WHOLE
+}
+
 template <int DT, int V>
 static void gn_fwd_launch(const GnPlan& p, GnArgs a, bool silu, hipStream_t st) {
+  if (p.whole) {
+    if (silu) gn_whole_launch<DT, V, true>(p, a, st);
+    else gn_whole_launch<DT, V, false>(p, a, st);
+    return;
+  }
   const dim3 grid((unsigned)p.wgs), block(kGnThreads);
   if (p.last) {
-    if (a.cg % V == 0) hipLaunchKernelGGL((gn_cl_stats_kernel<DT, V, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((gn_cl_stats_kernel<DT, V, false>), grid, block, 0, st, a);
+    if (a.cg % V == 0) hipLaunchKernelGGL((gn_cl_stats_kernel<DT, V, 1>), grid, block, 0, st, a);
+    else if (a.cg >= V) hipLaunchKernelGGL((gn_cl_stats_kernel<DT, V, (V < 2 ? 1 : 2)>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((gn_cl_stats_kernel<DT, V, V>), grid, block, 0, st, a);
   } else if (p.tpu == 256) hipLaunchKernelGGL((gn_pl_stats_kernel<DT, V, 256>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((gn_pl_stats_kernel<DT, V, 64>), grid, block, 0, st, a);
   if (p.finish) {

@@ -107,7 +107,10 @@ def _check(x, dy, G, w, b, relu, layout, eps=1e-5, dtype=None):
 # row chunks that end ragged
 SHAPES = [(1, 4, (1, 1), 2), (2, 3, (1, 1), 3), (1, 8, (5, 7), 8), (2, 6, (9, 5), 3), (3, 30, (13, 11), 5), (1, 64, (8, 8, 10), 8),
           (2, 320, (9, 9), 32), (1, 1030, (3, 5), 1), (1, 2080, (2, 3), 5), (2, 520, (7,), 4), (1, 7, (129, 131), 1),
-          (1, 12, (3, 4099), 4), (5, 24, (1, 17), 24), (1, 1, (33, 3), 1)]
+          (1, 12, (3, 4099), 4), (5, 24, (1, 17), 24), (1, 1, (33, 3), 1),
+          # one launch by 256 and 1024 threads, and just too large for either; groups across the borders of 16-byte accesses
+          (2, 8, (32, 32), 2), (2, 8, (32, 33), 2), (2, 8, (64, 64), 2), (2, 8, (64, 65), 2), (2, 60, (21, 20), 6), (1, 24, (90, 31), 8),
+          (2, 320, (64, 5), 32), (1, 40, (23, 29), 8), (1, 96, (7, 300), 2)]
 
 
 @gpu
