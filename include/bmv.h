@@ -365,7 +365,8 @@ int bmv_group_norm_bwd(const void* x, const void* dy, const void* weight, const 
  * Newton-Schulz iteration of `count` matrices src[i] (rows[i], cols[i]), row-major, contiguous, all of `dtype` (0 fp32, 1 bf16,
  * 2 fp16) -> dst[i]: X = src / max(|src|_F, eps), then `steps` times A = X X^T, X = a X + (b A + c A A) X (on the transpose
  * where rows > cols).  operands of 24 bits (bf16: 17), one rounding at the end; a non-finite value makes its matrix NaN and
- * leaves the others alone.  The arrays are HOST arrays, read before the call returns; eps >= 1e-12, sides up to 65536.
+ * leaves the others alone.  Reproducible; a matrix' last bits depend on what else is in the list (where sums are cut).  The arrays are
+ * HOST arrays, read before the call returns; eps >= 1e-12, sides up to 65536.
  * workspace: bmv_newton_schulz_workspace(...) bytes, beginning at a 256-byte border. */
 long bmv_newton_schulz_workspace(int count, const int* rows, const int* cols, int dtype);
 int bmv_newton_schulz(int count, const void* const* src, void* const* dst, const int* rows, const int* cols, int dtype, int steps,

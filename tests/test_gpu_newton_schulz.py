@@ -87,9 +87,12 @@ def test_newton_schulz_matches_the_formula(dtype, way):
     for got, u, src, keep in zip(out, mats, on_gpu, before):
         assert got.shape == u.shape and got.dtype == dtype and torch.equal(src, keep)
         _check(got, u)
-    # one call for the list, one call each: the same
-    for got, src in zip(out, on_gpu):
-        assert torch.equal(ops.newton_schulz(src), got), src.shape
+    # the same call again is the same bit for bit; a matrix alone is cut along k in other places (sums of fp32 in another order),
+    # so it agrees within the tolerance
+    for got, again in zip(out, ops.newton_schulz(on_gpu)):
+        assert torch.equal(got, again), got.shape
+    for src, u in zip(on_gpu, mats):
+        _check(ops.newton_schulz(src), u)
 
 
 @gpu
