@@ -43,6 +43,7 @@ constexpr int kNsTile = 128;     // output tile of a workgroup; matrices are pad
 constexpr int kNsK = 16;         // k-values of a stage
 constexpr int kNsCell = 2048;    // elements of a piece of a block: 128 rows of 16 k-values
 constexpr int kNsChunk = 8192;   // elements of a workgroup of the norm
+constexpr int kNsUnits = 256, kNsLdsBytes = 160 * 1024;    // compute units, LDS of one
 constexpr int kNsSlots = 512;    // workgroups that run at once: two on each of 256 compute units
 constexpr int kNsRun = 4;        // stages of the shortest run that a workgroup is started for
 
@@ -61,6 +62,7 @@ struct NsArgs {
   double* sq;           // partial sums of squares: [item][chunk], kNsList * sqn of them
   float* part;          // partial tiles
   int count, sqn, dtype, muon, nesterov, first, last, flip;
+  int least;            // short sides: columns of a workgroup at least
   int full, run;        // a product's tiles that are a workgroup each; stages of a run of the others
   float a, b, c, eps, mu, nu, keep;      // nu: 1 - mu, rounded once
 };
@@ -432,11 +434,21 @@ __global__ void __launch_bounds__(256) ns_join_kernel(NsArgs g) {
 // products are too small for the split of the operands to pay.
 // LDS rows are m + 4 floats (m a multiple of 16): rows 4 apart are 16 banks apart, which keeps both the 16-byte reads along k
 // (16 rows, one k) and the 4-byte reads across rows (16 values of rows 4 apart) free of conflicts.
-constexpr int kNsShort = 128, kNsShortLong = 4096;      // short and long side up to which this way is taken
+// T.  A step costs a workgroup 0.19 us (m = 128; 0.07 at 64) for each of its columns and 0.34 us (0.12) for each of the n / T
+// shares of A that it adds up, measured over 16, 32 and 64 columns: T^2 = 1.7 n or so for either, the power of two next to it --
+// unless the list then has more workgroups than fit the card at once: more columns each are cheaper than a second round.  (64
+// columns of more than 64 rows would be four blocks a wave: 10 % slower at 128 x 2048 than 32.)
+// Long sides: the shares that everybody adds up grow with n^2.  128 x 4096 285 us (through the large matrices' way 295),
+// 128 x 8192 515 (438); 64 x 8192 130 (437).
+constexpr int kNsShort = 128, kNsShortLong = 16384;      // short side, and long side (a quarter of it above 64 rows), up to which this way is taken
+__host__ __device__ __forceinline__ int ns_columns(int m, int n, int least) {
+  const int t = n <= 288 ? 16 : n <= 1152 ? 32 : 64, u = t > least ? t : least;
+  return m > 64 && u > 32 ? 32 : u;
+}
 struct NsShort {
   int m, n, mp, mb, T, parts, blocks, pitch;            // m in 16s: mp = 16 mb; columns of a workgroup; workgroups; 16 x 16 blocks of A's lower triangle
-  __host__ __device__ NsShort(const NsShape& s) {
-    m = s.m, n = s.n, mp = (m + 15) & ~15, mb = mp / 16, T = mp <= 64 ? 64 : 32;
+  __host__ __device__ NsShort(const NsShape& s, int least) {
+    m = s.m, n = s.n, mp = (m + 15) & ~15, mb = mp / 16, T = ns_columns(m, n, least);
     parts = (n + T - 1) / T, blocks = mb * (mb + 1) / 2, pitch = mp + 4;
   }
   __host__ __device__ long x() const { return (long)n * mp; }                     // floats of X^T
@@ -457,7 +469,7 @@ __global__ void __launch_bounds__(512) ns_short_kernel(NsArgs g) {
   const int i = ns_find(g, blockIdx.x);
   const NsItem it = g.it[i];
   const NsShape shape(it.rows, it.cols);
-  const NsShort s(shape);
+  const NsShort s(shape, g.least);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, c16 = lane & 15;
   const int wg = blockIdx.x - it.at, j0 = wg * s.T, nj = min(s.T, s.n - j0);
   float *xs = sm, *ys = xs + s.T * s.pitch, *as = ys + s.T * s.pitch;      // [column][row], [column][row], [row][row]
@@ -472,7 +484,7 @@ __global__ void __launch_bounds__(512) ns_short_kernel(NsArgs g) {
       for (int j = wave; j < s.T; j += 8)
         for (int k = lane; k < s.mp; k += 64) xs[j * s.pitch + k] = j < nj && k < s.m ? ns_start(g, it, (long)(j0 + j) * it.cols + k, true) : 0.f;
     } else {
-      const int sh = s.T == 64 ? 6 : 5;
+      const int sh = 31 - __clz(s.T);
 #pragma unroll 8
       for (int e = threadIdx.x; e < s.mp << sh; e += 512) {
         const int k = e >> sh, j = e & (s.T - 1);
@@ -539,52 +551,56 @@ __global__ void __launch_bounds__(512) ns_short_kernel(NsArgs g) {
       for (int e = threadIdx.x; e < s.T * s.pitch; e += 512) xs[e] *= f;
       __syncthreads();
     }
-    // block e of the wave: rows 16 rb ..., columns 16 cb ...; at most two of the at most 16 blocks of a tile
-    const int tiles = s.mb * (s.T / 16);
-    int at[2];
-    nsf4 acc[2];
-    // A v: the lane's four k-values are 4 q ... 4 q + 3 of every 16, each summed on its own (a chain of m / 4 roundings, not m)
-    auto product = [&](const float* v) {
-      nsf4 sum[2][4] = {};
-      for (int k = 0; k < s.mp; k += 16)
+    // block b of the tile: rows 16 (b % mb) ..., columns 16 (b / mb) ...; NE of them a wave: wave, wave + 8, ...  (a wave without
+    // a block of its own computes the last one again and writes the same values)
+    auto step = [&](auto ne) {
+      constexpr int NE = decltype(ne)::value;
+      const int tiles = s.mb * (s.T / 16);
+      int at[NE], ar[NE], vc[NE];
+      nsf4 acc[NE];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int b = min(wave + 8 * e, tiles - 1), rb = b % s.mb, cb = b / s.mb;
-          const nsf4 av = *reinterpret_cast<const nsf4*>(as + (16 * rb + c16) * s.pitch + k + 4 * q);
-          const nsf4 bv = *reinterpret_cast<const nsf4*>(v + (16 * cb + c16) * s.pitch + k + 4 * q);
+      for (int e = 0; e < NE; ++e) {
+        const int b = min(wave + 8 * e, tiles - 1), rb = b % s.mb, cb = b / s.mb;
+        ar[e] = (16 * rb + c16) * s.pitch + 4 * q, vc[e] = (16 * cb + c16) * s.pitch + 4 * q;
+        at[e] = (16 * cb + c16) * s.pitch + 16 * rb + 4 * q;      // the lane's four rows of its column
+      }
+      // A v: the lane's four k-values are 4 q ... 4 q + 3 of every 16, each summed on its own (a chain of m / 4 roundings, not m)
+      auto product = [&](const float* v) {
+        nsf4 sum[NE][4] = {};
+        for (int k = 0; k < s.mp; k += 16)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) sum[e][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[j], bv[j], sum[e][j], 0, 0, 0);
-        }
+          for (int e = 0; e < NE; ++e) {
+            const nsf4 av = *reinterpret_cast<const nsf4*>(as + ar[e] + k), bv = *reinterpret_cast<const nsf4*>(v + vc[e] + k);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) acc[e] = (sum[e][0] + sum[e][1]) + (sum[e][2] + sum[e][3]);
+            for (int j = 0; j < 4; ++j) sum[e][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[j], bv[j], sum[e][j], 0, 0, 0);
+          }
+#pragma unroll
+        for (int e = 0; e < NE; ++e) acc[e] = (sum[e][0] + sum[e][1]) + (sum[e][2] + sum[e][3]);
+      };
+      product(xs);
+#pragma unroll
+      for (int e = 0; e < NE; ++e) *reinterpret_cast<nsf4*>(ys + at[e]) = acc[e];
+      __syncthreads();
+      product(ys);
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        const nsf4 xv = *reinterpret_cast<const nsf4*>(xs + at[e]), yv = *reinterpret_cast<const nsf4*>(ys + at[e]);
+        acc[e] = g.a * xv + (g.b * yv + g.c * acc[e]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < NE; ++e) *reinterpret_cast<nsf4*>(xs + at[e]) = acc[e];
+      __syncthreads();
     };
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int b = min(wave + 8 * e, tiles - 1);
-      at[e] = (16 * (b / s.mb) + c16) * s.pitch + 16 * (b % s.mb) + 4 * q;      // the lane's four rows of its column
-    }
-    product(xs);
-    // (a wave without a block of its own computes the last one again and writes the same values)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) *reinterpret_cast<nsf4*>(ys + at[e]) = acc[e];
-    __syncthreads();
-    product(ys);
-    nsf4 next[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const nsf4 xv = *reinterpret_cast<const nsf4*>(xs + at[e]), yv = *reinterpret_cast<const nsf4*>(ys + at[e]);
-      next[e] = g.a * xv + (g.b * yv + g.c * acc[e]);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 2; ++e) *reinterpret_cast<nsf4*>(xs + at[e]) = next[e];
-    __syncthreads();
+    const int tiles = s.mb * (s.T / 16);
+    if (tiles <= 8) step(std::integral_constant<int, 1>{});
+    else step(std::integral_constant<int, 2>{});
     if (g.last) {
       if (shape.tall) {
         for (int j = wave; j < nj; j += 8)
           for (int k = lane; k < s.m; k += 64) ns_result(g, it, (long)(j0 + j) * it.cols + k, xs[j * s.pitch + k]);
       } else {
-        const int sh = s.T == 64 ? 6 : 5;
+        const int sh = 31 - __clz(s.T);
         for (int e = threadIdx.x; e < s.m << sh; e += 512) {
           const int k = e >> sh, j = e & (s.T - 1);
           if (j < nj) ns_result(g, it, (long)k * it.cols + j0 + j, xs[j * s.pitch + k]);
@@ -644,13 +660,28 @@ static bool ns_apart(int count, const int* rows, const int* cols, int size, cons
 static int ns_chunks(int rows, int cols) { return (int)(((long)rows * cols + kNsChunk - 1) / kNsChunk); }
 
 static bool ns_is_short(int rows, int cols) {
-  return std::min(rows, cols) <= std::min(kNsShort, tuning("BMV_NS_SHORT", kNsShort)) && std::max(rows, cols) <= kNsShortLong;
+  const int m = std::min(rows, cols);
+  return m <= std::min(kNsShort, tuning("BMV_NS_SHORT", kNsShort)) && std::max(rows, cols) <= (m > 64 ? kNsShortLong / 4 : kNsShortLong);
 }
 // Workspace of a part of the list (indices): the short ones' X and shares, or the others' pieces, then the norm's partial
 // sums, then partial tiles
+// a workgroup's columns at least: the fewest with which the list runs at once (or nearly)
+static int ns_short_least(const int* rows, const int* cols, const int* idx, int n) {
+  for (int least = 16; least < 64; least *= 2) {
+    long wgs = 0;
+    int lds = 1;
+    for (int k = 0; k < n; ++k) {
+      const NsShort s(NsShape(rows[idx[k]], cols[idx[k]]), least);
+      wgs += s.parts, lds = std::max(lds, s.lds());
+    }
+    if (wgs <= kNsUnits * std::min(4, kNsLdsBytes / lds)) return least;
+  }
+  return 64;
+}
 static long ns_short_room(const int* rows, const int* cols, const int* idx, int n) {
+  const int least = ns_short_least(rows, cols, idx, n);
   long bytes = 0;
-  for (int k = 0; k < n; ++k) bytes += NsShort(NsShape(rows[idx[k]], cols[idx[k]])).bytes();
+  for (int k = 0; k < n; ++k) bytes += NsShort(NsShape(rows[idx[k]], cols[idx[k]]), least).bytes();
   return bytes;
 }
 struct NsRoom {
@@ -724,12 +755,12 @@ static void ns_fill(NsArgs& g, const NsLists& l, const int* idx, int n) {
   }
 }
 
-static void ns_run_short(NsArgs& g, int steps, char* ws, hipStream_t st) {
+static void ns_run_short(NsArgs& g, int least, int steps, char* ws, hipStream_t st) {
   long off = 0, wgs = 0;
   int lds = 0;
-  g.ws = ws;
+  g.ws = ws, g.least = least;
   for (int i = 0; i < g.count; ++i) {
-    const NsShort s(NsShape(g.it[i].rows, g.it[i].cols));
+    const NsShort s(NsShape(g.it[i].rows, g.it[i].cols), least);
     g.it[i].ws = off, g.it[i].at = (int)wgs, off += s.bytes(), wgs += s.parts, lds = std::max(lds, s.lds());
   }
   g.flip = 1;                                             // (the first shares go to where step 0 reads)
@@ -770,8 +801,9 @@ static int ns_run(NsArgs g, int count, const NsLists& l, int dtype, int steps, v
   int shorts;
   const std::vector<int> v = ns_order(count, l.rows, l.cols, shorts);
   for (int b = 0; b < shorts; b += kNsList) {
-    ns_fill(g, l, &v[b], std::min(shorts - b, kNsList));
-    ns_run_short(g, steps, ws, st);
+    const int n = std::min(shorts - b, kNsList);
+    ns_fill(g, l, &v[b], n);
+    ns_run_short(g, ns_short_least(l.rows, l.cols, &v[b], n), steps, ws, st);
   }
   for (int b = shorts; b < count; b += kNsList) {
     const int n = std::min(count - b, kNsList);
