@@ -45,7 +45,6 @@ constexpr int kNsCell = 2048;    // elements of a piece of a block: 128 rows of 
 constexpr int kNsChunk = 8192;   // elements of a workgroup of the norm
 constexpr int kNsUnits = 256, kNsLdsBytes = 160 * 1024;    // compute units, LDS of one
 constexpr int kNsSlots = 512;    // workgroups that run at once: two on each of 256 compute units
-constexpr int kNsRun = 4;        // stages of the shortest run that a workgroup is started for
 
 struct NsItem {
   const void* src;      // U, or the gradient
@@ -250,7 +249,11 @@ __device__ __forceinline__ void ns_tile(int t, const NsShape& s, bool symmetric,
   i = 8 * sr + col + t, j = 8 * sr + col;
 }
 __device__ __forceinline__ int ns_tiles(const NsShape& s, int stage) { return stage == kNsApply ? s.mt() * s.nt() : (int)s.triangle(); }
-__host__ __device__ __forceinline__ int ns_stages(const NsShape& s, int stage) { return (stage == kNsGram ? s.np : s.mp) / kNsK; }
+// blocks of 16 k-values of a stage: two where a block has only 12 matrix instructions for a barrier (two pieces)
+template <int P>
+constexpr int kNsBlocks = P == 2 ? 2 : 1;
+template <int P>
+__host__ __device__ __forceinline__ int ns_stages(const NsShape& s, int stage) { return (stage == kNsGram ? s.np : s.mp) / (kNsK * kNsBlocks<P>); }
 
 // A workgroup = 128 x 128 of L R^T, four waves of 64 x 64 (2 x 2 accumulators of v_mfma_f32_32x32x16_bf16, twice: hi hi goes to
 // accumulators of its own, because the other products are 2^-8 of it and adding them into the large sums would round those
@@ -258,9 +261,11 @@ __host__ __device__ __forceinline__ int ns_stages(const NsShape& s, int stage) {
 // in the order of the accumulators, 16 bytes a lane; the joining launch knows that order.
 template <int P, int STAGE>
 __global__ void __launch_bounds__(256, 2) ns_product_kernel(NsArgs g) {
-  constexpr int kStage = 2 * P * kNsCell;                 // elements: L's block, then R's
-  constexpr int kLoads = 2 * P * kNsCell * 2 / 1024 / 4;  // 1 KB DMAs of a wave for a stage
-  __shared__ __align__(16) __bf16 lds[3 * kStage];
+  constexpr int kB = kNsBlocks<P>, kBufs = kB == 1 ? 3 : 2;
+  constexpr int kHalf = kB * P * kNsCell;                 // elements of an operand's stage
+  constexpr int kStage = 2 * kHalf;                       // L's, then R's
+  constexpr int kLoads = kStage * 2 / 1024 / 4;           // 1 KB DMAs of a wave for a stage
+  __shared__ __align__(16) __bf16 lds[kBufs * kStage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool whole = (int)blockIdx.x < g.full;
   // the unit range of this workgroup: unit = stage of a tile behind the whole ones
@@ -270,7 +275,7 @@ __global__ void __launch_bounds__(256, 2) ns_product_kernel(NsArgs g) {
   while (left > 0) {
     const NsItem it = g.it[i];
     const NsShape s(it.rows, it.cols);
-    const int stages = ns_stages(s, STAGE), tiles = ns_tiles(s, STAGE);
+    const int stages = ns_stages<P>(s, STAGE), tiles = ns_tiles(s, STAGE);
     if (!whole) {                                         // go to the tile that holds the next unit
       const long jump = min(skip / stages, (long)(it.at + tiles - t));
       t += (int)jump, skip -= jump * stages;
@@ -286,46 +291,49 @@ __global__ void __launch_bounds__(256, 2) ns_product_kernel(NsArgs g) {
     const NsPlanes<P> p(g.ws + it.ws, s);
     const __bf16* L = STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : p.q;
     const __bf16* R = STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : (g.flip ? p.xt1 : p.xt);
-    L += ((long)ti * stages + first) * (P * kNsCell), R += ((long)tj * stages + first) * (P * kNsCell);
-    auto fill = [&](int k) {                              // stage k into buffer k % 3
-      __bf16* to = lds + k % 3 * kStage;
+    L += ((long)ti * stages + first) * kHalf, R += ((long)tj * stages + first) * kHalf;
+    auto fill = [&](int k) {                              // stage k into buffer k % kBufs
+      __bf16* to = lds + k % kBufs * kStage;
 #pragma unroll
       for (int h = 0; h < kLoads; ++h) {
         const int c = wave + 4 * h, off = c % (kLoads * 2) * 512;      // (1 KB = 512 elements; L's first, then R's)
-        const __bf16* from = (c < kLoads * 2 ? L : R) + (long)k * (P * kNsCell) + off;
+        const __bf16* from = (c < kLoads * 2 ? L : R) + (long)k * kHalf + off;
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + lane * 8),
                                          (__attribute__((address_space(3))) void*)(to + c * 512), 16, 0, 0);
       }
     };
     const int lr = (wave >> 1) * 64 + (lane & 31), rr = (wave & 1) * 64 + (lane & 31), oct = lane >> 5;
-    auto read = [&](int k, int operand, int q, int row) {
-      return *reinterpret_cast<const nsb8*>(lds + k % 3 * kStage + (operand * P + q) * kNsCell + row * kNsK + ((oct ^ row >> 3) & 1) * 8);
+    auto read = [&](int k, int b, int operand, int q, int row) {
+      return *reinterpret_cast<const nsb8*>(lds + k % kBufs * kStage + operand * kHalf + (b * P + q) * kNsCell + row * kNsK + ((oct ^ row >> 3) & 1) * 8);
     };
     nsf16 acc[2][2] = {}, low[2][2] = {};
     fill(0);
-    if (count > 1) fill(1);
+    if (kBufs == 3 && count > 1) fill(1);
     for (int k = 0; k < count; ++k) {
       // this wave's part of stage k is in LDS (of the newer loads only those of stage k + 1 may be on their way), then
       // everybody's, and nobody reads stage k - 1 any more
-      if (k + 1 < count) asm volatile("s_waitcnt vmcnt(%0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads) : "memory");
+      if (kBufs == 3 && k + 1 < count) asm volatile("s_waitcnt vmcnt(%0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (k + 2 < count) fill(k + 2);
-      nsb8 lf[2][P], rf[2][P];
+      if (k + kBufs - 1 < count) fill(k + kBufs - 1);
 #pragma unroll
-      for (int q = P - 1; q >= 0; --q)
+      for (int b = 0; b < kB; ++b) {
+        nsb8 lf[2][P], rf[2][P];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) lf[e][q] = read(k, 0, q, lr + 32 * e), rf[e][P - 1 - q] = read(k, 1, P - 1 - q, rr + 32 * e);
-      // the products of pieces whose numbers add up to at most P - 1, small ones first
+        for (int q = P - 1; q >= 0; --q)
 #pragma unroll
-      for (int sum = P - 1; sum >= 0; --sum)
+          for (int e = 0; e < 2; ++e) lf[e][q] = read(k, b, 0, q, lr + 32 * e), rf[e][P - 1 - q] = read(k, b, 1, P - 1 - q, rr + 32 * e);
+        // the products of pieces whose numbers add up to at most P - 1, small ones first
 #pragma unroll
-        for (int q = sum; q >= 0; --q)
+        for (int sum = P - 1; sum >= 0; --sum)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+          for (int q = sum; q >= 0; --q)
 #pragma unroll
-            for (int f = 0; f < 2; ++f)
-              if (sum) low[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[e][q], rf[f][sum - q], low[e][f], 0, 0, 0);
-              else acc[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[e][q], rf[f][sum - q], acc[e][f], 0, 0, 0);
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int f = 0; f < 2; ++f)
+                if (sum) low[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[e][q], rf[f][sum - q], low[e][f], 0, 0, 0);
+                else acc[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[e][q], rf[f][sum - q], acc[e][f], 0, 0, 0);
+      }
     }
     // slot: a whole tile's number; behind those, run + tile, which grows by one from each run's piece of a tile to the next
     const long slot = whole ? t : t + (long)(blockIdx.x - g.full);
@@ -369,9 +377,9 @@ __global__ void __launch_bounds__(256) ns_join_kernel(NsArgs g) {
     for (int k = 0; k < i; ++k) {
       const NsShape o(g.it[k].rows, g.it[k].cols);
       const int begin = max(g.it[k].at, g.full), end = g.it[k].at + ns_tiles(o, STAGE);
-      if (end > begin) unit += (long)(end - begin) * ns_stages(o, STAGE);
+      if (end > begin) unit += (long)(end - begin) * ns_stages<P>(o, STAGE);
     }
-    const int stages = ns_stages(s, STAGE);
+    const int stages = ns_stages<P>(s, STAGE);
     unit += (long)(t - max(it.at, g.full)) * stages;
     lo = t + unit / g.run, hi = t + (unit + stages - 1) / g.run;
   }
@@ -731,9 +739,12 @@ static void ns_product(NsArgs& g, hipStream_t st) {
   for (int i = 0; i < g.count; ++i) {
     const NsShape s(g.it[i].rows, g.it[i].cols);
     const long end = i + 1 < g.count ? g.it[i + 1].at : tiles, begin = std::max<long>(g.it[i].at, g.full);
-    if (end > begin) units += (end - begin) * ns_stages(s, STAGE);
+    if (end > begin) units += (end - begin) * ns_stages<P>(s, STAGE);
   }
-  g.run = std::max<long>((units + kNsSlots - 1) / kNsSlots, kNsRun);
+  // A run for every compute unit (two for each hide more latency, but a partial tile is 64 KB through memory: 1024 x 1024 bf16
+  // 366 -> 308 us, 1024 x 4096 492 -> 450), but not too short for the same reason: of at least 8 stages, or 4 where even those are
+  // few (256 x 256 185 us, with 8 212; 512 x 2048 fp32 with 4 365 us, with 8 300).  Panels are multiples of 8 stages long.
+  g.run = (int)std::max<long>((units + kNsUnits - 1) / kNsUnits, units <= 2 * kNsUnits ? 4 : 8);
   hipLaunchKernelGGL((ns_product_kernel<P, STAGE>), dim3((unsigned)(g.full + (units + g.run - 1) / g.run)), dim3(256), 0, st, g);
   hipLaunchKernelGGL((ns_join_kernel<P, STAGE>), dim3((unsigned)(4 * tiles)), dim3(256), 0, st, g);
 }
