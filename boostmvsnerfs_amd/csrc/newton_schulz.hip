@@ -28,6 +28,7 @@
 // Matrices with a short side of up to 128 (every layer of the networks here) go another way, one launch a step: see below.
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "bmv_common.hpp"
@@ -227,10 +228,9 @@ enum { kNsGram = 0, kNsPoly = 1, kNsApply = 2 };
 
 // Tile t of a product: super-rows of 8 tile rows, in them column by column, so that neighbouring workgroups (the 64 of an XCD
 // at a time) share 8 + 8 panels of operands in its L2.  Symmetric products: only columns up to the row.
-__device__ __forceinline__ void ns_tile(int t, const NsShape& s, bool symmetric, int& i, int& j) {
-  const int mt = s.mt();
+__device__ __forceinline__ void ns_tile(int t, int mt, int nt, bool symmetric, int& i, int& j) {
   if (!symmetric) {
-    const int per = 8 * s.nt(), sr = t / per, h = min(8, mt - 8 * sr);
+    const int per = 8 * nt, sr = t / per, h = min(8, mt - 8 * sr);
     t -= sr * per;
     i = 8 * sr + t % h, j = t / h;
     return;
@@ -254,6 +254,46 @@ template <int P>
 constexpr int kNsBlocks = P == 2 ? 2 : 1;
 template <int P>
 __host__ __device__ __forceinline__ int ns_stages(const NsShape& s, int stage) { return (stage == kNsGram ? s.np : s.mp) / (kNsK * kNsBlocks<P>); }
+
+// A finished 64 x 64 block of a product in LDS, by its workgroup: the polynomial (kNsPoly), then both orientations as pieces, or
+// the result
+template <int P, int STAGE>
+__device__ __forceinline__ void ns_finish(const NsArgs& g, const NsItem& it, const NsShape& s, const NsPlanes<P>& p, int row0, int col0,
+                                          bool diagonal, float* tile) {
+  if (STAGE == kNsPoly) {                                 // a I + b A + c A A, in place
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int k = threadIdx.x + 256 * e, r = k >> 1 & 63, c = (k >> 7) * 16 + (k & 1) * 8;
+      const __bf16* ap = p.a + ns_cell<P>(row0 + r, col0 + c, s.mp);
+      float av[8] = {};
+#pragma unroll
+      for (int q = P - 1; q >= 0; --q) {
+        const nsb8 piece = *reinterpret_cast<const nsb8*>(ap + q * kNsCell);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) av[j] += (float)piece[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float* to = tile + r * kNsPitch + c + j;
+        *to = g.b * av[j] + g.c * *to + (row0 + r == col0 + c + j && row0 + r < s.m ? g.a : 0.f);
+      }
+    }
+    __syncthreads();
+  }
+  if (STAGE == kNsApply && g.last) {
+#pragma unroll 4
+    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+      const int hi_ = e >> 6, lo_ = e & 63;               // row and column of the source inside the block
+      const int r = (s.tall ? col0 : row0) + hi_, c = (s.tall ? row0 : col0) + lo_;
+      if (r < it.rows && c < it.cols)
+        ns_result(g, it, (long)r * it.cols + c, tile[s.tall ? lo_ * kNsPitch + hi_ : hi_ * kNsPitch + lo_]);
+    }
+    return;
+  }
+  __bf16* out = STAGE == kNsGram ? p.a : STAGE == kNsPoly ? p.q : p.x;
+  if (STAGE == kNsApply) ns_store_block<P>(tile, row0, col0, out, s.np, g.flip ? p.xt : p.xt1, s.mp);
+  else ns_store_block<P>(tile, row0, col0, out, s.mp, diagonal ? nullptr : out, s.mp);
+}
 
 // A workgroup = 128 x 128 of L R^T, four waves of 64 x 64 (2 x 2 accumulators of v_mfma_f32_32x32x16_bf16, twice: hi hi goes to
 // accumulators of its own, because the other products are 2^-8 of it and adding them into the large sums would round those
@@ -287,7 +327,7 @@ __global__ void __launch_bounds__(256, 2) ns_product_kernel(NsArgs g) {
     const int first = (int)skip, count = (int)min(left, (long)stages - first);
     skip = 0, left -= whole ? left : count;
     int ti, tj;
-    ns_tile(t - it.at, s, STAGE != kNsApply, ti, tj);
+    ns_tile(t - it.at, s.mt(), s.nt(), STAGE != kNsApply, ti, tj);
     const NsPlanes<P> p(g.ws + it.ws, s);
     const __bf16* L = STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : p.q;
     const __bf16* R = STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : (g.flip ? p.xt1 : p.xt);
@@ -369,7 +409,7 @@ __global__ void __launch_bounds__(256) ns_join_kernel(NsArgs g) {
   const NsShape s(it.rows, it.cols);
   const NsPlanes<P> p(g.ws + it.ws, s);
   int ti, tj;
-  ns_tile(t - it.at, s, STAGE != kNsApply, ti, tj);
+  ns_tile(t - it.at, s.mt(), s.nt(), STAGE != kNsApply, ti, tj);
   // the slots that hold this tile: its own number, or one for each run that has stages of it
   long lo = t, hi = t;
   if (t >= g.full) {
@@ -397,40 +437,77 @@ __global__ void __launch_bounds__(256) ns_join_kernel(NsArgs g) {
     for (int j = 0; j < 4; ++j)
       tile[((wave >> 1) * 32 + 8 * r + 4 * (lane >> 5) + j) * kNsPitch + (wave & 1) * 32 + (lane & 31)] = v[r][j];
   __syncthreads();
-  const int row0 = ti * kNsTile + (quarter >> 1) * 64, col0 = tj * kNsTile + (quarter & 1) * 64;
-  if (STAGE == kNsPoly) {                                 // a I + b A + c A A, in place
+  ns_finish<P, STAGE>(g, it, s, p, ti * kNsTile + (quarter >> 1) * 64, tj * kNsTile + (quarter & 1) * 64, ti == tj, tile);
+}
+
+// The same products 64 x 64 a workgroup, whole and in one launch: a wave has 32 x 32, a stage is 32 k-values.  Twice the bytes an
+// operation, and a compute unit holds one workgroup whose stages wait for memory -- so up to kBufs - 1 of them are on their way --,
+// but no partial tiles and no joining launch.
+template <int P>
+constexpr int kNsBlockBufs = P == 3 ? 6 : 8;
+template <int P>
+constexpr int kNsBlockLds = kNsBlockBufs<P> * 2 * 2 * P * 1024 * 2;      // stages of two operands' two blocks of P pieces
+template <int P, int STAGE>
+__global__ void __launch_bounds__(256, 1) ns_block_kernel(NsArgs g) {
+  constexpr int kB = 2, kBufs = kNsBlockBufs<P>;
+  constexpr int kPart = 1024;                             // elements of a piece of a block: 64 rows of 16 k-values
+  constexpr int kHalf = kB * P * kPart, kStage = 2 * kHalf, kLoads = kStage * 2 / 1024 / 4;
+  static_assert(kBufs * kStage * 2 == kNsBlockLds<P> && 64 * kNsPitch * 4 <= kNsBlockLds<P>, "LDS");
+  extern __shared__ __align__(16) __bf16 stages_[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = xcd_contiguous(blockIdx.x, gridDim.x), i = ns_find(g, t);
+  const NsItem it = g.it[i];
+  const NsShape s(it.rows, it.cols);
+  const NsPlanes<P> p(g.ws + it.ws, s);
+  int ti, tj;
+  ns_tile(t - it.at, 2 * s.mt(), 2 * s.nt(), STAGE != kNsApply, ti, tj);
+  const int K = STAGE == kNsGram ? s.np : s.mp, count = K / (kNsK * kB);
+  // a panel's half: rows 64 (t & 1) ... of every block's pieces
+  const long panel = (long)(K / kNsK) * (P * kNsCell);
+  const __bf16* L = (STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : p.q) + (ti >> 1) * panel + (ti & 1) * kPart;
+  const __bf16* R = (STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : (g.flip ? p.xt1 : p.xt)) + (tj >> 1) * panel + (tj & 1) * kPart;
+  auto fill = [&](int k) {
+    __bf16* to = stages_ + k % kBufs * kStage;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int k = threadIdx.x + 256 * e, r = k >> 1 & 63, c = (k >> 7) * 16 + (k & 1) * 8;
-      const __bf16* ap = p.a + ns_cell<P>(row0 + r, col0 + c, s.mp);
-      float av[8] = {};
-#pragma unroll
-      for (int q = P - 1; q >= 0; --q) {
-        const nsb8 piece = *reinterpret_cast<const nsb8*>(ap + q * kNsCell);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) av[j] += (float)piece[j];
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float* to = tile + r * kNsPitch + c + j;
-        *to = g.b * av[j] + g.c * *to + (row0 + r == col0 + c + j && row0 + r < s.m ? g.a : 0.f);
-      }
+    for (int h = 0; h < kLoads; ++h) {
+      const int c = wave + 4 * h, d = c % (kLoads * 2);   // (1 KB = half a piece of a block; L's first, then R's)
+      const __bf16* from = (c < kLoads * 2 ? L : R) + (long)k * (kB * P * kNsCell) + (d >> 1) * kNsCell + (d & 1) * 512;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + lane * 8),
+                                       (__attribute__((address_space(3))) void*)(to + c * 512), 16, 0, 0);
     }
-    __syncthreads();
+  };
+  const int lr = (wave >> 1) * 32 + (lane & 31), rr = (wave & 1) * 32 + (lane & 31), oct = lane >> 5;
+  auto read = [&](int k, int b, int operand, int q, int row) {
+    return *reinterpret_cast<const nsb8*>(stages_ + k % kBufs * kStage + operand * kHalf + (b * P + q) * kPart + row * kNsK + ((oct ^ row >> 3) & 1) * 8);
+  };
+  nsf16 acc = {}, low = {};
+  for (int k = 0; k < kBufs - 1 && k < count; ++k) fill(k);
+  for (int k = 0; k < count; ++k) {
+    // (as in ns_product_kernel, with kBufs - 2 stages behind stage k on their way)
+    if (k + kBufs - 2 < count) asm volatile("s_waitcnt vmcnt(%0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::"n"((kBufs - 2) * kLoads) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (k + kBufs - 1 < count) fill(k + kBufs - 1);
+    nsb8 lf[kB][P], rf[kB][P];
+#pragma unroll
+    for (int b = 0; b < kB; ++b)
+#pragma unroll
+      for (int q = 0; q < P; ++q) lf[b][q] = read(k, b, 0, q, lr), rf[b][q] = read(k, b, 1, q, rr);
+#pragma unroll
+    for (int sum = P - 1; sum >= 0; --sum)
+#pragma unroll
+      for (int q = sum; q >= 0; --q)
+#pragma unroll
+        for (int b = 0; b < kB; ++b)
+          if (sum) low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[b][q], rf[b][sum - q], low, 0, 0, 0);
+          else acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[b][q], rf[b][sum - q], acc, 0, 0, 0);
   }
-  if (STAGE == kNsApply && g.last) {
-#pragma unroll 4
-    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-      const int hi_ = e >> 6, lo_ = e & 63;               // row and column of the source inside the block
-      const int r = (s.tall ? col0 : row0) + hi_, c = (s.tall ? row0 : col0) + lo_;
-      if (r < it.rows && c < it.cols)
-        ns_result(g, it, (long)r * it.cols + c, tile[s.tall ? lo_ * kNsPitch + hi_ : hi_ * kNsPitch + lo_]);
-    }
-    return;
-  }
-  __bf16* out = STAGE == kNsGram ? p.a : STAGE == kNsPoly ? p.q : p.x;
-  if (STAGE == kNsApply) ns_store_block<P>(tile, row0, col0, out, s.np, g.flip ? p.xt : p.xt1, s.mp);
-  else ns_store_block<P>(tile, row0, col0, out, s.mp, ti == tj ? nullptr : out, s.mp);
+  __syncthreads();
+  float* tile = reinterpret_cast<float*>(stages_);
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    tile[((wave >> 1) * 32 + 8 * (r >> 2) + 4 * oct + (r & 3)) * kNsPitch + (wave & 1) * 32 + (lane & 31)] = acc[r] + low[r];
+  __syncthreads();
+  ns_finish<P, STAGE>(g, it, s, p, ti * 64, tj * 64, ti == tj, tile);
 }
 
 // ---- short sides of up to 128 ------------------------------------------------------------------------------------------------
@@ -727,8 +804,31 @@ static long ns_workspace(int count, const int* rows, const int* cols, int dtype)
   return most;
 }
 
+// 64 x 64 blocks, where a round of them on all compute units is cheaper than tiles, a cut along k and a join: that goes by the k
+// a compute unit walks.  fp32: 6.3 us and 0.4 us for 32 k-values, against 14 ... 25 us for cut tiles and the launch that joins
+// them: 333 x 1000 (k = 1024) 18.9 us (cut 20.5), 1024 x 1024 21.5 (27), 512 x 2048 (k = 2048) 31.9 (24).  bf16: 4.5 and 0.24 us,
+// 1024 x 1024 14 us (24), k = 2048 20 (18).
+constexpr int kNsBlockK = 1024;
+template <int P, int STAGE>
+static bool ns_blocks(NsArgs& g, hipStream_t st) {
+  long blocks = 0, most = 0;
+  for (int i = 0; i < g.count; ++i) {
+    const NsShape s(g.it[i].rows, g.it[i].cols);
+    blocks += STAGE == kNsApply ? 4l * s.mt() * s.nt() : (long)s.mt() * (2 * s.mt() + 1);
+    most = std::max<long>(most, STAGE == kNsGram ? s.np : s.mp);
+  }
+  if ((blocks + kNsUnits - 1) / kNsUnits * most > tuning("BMV_NS_BLOCK_K", kNsBlockK)) return false;
+  for (int i = 0, at = 0; i < g.count; ++i) {
+    const NsShape s(g.it[i].rows, g.it[i].cols);
+    g.it[i].at = at, at += STAGE == kNsApply ? 4 * s.mt() * s.nt() : s.mt() * (2 * s.mt() + 1);
+  }
+  hipLaunchKernelGGL((ns_block_kernel<P, STAGE>), dim3((unsigned)blocks), dim3(256), kNsBlockLds<P>, st, g);
+  return true;
+}
+
 template <int P, int STAGE>
 static void ns_product(NsArgs& g, hipStream_t st) {
+  if (ns_blocks<P, STAGE>(g, st)) return;
   long tiles = 0, units = 0;
   for (int i = 0; i < g.count; ++i) {
     const NsShape s(g.it[i].rows, g.it[i].cols);
@@ -804,9 +904,21 @@ static void ns_run_long(NsArgs& g, const NsRoom& room, int steps, char* ws, hipS
 }
 
 static int ns_run(NsArgs g, int count, const NsLists& l, int dtype, int steps, void* workspace, hipStream_t st) {
-  constexpr int kLds = (2 * 32 + 128) * (128 + 4) * 4;    // the largest NsShort::lds(): above what a kernel gets without asking
-  static const bool ready = hipFuncSetAttribute((const void*)ns_short_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess &&
-                            hipFuncSetAttribute((const void*)ns_short_kernel<false>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess;
+  static constexpr int kLds = (2 * 32 + 128) * (128 + 4) * 4;    // the largest NsShort::lds()
+  // (above 64 KB of LDS, which a kernel gets only where it was asked for)
+  static const bool ready = [] {
+    const std::pair<const void*, int> f[] = {{(const void*)ns_short_kernel<true>, kLds},
+                                             {(const void*)ns_short_kernel<false>, kLds},
+                                             {(const void*)ns_block_kernel<3, kNsGram>, kNsBlockLds<3>},
+                                             {(const void*)ns_block_kernel<3, kNsPoly>, kNsBlockLds<3>},
+                                             {(const void*)ns_block_kernel<3, kNsApply>, kNsBlockLds<3>},
+                                             {(const void*)ns_block_kernel<2, kNsGram>, kNsBlockLds<2>},
+                                             {(const void*)ns_block_kernel<2, kNsPoly>, kNsBlockLds<2>},
+                                             {(const void*)ns_block_kernel<2, kNsApply>, kNsBlockLds<2>}};
+    for (const auto& k : f)
+      if (hipFuncSetAttribute(k.first, hipFuncAttributeMaxDynamicSharedMemorySize, k.second) != hipSuccess) return false;
+    return true;
+  }();
   if (!ready) return -1;
   char* ws = static_cast<char*>(workspace);
   int shorts;

@@ -67,13 +67,16 @@ SHAPES = [(1, 1), (1, 7), (9, 1), (2, 2), (3, 64), (8, 27), (16, 200), (35, 4), 
           (65, 40), (80, 100), (127, 129), (128, 63), (8, 4000), (128, 4096), (128, 4097), (33, 1000), (5, 16384), (17, 16385), (60, 1153), (112, 288), (112, 289), (96, 1200), (128, 128), (128, 515), (129, 129), (130, 1000), (333, 257), (256, 384), (700, 90)]
 
 
-@pytest.fixture(params=["short", "long"])
+@pytest.fixture(params=["short", "blocks", "tiles"])
 def way(request):
-    """Short sides of up to 128 one launch a step (default), and through the tiles of the large ones."""
+    """Short sides of up to 128 one launch a step (default), all through 64 x 64 blocks where those are taken (default above 128),
+    all through the tiles of the large ones."""
     from boostmvsnerfs_amd import _lib
     _lib.set_tuning("BMV_NS_SHORT", None if request.param == "short" else 0)
+    _lib.set_tuning("BMV_NS_BLOCK_K", {"short": None, "blocks": 1 << 20, "tiles": 0}[request.param])
     yield request.param
     _lib.set_tuning("BMV_NS_SHORT", None)
+    _lib.set_tuning("BMV_NS_BLOCK_K", None)
 
 
 @gpu
