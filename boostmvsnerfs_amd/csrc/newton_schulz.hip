@@ -481,26 +481,39 @@ __global__ void __launch_bounds__(256, 1) ns_block_kernel(NsArgs g) {
     return *reinterpret_cast<const nsb8*>(stages_ + k % kBufs * kStage + operand * kHalf + (b * P + q) * kPart + row * kNsK + ((oct ^ row >> 3) & 1) * 8);
   };
   nsf16 acc = {}, low = {};
-  for (int k = 0; k < kBufs - 1 && k < count; ++k) fill(k);
-  for (int k = 0; k < count; ++k) {
-    // (as in ns_product_kernel, with kBufs - 2 stages behind stage k on their way)
-    if (k + kBufs - 2 < count) asm volatile("s_waitcnt vmcnt(%0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::"n"((kBufs - 2) * kLoads) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (k + kBufs - 1 < count) fill(k + kBufs - 1);
-    nsb8 lf[kB][P], rf[kB][P];
+  nsb8 lf[2][kB][P], rf[2][kB][P];                        // operands of the stage that is multiplied, and of the next
+  auto fetch = [&](int k, int into) {
 #pragma unroll
     for (int b = 0; b < kB; ++b)
 #pragma unroll
-      for (int q = 0; q < P; ++q) lf[b][q] = read(k, b, 0, q, lr), rf[b][q] = read(k, b, 1, q, rr);
+      for (int q = 0; q < P; ++q) lf[into][b][q] = read(k, b, 0, q, lr), rf[into][b][q] = read(k, b, 1, q, rr);
+  };
+  // stage k is in LDS for everybody (behind it up to kBufs - 2 may be on their way), and nobody reads stage k - 1 any more
+  auto arrive = [&](int k) {
+    if (k + kBufs - 2 < count) asm volatile("s_waitcnt vmcnt(%0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::"n"((kBufs - 2) * kLoads) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  for (int k = 0; k < kBufs - 1 && k < count; ++k) fill(k);
+  arrive(0);
+  if (kBufs - 1 < count) fill(kBufs - 1);
+  fetch(0, 0);
+  for (int k = 0; k < count; k += 2)                      // (an even number of stages: k is a multiple of 128)
 #pragma unroll
-    for (int sum = P - 1; sum >= 0; --sum)
+    for (int u = 0; u < 2; ++u) {
+      // the next stage's operands are read under this one's products: all four waves would otherwise first read, then multiply
+      // (behind the last stage: that one again, unused)
+      arrive(k + u + 1);
+      if (k + u + kBufs < count) fill(k + u + kBufs);
+      fetch(min(k + u + 1, count - 1), u ^ 1);
 #pragma unroll
-      for (int q = sum; q >= 0; --q)
+      for (int sum = P - 1; sum >= 0; --sum)
 #pragma unroll
-        for (int b = 0; b < kB; ++b)
-          if (sum) low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[b][q], rf[b][sum - q], low, 0, 0, 0);
-          else acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[b][q], rf[b][sum - q], acc, 0, 0, 0);
-  }
+        for (int q = sum; q >= 0; --q)
+#pragma unroll
+          for (int b = 0; b < kB; ++b)
+            if (sum) low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[u][b][q], rf[u][b][sum - q], low, 0, 0, 0);
+            else acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[u][b][q], rf[u][b][sum - q], acc, 0, 0, 0);
+    }
   __syncthreads();
   float* tile = reinterpret_cast<float*>(stages_);
 #pragma unroll
