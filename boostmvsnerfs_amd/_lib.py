@@ -50,6 +50,11 @@ class MvsRenderArgs(C.Structure):
                 + [(n, C.c_void_p) for n in ("raw", "z_vals", "mask", "inputs86")])
 
 
+class GroupNormSpec(C.Structure):
+    _fields_ = ([(n, C.c_int) for n in ("N", "C", "G", "dtype", "param_dtype", "channels_last", "act")]
+                + [("slope", C.c_float), ("S", C.c_long), ("eps", C.c_double)])
+
+
 # name -> argtypes (all return int unless noted); mirrors include/bmv.h one to one
 SIGNATURES = {
     "bmv_proj_mats": [c_f, c_f, c_f, c_f, c_fl, c_fl, c_i, c_i, c_f, c_f],
@@ -141,9 +146,9 @@ SIGNATURES = {
     "bmv_bn_chunks": [c_i, c_l],
     "bmv_bn_train_fwd": [c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_l, c_fl, c_fl, c_fl, c_f, c_f, c_f, c_f, c_f],
     "bmv_bn_train_bwd": [c_f, c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_l, c_fl, c_f, c_f, c_f, c_f, c_f],
-    "bmv_group_norm_workspace": [c_i, c_i, c_l, c_i, c_i, c_i, c_i],
-    "bmv_group_norm_fwd": [c_f, c_f, c_f, c_i, c_i, c_l, c_i, c_i, c_i, c_i, C.c_double, c_i, c_fl, c_f, c_f, c_f, c_f, c_f],
-    "bmv_group_norm_bwd": [c_f, c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_l, c_i, c_i, c_i, c_i, c_i, c_fl, c_f, c_f, c_f, c_f, c_f],
+    "bmv_group_norm_workspace": [C.POINTER(GroupNormSpec), c_i],
+    "bmv_group_norm_fwd": [C.POINTER(GroupNormSpec), c_f, c_f, c_f, c_f, c_f, c_f, c_f],
+    "bmv_group_norm_bwd": [C.POINTER(GroupNormSpec), c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f],
     "bmv_newton_schulz_workspace": [c_i, C.POINTER(C.c_int), C.POINTER(C.c_int), c_i],
     "bmv_newton_schulz": [c_i, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_int), C.POINTER(C.c_int), c_i, c_i, c_fl, c_fl,
                           c_fl, c_fl, c_f, c_f],

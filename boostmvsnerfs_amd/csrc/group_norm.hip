@@ -928,13 +928,18 @@ static void gn_dispatch(const GnPlan& p, const GnArgs& a, int dtype, bool bwd, b
 
 static bool gn_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-static const char* gn_bad_shape(int N, int C, long S, int G, int dtype) {
-  if (N <= 0 || C <= 0 || S <= 0) return "bad shape";
-  if (G <= 0 || C % G) return "the channels are no multiple of the groups";
-  if (dtype < 0 || dtype > 2) return "unknown type";
-  if ((long)N * C > (1l << 24) || S > (1l << 40) / ((long)N * C)) return "the map is too large";
+static const char* gn_bad(const bmv_group_norm_spec* s) {
+  if (!s) return "no spec";
+  if (s->N <= 0 || s->C <= 0 || s->S <= 0) return "bad shape";
+  if (s->G <= 0 || s->C % s->G) return "the channels are no multiple of the groups";
+  if (s->dtype < 0 || s->dtype > 2) return "unknown type";
+  if (s->param_dtype != 0 && s->param_dtype != s->dtype) return "weight and bias are 32-bit or of the map's type";
+  if (s->act != 0 && s->act != 1) return "unknown activation";
+  if (!(s->eps >= 0.)) return "eps must not be negative";
+  if ((long)s->N * s->C > (1l << 24) || s->S > (1l << 40) / ((long)s->N * s->C)) return "the map is too large";
   return nullptr;
 }
+static GnPlan gn_plan_of(const bmv_group_norm_spec* s) { return gn_plan(s->N, s->C, s->S, s->G, s->dtype, s->channels_last); }
 
 }  // namespace bmv
 
@@ -942,48 +947,42 @@ using namespace bmv;
 
 extern "C" {
 
-long bmv_group_norm_workspace(int N, int C, long S, int G, int dtype, int channels_last, int backward) {
-  const char* bad = gn_bad_shape(N, C, S, G, dtype);
-  BMV_REQUIRE(!bad, "bmv_group_norm_workspace: %s (N %d, C %d, S %ld, groups %d)", bad, N, C, S, G);
-  const GnPlan p = gn_plan(N, C, S, G, dtype, channels_last);
+long bmv_group_norm_workspace(const bmv_group_norm_spec* spec, int backward) {
+  const char* bad = gn_bad(spec);
+  BMV_REQUIRE(!bad, "bmv_group_norm_workspace: %s", bad);
+  const GnPlan p = gn_plan_of(spec);
   return 2 * (p.part + p.fin + (backward ? p.partc : 0));
 }
 
-int bmv_group_norm_fwd(const void* x, const void* weight, const void* bias, int N, int C, long S, int G, int dtype,
-                       int param_dtype, int channels_last, double eps, int act, float slope, double* workspace, double* mean,
-                       double* rstd, void* y, bmv_stream_t stream) {
-  BMV_REQUIRE(x && workspace && mean && rstd && y, "bmv_group_norm_fwd: null pointer");
-  const char* bad = gn_bad_shape(N, C, S, G, dtype);
-  BMV_REQUIRE(!bad, "bmv_group_norm_fwd: %s (N %d, C %d, S %ld, groups %d)", bad, N, C, S, G);
-  BMV_REQUIRE(param_dtype == 0 || param_dtype == dtype, "bmv_group_norm_fwd: weight and bias are 32-bit or of the map's type");
-  BMV_REQUIRE(eps >= 0., "bmv_group_norm_fwd: eps must not be negative");
-  BMV_REQUIRE(act == 0 || act == 1, "bmv_group_norm_fwd: unknown activation %d", act);
+int bmv_group_norm_fwd(const bmv_group_norm_spec* spec, const void* x, const void* weight, const void* bias, double* stats,
+                       double* workspace, void* y, bmv_stream_t stream) {
+  const char* bad = gn_bad(spec);
+  BMV_REQUIRE(!bad, "bmv_group_norm_fwd: %s", bad);
+  BMV_REQUIRE(x && stats && workspace && y, "bmv_group_norm_fwd: null pointer");
   BMV_REQUIRE(gn_aligned(x) && gn_aligned(y) && gn_aligned(workspace), "bmv_group_norm_fwd: x, y and workspace begin at 16-byte addresses");
-  const GnPlan p = gn_plan(N, C, S, G, dtype, channels_last);
+  const GnPlan p = gn_plan_of(spec);
   GnArgs a = p.a;
-  a.x = x, a.w = weight, a.b = bias, a.out = y, a.mean = mean, a.rstd = rstd, a.wdt = param_dtype, a.eps = eps, a.slope = slope;
+  a.x = x, a.w = weight, a.b = bias, a.out = y, a.wdt = spec->param_dtype, a.eps = spec->eps, a.slope = spec->slope;
+  a.mean = stats, a.rstd = stats + (long)a.N * a.G;
   a.part = reinterpret_cast<double2*>(workspace);
-  gn_dispatch(p, a, dtype, false, act == 1, as_stream(stream));
+  gn_dispatch(p, a, spec->dtype, false, spec->act == 1, as_stream(stream));
   BMV_LAUNCH_END("bmv_group_norm_fwd");
 }
 
-int bmv_group_norm_bwd(const void* x, const void* dy, const void* weight, const void* bias, const double* mean,
-                       const double* rstd, int N, int C, long S, int G, int dtype, int param_dtype, int channels_last, int act,
-                       float slope, double* workspace, void* dx, void* dweight, void* dbias, bmv_stream_t stream) {
-  BMV_REQUIRE(x && dy && mean && rstd && workspace && dx, "bmv_group_norm_bwd: null pointer");
-  const char* bad = gn_bad_shape(N, C, S, G, dtype);
-  BMV_REQUIRE(!bad, "bmv_group_norm_bwd: %s (N %d, C %d, S %ld, groups %d)", bad, N, C, S, G);
-  BMV_REQUIRE(param_dtype == 0 || param_dtype == dtype, "bmv_group_norm_bwd: weight and bias are 32-bit or of the map's type");
-  BMV_REQUIRE(act == 0 || act == 1, "bmv_group_norm_bwd: unknown activation %d", act);
+int bmv_group_norm_bwd(const bmv_group_norm_spec* spec, const void* x, const void* dy, const void* weight, const void* bias,
+                       const double* stats, double* workspace, void* dx, void* dweight, void* dbias, bmv_stream_t stream) {
+  const char* bad = gn_bad(spec);
+  BMV_REQUIRE(!bad, "bmv_group_norm_bwd: %s", bad);
+  BMV_REQUIRE(x && dy && stats && workspace && dx, "bmv_group_norm_bwd: null pointer");
   BMV_REQUIRE(gn_aligned(x) && gn_aligned(dy) && gn_aligned(dx) && gn_aligned(workspace),
               "bmv_group_norm_bwd: x, dy, dx and workspace begin at 16-byte addresses");
-  const GnPlan p = gn_plan(N, C, S, G, dtype, channels_last);
+  const GnPlan p = gn_plan_of(spec);
   GnArgs a = p.a;
-  a.x = x, a.dy = dy, a.w = weight, a.b = bias, a.out = dx, a.dw = dweight, a.db = dbias, a.wdt = param_dtype, a.slope = slope;
-  a.mean = const_cast<double*>(mean), a.rstd = const_cast<double*>(rstd);
+  a.x = x, a.dy = dy, a.w = weight, a.b = bias, a.out = dx, a.dw = dweight, a.db = dbias, a.wdt = spec->param_dtype, a.slope = spec->slope;
+  a.mean = const_cast<double*>(stats), a.rstd = a.mean + (long)a.N * a.G;
   a.part = reinterpret_cast<double2*>(workspace);
   a.partc = dweight || dbias ? a.part + p.part + p.fin : nullptr;
-  gn_dispatch(p, a, dtype, true, act == 1, as_stream(stream));
+  gn_dispatch(p, a, spec->dtype, true, spec->act == 1, as_stream(stream));
   BMV_LAUNCH_END("bmv_group_norm_bwd");
 }
 

@@ -1370,66 +1370,80 @@ def _gpu_float(t, name, like=None):
     return t
 
 
-def _gn_dense(x):
-    """(x dense in one of the two layouts, 1 for channel-last / 0 for planar)."""
-    last = 0
-    if not x.is_contiguous():
-        d = x.dim()
-        last = int((d == 4 and x.is_contiguous(memory_format=torch.channels_last))
-                   or (d == 5 and x.is_contiguous(memory_format=torch.channels_last_3d))
-                   or (d == 3 and x.transpose(1, 2).is_contiguous()))
-        if not last:
-            x = x.contiguous()
-    if x.data_ptr() & 15:           # (a view that begins inside a 16-byte piece)
-        x = x.clone(memory_format=torch.preserve_format)
-    return x, last
+def _gn_layout(x):
+    """1: dense channel-last, 0: dense planar, None: neither."""
+    if x.is_contiguous():
+        return 0
+    d = x.dim()
+    last = ((d == 4 and x.is_contiguous(memory_format=torch.channels_last))
+            or (d == 5 and x.is_contiguous(memory_format=torch.channels_last_3d)) or (d == 3 and x.transpose(1, 2).is_contiguous()))
+    return 1 if last else None
 
 
-def _gn_check(x, groups, weight, bias, relu):
-    """-> groups, activation code, slope, the parameters' type code."""
-    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in _FLOAT_CODES):
-        _gpu_float(x, "x")           # raises
-    shape = x.shape
-    if len(shape) < 2:
-        raise ValueError(f"x: expected (N, C, *spatial), got {tuple(shape)}")
-    C_ = shape[1]
-    groups = int(groups)
-    if groups <= 0 or C_ == 0 or C_ % groups:
+class _GnPlan:
+    """What calls of one kind (shapes, strides, types, activation) share: checked arguments, the library's spec, sizes."""
+    __slots__ = ("device", "dense", "empty", "spec", "ref", "stats", "fwd", "bwd")
+
+
+_GN_PLANS = {}
+
+
+def _gn_plan(x, groups, weight, bias, eps, relu):
+    try:
+        # (a Python-bound path: the key is all that is asked of the arguments from the second call of a kind on; True == 1.0)
+        key = (x.shape, x.stride(), x.dtype, x.get_device(), groups, eps, relu, type(relu),
+               weight if weight is None else (weight.shape, weight.dtype, weight.get_device()),
+               bias if bias is None else (bias.shape, bias.dtype, bias.get_device()))
+        plan = _GN_PLANS.get(key)
+        if plan is not None:
+            return plan
+    except (AttributeError, TypeError, RuntimeError):
+        key = None
+    _gpu_float(x, "x")
+    if x.dim() < 2:
+        raise ValueError(f"x: expected (N, C, *spatial), got {tuple(x.shape)}")
+    N, C_ = x.shape[:2]
+    G = int(groups)
+    if G <= 0 or C_ == 0 or C_ % G:
         raise ValueError(f"groups: {groups} do not divide {C_} channels")
-    code = None
+    if not eps >= 0:
+        raise ValueError(f"eps: {eps} is negative")
     for t, name in ((weight, "weight"), (bias, "bias")):
         if t is None:
             continue
-        if not (isinstance(t, torch.Tensor) and t.device == x.device and t.dtype in _FLOAT_CODES):
-            _gpu_float(t, name, x)
-        if t.shape != (C_,):
+        _gpu_float(t, name, x)
+        if tuple(t.shape) != (C_,):
             raise ValueError(f"{name}: expected ({C_},), got {tuple(t.shape)}")
-        if t.dtype is not torch.float32 and t.dtype is not x.dtype:
+        if t.dtype not in (torch.float32, x.dtype):
             raise TypeError(f"{name}: expected float32 or {x.dtype}, got {t.dtype}")
-        mine = _FLOAT_CODES[t.dtype]
-        if code is not None and code != mine:
-            raise TypeError(f"weight and bias: {weight.dtype} and {bias.dtype}, expected one type")
-        code = mine
-    if isinstance(relu, str):
-        if relu != "silu":
-            raise ValueError(f"relu: expected False, True, a slope or 'silu', got {relu!r}")
-        return groups, 1, 0.0, code or 0
-    return groups, 0, _act_slope(relu), code or 0
-
-
-_GN_WORKSPACE = {}      # bmv_group_norm_workspace by its arguments (a few shapes a network; asked once each)
-
-
-def _gn_workspace(lib, key, device):
-    n = _GN_WORKSPACE.get(key)
-    if n is None:
-        n = lib.bmv_group_norm_workspace(*key)
-        if n < 0:
-            _lib.check(int(n), "group_norm_workspace")
-        if len(_GN_WORKSPACE) >= 4096:
-            _GN_WORKSPACE.clear()
-        _GN_WORKSPACE[key] = n
-    return torch.empty(n, device=device, dtype=torch.float64)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"weight and bias: {weight.dtype} and {bias.dtype}, expected one type")
+    if isinstance(relu, str) and relu != "silu":
+        raise ValueError(f"relu: expected False, True, a slope or 'silu', got {relu!r}")
+    plan = _GnPlan()
+    plan.device, plan.empty, plan.stats = x.device, x.numel() == 0, 2 * N * G
+    last = _gn_layout(x)
+    plan.dense = last is not None
+    plan.spec = plan.ref = None
+    plan.fwd = plan.bwd = 0
+    if plan.dense and not plan.empty:
+        S = x.numel() // (N * C_)
+        first = weight if weight is not None else bias
+        plan.spec = _lib.GroupNormSpec(N=N, C=C_, G=G, dtype=_FLOAT_CODES[x.dtype], param_dtype=0 if first is None else _FLOAT_CODES[first.dtype],
+                                       # (a single position: both layouts are one, the channel axis the contiguous one)
+                                       channels_last=1 if S == 1 else last, act=int(relu == "silu"),
+                                       slope=0.0 if relu == "silu" else _act_slope(relu), S=S, eps=float(eps))
+        plan.ref = C.byref(plan.spec)
+        lib = _lib.load()
+        plan.fwd, plan.bwd = (lib.bmv_group_norm_workspace(plan.ref, k) for k in (0, 1))
+        for n in (plan.fwd, plan.bwd):
+            if n < 0:
+                _lib.check(int(n), "group_norm_workspace")
+    if key is not None:
+        if len(_GN_PLANS) >= 4096:
+            _GN_PLANS.clear()
+        _GN_PLANS[key] = plan
+    return plan
 
 
 def _region(name):
@@ -1440,35 +1454,33 @@ _NO_REGION = contextlib.nullcontext()
 
 
 def group_norm_stats_fwd(x, groups, weight=None, bias=None, eps=1e-5, relu=False):
-    """`group_norm_fwd` with its statistics as one tensor: -> y, (2, N, groups) float64 (mean, rstd)."""
-    groups, act, slope, pcode = _gn_check(x, groups, weight, bias, relu)
-    if not eps >= 0:
-        raise ValueError(f"eps: {eps} is negative")
-    device = x.device
+    """`group_norm_fwd` for autograd: -> y, and what `group_norm_stats_bwd` wants to have (float64, the statistics in front)."""
+    plan = _gn_plan(x, groups, weight, bias, eps, relu)
+    device = plan.device
     if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return group_norm_stats_fwd(x, groups, weight, bias, eps, relu)
-    x, last = _gn_dense(x)
-    shape = x.shape
-    N, C_ = shape[0], shape[1]
+    if not plan.dense:
+        return group_norm_stats_fwd(x.contiguous(), groups, weight, bias, eps, relu)
+    px = x.data_ptr()
+    if px & 15:                      # (a view that begins inside a 16-byte piece)
+        x = x.clone(memory_format=torch.preserve_format)
+        px = x.data_ptr()
     y = torch.empty_like(x)
-    stats = torch.empty((2, N, groups), device=device, dtype=torch.float64)
-    numel = x.numel()
-    if numel == 0:
-        return y, stats.zero_()
-    S = numel // (N * C_)
-    last = 1 if S == 1 else last        # (a single position: both layouts are one, the channel axis the contiguous one)
-    weight, bias = weight if weight is None else _c(weight), bias if bias is None else _c(bias)
-    lib = _lib.load()
-    code = _FLOAT_CODES[x.dtype]
-    ws = _gn_workspace(lib, (N, C_, S, groups, code, last, 0), device)
-    mean = stats.data_ptr()
+    buf = torch.empty(plan.stats + plan.fwd, device=device, dtype=torch.float64)
+    if plan.empty:
+        return y, buf.zero_()
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    stats = buf.data_ptr()
     with _region("group_norm_fwd"):
-        rc = lib.bmv_group_norm_fwd(x.data_ptr(), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
-                                    N, C_, S, groups, code, pcode, last, float(eps), act, slope, ws.data_ptr(), mean,
-                                    mean + 8 * N * groups, y.data_ptr(), stream())
-    _lib.check(rc, "group_norm_fwd")
-    return y, stats
+        rc = _lib.load().bmv_group_norm_fwd(plan.ref, px, None if weight is None else weight.data_ptr(),
+                                            None if bias is None else bias.data_ptr(), stats, stats + 8 * plan.stats, y.data_ptr(), stream())
+    if rc:
+        _lib.check(rc, "group_norm_fwd")
+    return y, buf
 
 
 def group_norm_fwd(x, groups, weight=None, bias=None, eps=1e-5, relu=False):
@@ -1476,44 +1488,46 @@ def group_norm_fwd(x, groups, weight=None, bias=None, eps=1e-5, relu=False):
     copied to planar): y = act((x - mean) / sqrt(var + eps) * weight + bias), statistics over a sample's C / groups channels.
     `relu`: False, True, a leaky slope, or "silu".  weight / bias (C): fp32 or x's type, or None.
     -> y (x's layout and type), mean, rstd (N, groups; float64, what `group_norm_bwd` reads)."""
-    y, stats = group_norm_stats_fwd(x, groups, weight, bias, eps, relu)
-    return (y, *stats.unbind())
+    y, buf = group_norm_stats_fwd(x, groups, weight, bias, eps, relu)
+    N = x.shape[0]
+    return (y, *buf[:2 * N * int(groups)].view(2, N, int(groups)).unbind())
 
 
-def group_norm_stats_bwd(x, dy, groups, weight, bias, stats, relu=False, want_params=True):
-    """`group_norm_bwd` with the statistics as `group_norm_stats_fwd` returns them."""
-    groups, act, slope, pcode = _gn_check(x, groups, weight, bias, relu)
-    if not (isinstance(dy, torch.Tensor) and dy.shape == x.shape and dy.dtype == x.dtype and dy.device == x.device):
+def group_norm_stats_bwd(x, dy, groups, weight, bias, buf, relu=False, want_params=True):
+    """`group_norm_bwd` with what `group_norm_stats_fwd` returned."""
+    plan = _gn_plan(x, groups, weight, bias, 1e-5, relu)
+    if not (isinstance(dy, torch.Tensor) and dy.shape == x.shape and dy.dtype == x.dtype and dy.device == plan.device):
         _gpu_float(dy, "dy", x)
         raise ValueError(f"dy: expected {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
-    device = x.device
+    device = plan.device
     if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
-            return group_norm_stats_bwd(x, dy, groups, weight, bias, stats, relu, want_params)
-    x, last = _gn_dense(x)
-    if dy.stride() != x.stride() or dy.data_ptr() & 15:
+            return group_norm_stats_bwd(x, dy, groups, weight, bias, buf, relu, want_params)
+    if not plan.dense:
+        return group_norm_stats_bwd(x.contiguous(), dy, groups, weight, bias, buf, relu, want_params)
+    px, pdy = x.data_ptr(), dy.data_ptr()
+    if px & 15:
+        x = x.clone(memory_format=torch.preserve_format)
+        px = x.data_ptr()
+    if pdy & 15 or dy.stride() != x.stride():
         dy = torch.empty_like(x).copy_(dy)
-    shape = x.shape
-    N, C_ = shape[0], shape[1]
+        pdy = dy.data_ptr()
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     dx = torch.empty_like(x)
-    weight, bias = weight if weight is None else _c(weight), bias if bias is None else _c(bias)
-    dw = torch.empty_like(weight) if weight is not None and want_params else None
-    db = torch.empty_like(bias) if bias is not None and want_params else None
-    numel = x.numel()
-    if numel == 0:
+    dw = torch.empty_like(weight) if want_params and weight is not None else None
+    db = torch.empty_like(bias) if want_params and bias is not None else None
+    if plan.empty:
         return dx, dw if dw is None else dw.zero_(), db if db is None else db.zero_()
-    S = numel // (N * C_)
-    last = 1 if S == 1 else last
-    lib = _lib.load()
-    code = _FLOAT_CODES[x.dtype]
-    ws = _gn_workspace(lib, (N, C_, S, groups, code, last, 1), device)
-    mean = stats.data_ptr()
+    ws = torch.empty(plan.bwd, device=device, dtype=torch.float64)
     with _region("group_norm_bwd"):
-        rc = lib.bmv_group_norm_bwd(x.data_ptr(), dy.data_ptr(), None if weight is None else weight.data_ptr(),
-                                    None if bias is None else bias.data_ptr(), mean, mean + 8 * N * groups, N, C_, S, groups, code, pcode,
-                                    last, act, slope, ws.data_ptr(), dx.data_ptr(), None if dw is None else dw.data_ptr(),
-                                    None if db is None else db.data_ptr(), stream())
-    _lib.check(rc, "group_norm_bwd")
+        rc = _lib.load().bmv_group_norm_bwd(plan.ref, px, pdy, None if weight is None else weight.data_ptr(),
+                                            None if bias is None else bias.data_ptr(), buf.data_ptr(), ws.data_ptr(), dx.data_ptr(),
+                                            None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), stream())
+    if rc:
+        _lib.check(rc, "group_norm_bwd")
     return dx, dw, db
 
 

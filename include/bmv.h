@@ -351,15 +351,19 @@ int bmv_bn_train_bwd(const float* x, const float* y, const float* dy, const floa
  * at 16-byte addresses.  weight, bias, dweight, dbias (C): `param_dtype` = 0 (fp32) or dtype; each may be NULL.
  * y = act((x - mean) rstd w + b) with the mean and (biased) variance of a sample's group of C / G channels, rstd =
  * 1 / sqrt(var + eps); act 0: v > 0 ? v : slope * v (1 none, 0 ReLU), act 1: v / (1 + exp(-v)) (slope ignored).
- * mean, rstd (N, G) are 64-bit: the backward recomputes z and decides its sign with them.
- * workspace: bmv_group_norm_workspace(...) doubles (backward = 1 for the gradients' call). */
-long bmv_group_norm_workspace(int N, int C, long S, int G, int dtype, int channels_last, int backward);
-int bmv_group_norm_fwd(const void* x, const void* weight, const void* bias, int N, int C, long S, int G, int dtype,
-                       int param_dtype, int channels_last, double eps, int act, float slope, double* workspace, double* mean,
-                       double* rstd, void* y, bmv_stream_t stream);
-int bmv_group_norm_bwd(const void* x, const void* dy, const void* weight, const void* bias, const double* mean,
-                       const double* rstd, int N, int C, long S, int G, int dtype, int param_dtype, int channels_last, int act,
-                       float slope, double* workspace, void* dx, void* dweight, void* dbias, bmv_stream_t stream);
+ * stats: mean (N, G), then rstd (N, G), 64-bit: the backward recomputes z and decides its sign with them.
+ * workspace: bmv_group_norm_workspace(...) doubles (backward = 1 for the gradients' call), at a 16-byte address. */
+typedef struct {
+  int N, C, G, dtype, param_dtype, channels_last, act;
+  float slope;
+  long S;
+  double eps;
+} bmv_group_norm_spec;
+long bmv_group_norm_workspace(const bmv_group_norm_spec* spec, int backward);
+int bmv_group_norm_fwd(const bmv_group_norm_spec* spec, const void* x, const void* weight, const void* bias, double* stats,
+                       double* workspace, void* y, bmv_stream_t stream);
+int bmv_group_norm_bwd(const bmv_group_norm_spec* spec, const void* x, const void* dy, const void* weight, const void* bias,
+                       const double* stats, double* workspace, void* dx, void* dweight, void* dbias, bmv_stream_t stream);
 
 /* ---- orthogonalised updates of weight matrices (training; beside the reference's Adam, lib/train/optimizer.py:12-28)
  * Newton-Schulz iteration of `count` matrices src[i] (rows[i], cols[i]), row-major, contiguous, all of `dtype` (0 fp32, 1 bf16,

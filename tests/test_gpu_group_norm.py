@@ -322,11 +322,16 @@ def test_group_norm_refusals_on_the_gpu():
         ops.group_norm_fwd(x, 2, w, w, eps=-1.0)
     with pytest.raises(ValueError, match="N, C"):
         ops.group_norm_fwd(w, 2)
+    # what is remembered of a kind of call tells a slope of 1 from a ReLU and of 0 from none
+    v = torch.randn(1, 4, 3, 3, device="cuda")
+    assert (ops.group_norm_fwd(v, 2, w, w * 0, relu=True)[0] >= 0).all() and (ops.group_norm_fwd(v, 2, w, w * 0, relu=1.0)[0] < 0).any()
+    assert (ops.group_norm_fwd(v, 2, w, w * 0, relu=0.0)[0] >= 0).all() and (ops.group_norm_fwd(v, 2, w, w * 0, relu=False)[0] < 0).any()
     y, mean, rstd = ops.group_norm_fwd(x, 2, w, w)
     with pytest.raises(ValueError, match="dy"):
         ops.group_norm_bwd(x, y.half(), 2, w, w, mean, rstd)
     with pytest.raises(ValueError, match="mean"):
         ops.group_norm_bwd(x, y, 2, w, w, mean.float(), rstd)
     lib = _lib.load()
-    assert lib.bmv_group_norm_workspace(1, 4, 4, 3, 0, 1, 0) == -1
+    import ctypes as C
+    assert lib.bmv_group_norm_workspace(C.byref(_lib.GroupNormSpec(N=1, C=4, G=3, S=4, channels_last=1)), 0) == -1
     assert b"multiple" in lib.bmv_last_error()
