@@ -230,17 +230,15 @@ class GroupNormAct(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, groups, weight, bias, eps=1e-5, relu=False):
-        y, stats = ops.group_norm_stats_fwd(x, groups, weight, bias, eps, relu)
+        y, ctx.plan, stats = ops.group_norm_begin(x, groups, weight, bias, eps, relu)
         ctx.save_for_backward(x, weight, bias, stats)
-        ctx.cfg = (groups, relu)
         return y
 
     @staticmethod
     def backward(ctx, dy):
         x, weight, bias, stats = ctx.saved_tensors
-        groups, relu = ctx.cfg
         _, _, want_w, want_b, _, _ = ctx.needs_input_grad
-        dx, dw, db = ops.group_norm_stats_bwd(x, dy, groups, weight, bias, stats, relu, want_w or want_b)
+        dx, dw, db = ops.group_norm_end(ctx.plan, x, dy, weight, bias, stats, want_w or want_b)
         if torch.is_grad_enabled():          # create_graph: the gradients depend on all of these
             dx, dw, db = _NotAgain.apply(dx, dw, db, x, weight, bias, dy)
         return dx, None, dw if want_w else None, db if want_b else None, None, None

@@ -1382,7 +1382,7 @@ def _gn_layout(x):
 
 class _GnPlan:
     """What calls of one kind (shapes, strides, types, activation) share: checked arguments, the library's spec, sizes."""
-    __slots__ = ("device", "dense", "empty", "spec", "ref", "stats", "fwd", "bwd")
+    __slots__ = ("device", "dense", "empty", "spec", "ref", "stats", "fwd", "bwd", "stride")
 
 
 _GN_PLANS = {}
@@ -1422,6 +1422,7 @@ def _gn_plan(x, groups, weight, bias, eps, relu):
         raise ValueError(f"relu: expected False, True, a slope or 'silu', got {relu!r}")
     plan = _GnPlan()
     plan.device, plan.empty, plan.stats = x.device, x.numel() == 0, 2 * N * G
+    plan.stride = x.stride()
     last = _gn_layout(x)
     plan.dense = last is not None
     plan.spec = plan.ref = None
@@ -1453,34 +1454,73 @@ def _region(name):
 _NO_REGION = contextlib.nullcontext()
 
 
-def group_norm_stats_fwd(x, groups, weight=None, bias=None, eps=1e-5, relu=False):
-    """`group_norm_fwd` for autograd: -> y, and what `group_norm_stats_bwd` wants to have (float64, the statistics in front)."""
+def _gn_dense(x):
+    """x planar if it is dense in neither layout, and beginning at a 16-byte address."""
+    if _gn_layout(x) is None:
+        return x.contiguous()
+    return x.clone(memory_format=torch.preserve_format) if x.data_ptr() & 15 else x
+
+
+def group_norm_begin(x, groups, weight=None, bias=None, eps=1e-5, relu=False):
+    """`group_norm_fwd` for autograd: -> y, and what `group_norm_end` wants: the plan, a float64 tensor (the statistics in front)."""
     plan = _gn_plan(x, groups, weight, bias, eps, relu)
     device = plan.device
     if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
-            return group_norm_stats_fwd(x, groups, weight, bias, eps, relu)
-    if not plan.dense:
-        return group_norm_stats_fwd(x.contiguous(), groups, weight, bias, eps, relu)
+            return group_norm_begin(x, groups, weight, bias, eps, relu)
     px = x.data_ptr()
-    if px & 15:                      # (a view that begins inside a 16-byte piece)
-        x = x.clone(memory_format=torch.preserve_format)
-        px = x.data_ptr()
+    if not plan.dense or px & 15:
+        return group_norm_begin(_gn_dense(x), groups, weight, bias, eps, relu)
     y = torch.empty_like(x)
     buf = torch.empty(plan.stats + plan.fwd, device=device, dtype=torch.float64)
     if plan.empty:
-        return y, buf.zero_()
-    if weight is not None and not weight.is_contiguous():
-        weight = weight.contiguous()
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
+        return y, plan, buf.zero_()
+    pw = pb = None
+    if weight is not None:
+        weight = _c(weight)
+        pw = weight.data_ptr()
+    if bias is not None:
+        bias = _c(bias)
+        pb = bias.data_ptr()
     stats = buf.data_ptr()
     with _region("group_norm_fwd"):
-        rc = _lib.load().bmv_group_norm_fwd(plan.ref, px, None if weight is None else weight.data_ptr(),
-                                            None if bias is None else bias.data_ptr(), stats, stats + 8 * plan.stats, y.data_ptr(), stream())
+        rc = _lib.load().bmv_group_norm_fwd(plan.ref, px, pw, pb, stats, stats + 8 * plan.stats, y.data_ptr(),
+                                            torch._C._cuda_getCurrentRawStream(device.index))
     if rc:
         _lib.check(rc, "group_norm_fwd")
-    return y, buf
+    return y, plan, buf
+
+
+def group_norm_end(plan, x, dy, weight, bias, buf, want_params=True):
+    """`group_norm_bwd` of a `group_norm_begin` with this x: dy has x's shape, type and device."""
+    device = plan.device
+    if device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return group_norm_end(plan, x, dy, weight, bias, buf, want_params)
+    if x.stride() != plan.stride or x.data_ptr() & 15:      # (as in group_norm_begin, whose plan is that of the copy)
+        x = _gn_dense(x)
+    px, pdy = x.data_ptr(), dy.data_ptr()
+    if pdy & 15 or dy.stride() != plan.stride:
+        dy = torch.empty_like(x).copy_(dy)
+        pdy = dy.data_ptr()
+    dx = torch.empty_like(x)
+    pw = pb = dw = db = None
+    if weight is not None:
+        weight = _c(weight)
+        pw, dw = weight.data_ptr(), torch.empty_like(weight) if want_params else None
+    if bias is not None:
+        bias = _c(bias)
+        pb, db = bias.data_ptr(), torch.empty_like(bias) if want_params else None
+    if plan.empty:
+        return dx, dw if dw is None else dw.zero_(), db if db is None else db.zero_()
+    ws = torch.empty(plan.bwd, device=device, dtype=torch.float64)
+    with _region("group_norm_bwd"):
+        rc = _lib.load().bmv_group_norm_bwd(plan.ref, px, pdy, pw, pb, buf.data_ptr(), ws.data_ptr(), dx.data_ptr(),
+                                            None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
+                                            torch._C._cuda_getCurrentRawStream(device.index))
+    if rc:
+        _lib.check(rc, "group_norm_bwd")
+    return dx, dw, db
 
 
 def group_norm_fwd(x, groups, weight=None, bias=None, eps=1e-5, relu=False):
@@ -1488,55 +1528,23 @@ def group_norm_fwd(x, groups, weight=None, bias=None, eps=1e-5, relu=False):
     copied to planar): y = act((x - mean) / sqrt(var + eps) * weight + bias), statistics over a sample's C / groups channels.
     `relu`: False, True, a leaky slope, or "silu".  weight / bias (C): fp32 or x's type, or None.
     -> y (x's layout and type), mean, rstd (N, groups; float64, what `group_norm_bwd` reads)."""
-    y, buf = group_norm_stats_fwd(x, groups, weight, bias, eps, relu)
-    N = x.shape[0]
-    return (y, *buf[:2 * N * int(groups)].view(2, N, int(groups)).unbind())
-
-
-def group_norm_stats_bwd(x, dy, groups, weight, bias, buf, relu=False, want_params=True):
-    """`group_norm_bwd` with what `group_norm_stats_fwd` returned."""
-    plan = _gn_plan(x, groups, weight, bias, 1e-5, relu)
-    if not (isinstance(dy, torch.Tensor) and dy.shape == x.shape and dy.dtype == x.dtype and dy.device == plan.device):
-        _gpu_float(dy, "dy", x)
-        raise ValueError(f"dy: expected {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
-    device = plan.device
-    if device.index != torch._C._cuda_getDevice():
-        with torch.cuda.device(device):
-            return group_norm_stats_bwd(x, dy, groups, weight, bias, buf, relu, want_params)
-    if not plan.dense:
-        return group_norm_stats_bwd(x.contiguous(), dy, groups, weight, bias, buf, relu, want_params)
-    px, pdy = x.data_ptr(), dy.data_ptr()
-    if px & 15:
-        x = x.clone(memory_format=torch.preserve_format)
-        px = x.data_ptr()
-    if pdy & 15 or dy.stride() != x.stride():
-        dy = torch.empty_like(x).copy_(dy)
-        pdy = dy.data_ptr()
-    if weight is not None and not weight.is_contiguous():
-        weight = weight.contiguous()
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
-    dx = torch.empty_like(x)
-    dw = torch.empty_like(weight) if want_params and weight is not None else None
-    db = torch.empty_like(bias) if want_params and bias is not None else None
-    if plan.empty:
-        return dx, dw if dw is None else dw.zero_(), db if db is None else db.zero_()
-    ws = torch.empty(plan.bwd, device=device, dtype=torch.float64)
-    with _region("group_norm_bwd"):
-        rc = _lib.load().bmv_group_norm_bwd(plan.ref, px, pdy, None if weight is None else weight.data_ptr(),
-                                            None if bias is None else bias.data_ptr(), buf.data_ptr(), ws.data_ptr(), dx.data_ptr(),
-                                            None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), stream())
-    if rc:
-        _lib.check(rc, "group_norm_bwd")
-    return dx, dw, db
+    y, plan, buf = group_norm_begin(x, groups, weight, bias, eps, relu)
+    return (y, *buf[:plan.stats].view(2, x.shape[0], int(groups)).unbind())
 
 
 def group_norm_bwd(x, dy, groups, weight, bias, mean, rstd, relu=False, want_params=True):
     """-> dx (x's layout and type), dweight, dbias (C; None where weight / bias is None or not `want_params`)."""
+    plan = _gn_plan(x, groups, weight, bias, 1e-5, relu)
+    if not (isinstance(dy, torch.Tensor) and dy.shape == x.shape and dy.dtype == x.dtype and dy.device == x.device):
+        _gpu_float(dy, "dy", x)
+        raise ValueError(f"dy: expected {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
     for t, name in ((mean, "mean"), (rstd, "rstd")):
         if not torch.is_tensor(t) or tuple(t.shape) != (x.shape[0], int(groups)) or t.dtype != torch.float64 or t.device != x.device:
             raise ValueError(f"{name}: expected ({x.shape[0]}, {groups}) float64 on {x.device}")
-    return group_norm_stats_bwd(x, dy, groups, weight, bias, torch.stack((mean, rstd)), relu, want_params)
+    if not plan.dense:
+        x = _gn_dense(x)
+        plan = _gn_plan(x, groups, weight, bias, 1e-5, relu)
+    return group_norm_end(plan, x, dy, weight, bias, torch.stack((mean, rstd)), want_params)
 
 
 NS_COEFFS = (3.4445, -4.7750, 2.0315)      # the quintic a s + b s^3 + c s^5 of a Newton-Schulz step
