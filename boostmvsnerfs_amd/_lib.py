@@ -151,9 +151,9 @@ SIGNATURES = {
     "bmv_group_norm_bwd": [C.POINTER(GroupNormSpec), c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f, c_f],
     "bmv_newton_schulz_workspace": [c_i, C.POINTER(C.c_int), C.POINTER(C.c_int), c_i],
     "bmv_newton_schulz": [c_i, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_int), C.POINTER(C.c_int), c_i, c_i, c_fl, c_fl,
-                          c_fl, c_fl, c_f, c_f],
+                          c_fl, c_fl, c_f, C.c_long, c_f],
     "bmv_muon_step": [c_i, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_int), C.POINTER(C.c_int),
-                      C.POINTER(C.c_float), c_i, C.c_double, c_i, C.c_double, c_i, c_fl, c_fl, c_fl, c_fl, c_f, c_f],
+                      C.POINTER(C.c_float), c_i, C.c_double, c_i, C.c_double, c_i, c_fl, c_fl, c_fl, c_fl, c_f, C.c_long, c_f],
     "bmv_conv_top_fwd": [c_f, c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_i, c_fl, c_i, c_f],
     "bmv_conv0_fused_fwd": [c_f, c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_i, c_i, c_fl, c_fl, c_f],
     "bmv_conv_heads_fwd": [c_f, c_f, c_f, c_f, c_f, c_i, c_i, c_i, c_i, c_i, c_f],

@@ -27,6 +27,8 @@
 //
 // Matrices with a short side of up to 128 (every layer of the networks here) go another way, one launch a step: see below.
 #include <algorithm>
+#include <atomic>
+#include <exception>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -732,6 +734,16 @@ static const char* ns_bad(int count, const int* rows, const int* cols) {
     if (rows[i] <= 0 || cols[i] <= 0 || rows[i] > (1 << 16) || cols[i] > (1 << 16)) return "a side is not in 1 ... 65536";
   return nullptr;
 }
+// the host's lists are the only thing of a call that can throw
+template <typename F>
+static auto ns_no_throw(F f) -> decltype(f()) {
+  try {
+    return f();
+  } catch (const std::exception&) {
+    set_error("Newton-Schulz: out of host memory");
+    return BMV_ERR_INVALID;
+  }
+}
 // what a call writes overlaps nothing else that it reads or writes
 static bool ns_apart(int count, const int* rows, const int* cols, int size, const void* const* in, const void* const* out,
                      const void* const* out32) {
@@ -757,9 +769,11 @@ static bool ns_apart(int count, const int* rows, const int* cols, int size, cons
 }
 static int ns_chunks(int rows, int cols) { return (int)(((long)rows * cols + kNsChunk - 1) / kNsChunk); }
 
-static bool ns_is_short(int rows, int cols) {
+// limit: of the short side, what BMV_NS_SHORT is at the call (read once: the workspace's layout goes by it)
+static int ns_limit() { return std::min(kNsShort, tuning("BMV_NS_SHORT", kNsShort)); }
+static bool ns_is_short(int rows, int cols, int limit) {
   const int m = std::min(rows, cols);
-  return m <= std::min(kNsShort, tuning("BMV_NS_SHORT", kNsShort)) && std::max(rows, cols) <= (m > 64 ? kNsShortLong / 4 : kNsShortLong);
+  return m <= limit && std::max(rows, cols) <= (m > 64 ? kNsShortLong / 4 : kNsShortLong);
 }
 // Workspace of a part of the list (indices): the short ones' X and shares, or the others' pieces, then the norm's partial
 // sums, then partial tiles
@@ -796,21 +810,19 @@ struct NsRoom {
   long bytes() const { return pieces + (long)kNsList * sqn * sizeof(double) + (tiles + kNsSlots) * (kNsTile * kNsTile * 4l); }
 };
 // the list's indices: the short ones, then the others
-static std::vector<int> ns_order(int count, const int* rows, const int* cols, int& shorts) {
+static std::vector<int> ns_order(int count, const int* rows, const int* cols, int limit, int& shorts) {
   std::vector<int> v;
   v.reserve(count);
   for (int i = 0; i < count; ++i)
-    if (ns_is_short(rows[i], cols[i])) v.push_back(i);
+    if (ns_is_short(rows[i], cols[i], limit)) v.push_back(i);
   shorts = (int)v.size();
   for (int i = 0; i < count; ++i)
-    if (!ns_is_short(rows[i], cols[i])) v.push_back(i);
+    if (!ns_is_short(rows[i], cols[i], limit)) v.push_back(i);
   return v;
 }
 // a list is done in parts of kNsList, which share the workspace
-static long ns_workspace(int count, const int* rows, const int* cols, int dtype) {
+static long ns_workspace(int count, const int* rows, const int* cols, int dtype, const std::vector<int>& v, int shorts) {
   long most = 0;
-  int shorts;
-  const std::vector<int> v = ns_order(count, rows, cols, shorts);
   for (int b = 0; b < shorts; b += kNsList) most = std::max(most, ns_short_room(rows, cols, &v[b], std::min(shorts - b, kNsList)));
   for (int b = shorts; b < count; b += kNsList)
     most = std::max(most, NsRoom(rows, cols, &v[b], std::min(count - b, kNsList), dtype == 1 ? 2 : 3).bytes());
@@ -916,26 +928,34 @@ static void ns_run_long(NsArgs& g, const NsRoom& room, int steps, char* ws, hipS
   }
 }
 
-static int ns_run(NsArgs g, int count, const NsLists& l, int dtype, int steps, void* workspace, hipStream_t st) {
+// More than 64 KB of LDS, which a kernel gets only where it was asked for, on each device
+static bool ns_lds() {
   static constexpr int kLds = (2 * 32 + 128) * (128 + 4) * 4;    // the largest NsShort::lds()
-  // (above 64 KB of LDS, which a kernel gets only where it was asked for)
-  static const bool ready = [] {
-    const std::pair<const void*, int> f[] = {{(const void*)ns_short_kernel<true>, kLds},
-                                             {(const void*)ns_short_kernel<false>, kLds},
-                                             {(const void*)ns_block_kernel<3, kNsGram>, kNsBlockLds<3>},
-                                             {(const void*)ns_block_kernel<3, kNsPoly>, kNsBlockLds<3>},
-                                             {(const void*)ns_block_kernel<3, kNsApply>, kNsBlockLds<3>},
-                                             {(const void*)ns_block_kernel<2, kNsGram>, kNsBlockLds<2>},
-                                             {(const void*)ns_block_kernel<2, kNsPoly>, kNsBlockLds<2>},
-                                             {(const void*)ns_block_kernel<2, kNsApply>, kNsBlockLds<2>}};
-    for (const auto& k : f)
-      if (hipFuncSetAttribute(k.first, hipFuncAttributeMaxDynamicSharedMemorySize, k.second) != hipSuccess) return false;
-    return true;
-  }();
-  if (!ready) return -1;
-  char* ws = static_cast<char*>(workspace);
+  static std::atomic<unsigned long> ready{0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return false;
+  const unsigned long bit = dev < 64 ? 1ul << dev : 0;
+  if (ready.load(std::memory_order_acquire) & bit) return true;
+  const std::pair<const void*, int> f[] = {{(const void*)ns_short_kernel<true>, kLds},
+                                           {(const void*)ns_short_kernel<false>, kLds},
+                                           {(const void*)ns_block_kernel<3, kNsGram>, kNsBlockLds<3>},
+                                           {(const void*)ns_block_kernel<3, kNsPoly>, kNsBlockLds<3>},
+                                           {(const void*)ns_block_kernel<3, kNsApply>, kNsBlockLds<3>},
+                                           {(const void*)ns_block_kernel<2, kNsGram>, kNsBlockLds<2>},
+                                           {(const void*)ns_block_kernel<2, kNsPoly>, kNsBlockLds<2>},
+                                           {(const void*)ns_block_kernel<2, kNsApply>, kNsBlockLds<2>}};
+  for (const auto& k : f)
+    if (hipFuncSetAttribute(k.first, hipFuncAttributeMaxDynamicSharedMemorySize, k.second) != hipSuccess) return false;
+  ready.fetch_or(bit, std::memory_order_release);
+  return true;
+}
+
+static const char* ns_run(NsArgs g, int count, const NsLists& l, int dtype, int steps, void* workspace, long bytes, hipStream_t st) {
   int shorts;
-  const std::vector<int> v = ns_order(count, l.rows, l.cols, shorts);
+  const std::vector<int> v = ns_order(count, l.rows, l.cols, ns_limit(), shorts);
+  if (ns_workspace(count, l.rows, l.cols, dtype, v, shorts) > bytes) return "the workspace is too small";
+  if (!ns_lds()) return "LDS refused";
+  char* ws = static_cast<char*>(workspace);
   for (int b = 0; b < shorts; b += kNsList) {
     const int n = std::min(shorts - b, kNsList);
     ns_fill(g, l, &v[b], n);
@@ -947,7 +967,7 @@ static int ns_run(NsArgs g, int count, const NsLists& l, int dtype, int steps, v
     if (dtype == 1) ns_run_long<2>(g, NsRoom(l.rows, l.cols, &v[b], n, 2), steps, ws, st);
     else ns_run_long<3>(g, NsRoom(l.rows, l.cols, &v[b], n, 3), steps, ws, st);
   }
-  return 0;
+  return nullptr;
 }
 
 }  // namespace bmv
@@ -960,11 +980,15 @@ long bmv_newton_schulz_workspace(int count, const int* rows, const int* cols, in
   const char* bad = ns_bad(count, rows, cols);
   BMV_REQUIRE(!bad, "bmv_newton_schulz_workspace: %s", bad);
   BMV_REQUIRE(dtype >= 0 && dtype <= 2, "bmv_newton_schulz_workspace: unknown type %d", dtype);
-  return ns_workspace(count, rows, cols, dtype);
+  return ns_no_throw([&]() -> long {
+    int shorts;
+    const std::vector<int> v = ns_order(count, rows, cols, ns_limit(), shorts);
+    return ns_workspace(count, rows, cols, dtype, v, shorts);
+  });
 }
 
 int bmv_newton_schulz(int count, const void* const* src, void* const* dst, const int* rows, const int* cols, int dtype, int steps,
-                      float a, float b, float c, float eps, void* workspace, bmv_stream_t stream) {
+                      float a, float b, float c, float eps, void* workspace, long workspace_bytes, bmv_stream_t stream) {
   const char* bad = ns_bad(count, rows, cols);
   BMV_REQUIRE(!bad, "bmv_newton_schulz: %s", bad);
   BMV_REQUIRE(dtype >= 0 && dtype <= 2, "bmv_newton_schulz: unknown type %d", dtype);
@@ -972,17 +996,20 @@ int bmv_newton_schulz(int count, const void* const* src, void* const* dst, const
   if (count == 0) return BMV_OK;
   BMV_REQUIRE(src && dst && workspace && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "bmv_newton_schulz: null pointer, or a workspace off its 256-byte border");
   for (int i = 0; i < count; ++i) BMV_REQUIRE(src[i] && dst[i], "bmv_newton_schulz: null pointer (matrix %d)", i);
-  BMV_REQUIRE(ns_apart(count, rows, cols, dtype == 0 ? 4 : 2, src, dst, nullptr), "bmv_newton_schulz: a result overlaps another matrix");
-  NsArgs g{};
-  g.dtype = dtype, g.a = a, g.b = b, g.c = c, g.eps = eps;
-  const NsLists l{src, dst, nullptr, rows, cols, nullptr};
-  BMV_REQUIRE(ns_run(g, count, l, dtype, steps, workspace, as_stream(stream)) == 0, "bmv_newton_schulz: LDS refused");
-  BMV_LAUNCH_END("bmv_newton_schulz");
+  return ns_no_throw([&]() -> int {
+    BMV_REQUIRE(ns_apart(count, rows, cols, dtype == 0 ? 4 : 2, src, dst, nullptr), "bmv_newton_schulz: a result overlaps another matrix");
+    NsArgs g{};
+    g.dtype = dtype, g.a = a, g.b = b, g.c = c, g.eps = eps;
+    const NsLists l{src, dst, nullptr, rows, cols, nullptr};
+    bad = ns_run(g, count, l, dtype, steps, workspace, workspace_bytes, as_stream(stream));
+    BMV_REQUIRE(!bad, "bmv_newton_schulz: %s", bad);
+    BMV_LAUNCH_END("bmv_newton_schulz");
+  });
 }
 
 int bmv_muon_step(int count, void* const* params, const void* const* grads, float* const* momenta, const int* rows, const int* cols,
                   const float* scales, int dtype, double momentum, int nesterov, double keep, int steps, float a, float b, float c,
-                  float eps, void* workspace, bmv_stream_t stream) {
+                  float eps, void* workspace, long workspace_bytes, bmv_stream_t stream) {
   const char* bad = ns_bad(count, rows, cols);
   BMV_REQUIRE(!bad, "bmv_muon_step: %s", bad);
   BMV_REQUIRE(dtype >= 0 && dtype <= 2, "bmv_muon_step: unknown type %d", dtype);
@@ -991,13 +1018,16 @@ int bmv_muon_step(int count, void* const* params, const void* const* grads, floa
   BMV_REQUIRE(params && grads && momenta && scales && workspace && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
               "bmv_muon_step: null pointer, or a workspace off its 256-byte border");
   for (int i = 0; i < count; ++i) BMV_REQUIRE(params[i] && grads[i] && momenta[i], "bmv_muon_step: null pointer (matrix %d)", i);
-  BMV_REQUIRE(ns_apart(count, rows, cols, dtype == 0 ? 4 : 2, grads, params, reinterpret_cast<const void* const*>(momenta)),
-              "bmv_muon_step: a weight or a momentum overlaps another tensor (is one listed twice?)");
-  NsArgs g{};
-  g.dtype = dtype, g.a = a, g.b = b, g.c = c, g.eps = eps, g.muon = 1, g.nesterov = nesterov, g.mu = (float)momentum, g.nu = (float)(1. - momentum), g.keep = (float)keep;
-  const NsLists l{grads, params, momenta, rows, cols, scales};
-  BMV_REQUIRE(ns_run(g, count, l, dtype, steps, workspace, as_stream(stream)) == 0, "bmv_muon_step: LDS refused");
-  BMV_LAUNCH_END("bmv_muon_step");
+  return ns_no_throw([&]() -> int {
+    BMV_REQUIRE(ns_apart(count, rows, cols, dtype == 0 ? 4 : 2, grads, params, reinterpret_cast<const void* const*>(momenta)),
+                "bmv_muon_step: a weight or a momentum overlaps another tensor (is one listed twice?)");
+    NsArgs g{};
+    g.dtype = dtype, g.a = a, g.b = b, g.c = c, g.eps = eps, g.muon = 1, g.nesterov = nesterov, g.mu = (float)momentum, g.nu = (float)(1. - momentum), g.keep = (float)keep;
+    const NsLists l{grads, params, momenta, rows, cols, scales};
+    bad = ns_run(g, count, l, dtype, steps, workspace, workspace_bytes, as_stream(stream));
+    BMV_REQUIRE(!bad, "bmv_muon_step: %s", bad);
+    BMV_LAUNCH_END("bmv_muon_step");
+  });
 }
 
 }  // extern "C"

@@ -1625,7 +1625,7 @@ def newton_schulz(mats, steps=5, coeffs=NS_COEFFS, eps=NS_EPS):
             ws = _ns_workspace(lib, n, rows, cols, dtype, device)
             with _region("newton_schulz"):
                 rc = lib.bmv_newton_schulz(n, _pointers([mats[i] for i in idx]), _pointers([out[i] for i in idx]), rows, cols,
-                                           _FLOAT_CODES[dtype], steps, a, b, c, eps, ws.data_ptr(), stream())
+                                           _FLOAT_CODES[dtype], steps, a, b, c, eps, ws.data_ptr(), ws.numel(), stream())
             _lib.check(rc, "newton_schulz")
     return out
 
@@ -1672,7 +1672,7 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
             with _region("muon_step"):
                 rc = lib.bmv_muon_step(n, _pointers(p), _pointers([_c(grads[i]) for i in idx]), _pointers(m), rows, cols, scales,
                                        _FLOAT_CODES[dtype], float(momentum), int(bool(nesterov)), keep, steps, a, b, c, eps,
-                                       ws.data_ptr(), stream())
+                                       ws.data_ptr(), ws.numel(), stream())
             _lib.check(rc, "muon_step")
             for i, new in zip(idx, p):             # (weights of other strides went through a copy)
                 if new is not params[i]:

@@ -368,19 +368,20 @@ int bmv_group_norm_bwd(const bmv_group_norm_spec* spec, const void* x, const voi
 /* ---- orthogonalised updates of weight matrices (training; beside the reference's Adam, lib/train/optimizer.py:12-28)
  * Newton-Schulz iteration of `count` matrices src[i] (rows[i], cols[i]), row-major, contiguous, all of `dtype` (0 fp32, 1 bf16,
  * 2 fp16) -> dst[i]: X = src / max(|src|_F, eps), then `steps` times A = X X^T, X = a X + (b A + c A A) X (on the transpose
- * where rows > cols).  operands of 24 bits (bf16: 17), one rounding at the end; a non-finite value makes its matrix NaN and
- * leaves the others alone.  Reproducible; a matrix' last bits depend on what else is in the list (where sums are cut).  The arrays are
+ * where rows > cols).  operands of 24 bits (bf16: 17), one rounding at the end; a non-finite value (up to 128 rows: also a
+ * norm whose square leaves fp32) makes its matrix NaN and leaves the others alone.  Reproducible; a matrix' last bits depend on what else is in the list (where sums are cut).  The arrays are
  * HOST arrays, read before the call returns; eps >= 1e-12, sides up to 65536.
- * workspace: bmv_newton_schulz_workspace(...) bytes, beginning at a 256-byte border. */
+ * workspace: bmv_newton_schulz_workspace(...) bytes or more, beginning at a 256-byte border; the call refuses one that is too
+ * small (the size goes by the switch BMV_NS_SHORT). */
 long bmv_newton_schulz_workspace(int count, const int* rows, const int* cols, int dtype);
 int bmv_newton_schulz(int count, const void* const* src, void* const* dst, const int* rows, const int* cols, int dtype, int steps,
-                      float a, float b, float c, float eps, void* workspace, bmv_stream_t stream);
+                      float a, float b, float c, float eps, void* workspace, long workspace_bytes, bmv_stream_t stream);
 /* The optimiser's whole step around it, in place: momenta[i] (fp32) = momentum * itself + (1 - momentum) grad; U = (nesterov ?
  * (1 - momentum) grad + momentum * momenta[i] : momenta[i]); params[i] = keep * params[i] - scales[i] * iterate(U), rounded
  * once.  params and grads are of `dtype`.  Nothing that is written may overlap anything else of the call. */
 int bmv_muon_step(int count, void* const* params, const void* const* grads, float* const* momenta, const int* rows, const int* cols,
                   const float* scales, int dtype, double momentum, int nesterov, double keep, int steps, float a, float b, float c,
-                  float eps, void* workspace, bmv_stream_t stream);
+                  float eps, void* workspace, long workspace_bytes, bmv_stream_t stream);
 
 /* ======================= MVSNeRF backbone (lib/networks/mvsnerf) ======================= */
 

@@ -303,14 +303,17 @@ def test_overlaps_are_refused_by_the_entry_points():
     A, B, G, M, N, W = 0x1000000, 0x2000000, 0x3000000, 0x4000000, 0x5000000, 0x6000000
 
     def step(p, g, m):
-        return lib.bmv_muon_step(2, ptrs(*p), ptrs(*g), ptrs(*m), rows, cols, one, 0, 0.9, 1, 1.0, 5, *COEFFS, 1e-7, C.c_void_p(W), None)
+        return lib.bmv_muon_step(2, ptrs(*p), ptrs(*g), ptrs(*m), rows, cols, one, 0, 0.9, 1, 1.0, 5, *COEFFS, 1e-7, C.c_void_p(W), 1 << 40, None)
     for p, g, m in (((A, A), (G, G), (M, N)), ((A, A + 64), (G, G), (M, N)), ((A, B), (A, G), (M, N)), ((A, B), (G, G), (M, M)),
                     ((A, B), (G, G), (M, B)), ((A, B), (G, M + 4), (M, N))):
         assert step(p, g, m) == -1 and b"overlaps" in lib.bmv_last_error()
-    assert lib.bmv_newton_schulz(2, ptrs(A, B), ptrs(G, A), rows, cols, 0, 5, *COEFFS, 1e-7, C.c_void_p(W), None) == -1
+    assert lib.bmv_newton_schulz(2, ptrs(A, B), ptrs(G, A), rows, cols, 0, 5, *COEFFS, 1e-7, C.c_void_p(W), 1 << 40, None) == -1
     assert b"overlaps" in lib.bmv_last_error()
     assert lib.bmv_newton_schulz_workspace(1, (C.c_int * 1)(0), (C.c_int * 1)(4), 0) == -1
-    assert lib.bmv_newton_schulz(1, ptrs(A), ptrs(G), rows, cols, 7, 5, *COEFFS, 1e-7, C.c_void_p(W), None) == -1
+    need = lib.bmv_newton_schulz_workspace(2, rows, cols, 0)
+    assert lib.bmv_newton_schulz(2, ptrs(A, B), ptrs(G, M), rows, cols, 0, 5, *COEFFS, 1e-7, C.c_void_p(W), need - 1, None) == -1
+    assert b"too small" in lib.bmv_last_error()
+    assert lib.bmv_newton_schulz(1, ptrs(A), ptrs(G), rows, cols, 7, 5, *COEFFS, 1e-7, C.c_void_p(W), 1 << 40, None) == -1
 
 
 @gpu
