@@ -1440,7 +1440,7 @@ def _gn_plan(x, groups, weight, bias, eps, relu):
         for n in (plan.fwd, plan.bwd):
             if n < 0:
                 _lib.check(int(n), "group_norm_workspace")
-    if key is not None:
+    if key is not None and all(isinstance(v, (bool, int, float, str)) for v in (groups, eps, relu)):      # (values, not objects)
         if len(_GN_PLANS) >= 4096:
             _GN_PLANS.clear()
         _GN_PLANS[key] = plan
@@ -1497,8 +1497,9 @@ def group_norm_end(plan, x, dy, weight, bias, buf, want_params=True):
     if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return group_norm_end(plan, x, dy, weight, bias, buf, want_params)
-    if x.stride() != plan.stride or x.data_ptr() & 15:      # (as in group_norm_begin, whose plan is that of the copy)
-        x = _gn_dense(x)
+    if x.stride() != plan.stride or x.data_ptr() & 15:
+        # (in group_norm_begin too, whose plan is that of the copy; or a hook on saved tensors returned another layout)
+        x = torch.empty_strided(x.shape, plan.stride, dtype=x.dtype, device=x.device).copy_(x)
     px, pdy = x.data_ptr(), dy.data_ptr()
     if pdy & 15 or dy.stride() != plan.stride:
         dy = torch.empty_like(x).copy_(dy)
@@ -1668,6 +1669,9 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
             rows, cols = _sides(sizes, idx)
             scales = (C.c_float * n)(*[lr * MUON_SCALES[scale](*sizes[i]) for i in idx])
             p, m = [_c(params[i]) for i in idx], [_c(momenta[i]) for i in idx]
+            if any(a is not params[i] or b is not momenta[i] for a, b, i in zip(p, m, idx)):      # (copies do not overlap)
+                if len({t.data_ptr() for i in idx for t in (params[i], momenta[i])}) < 2 * n:
+                    raise RuntimeError("muon_step: a weight or a momentum overlaps another tensor (is one listed twice?)")
             ws = _ns_workspace(lib, n, rows, cols, dtype, device)
             with _region("muon_step"):
                 rc = lib.bmv_muon_step(n, _pointers(p), _pointers([_c(grads[i]) for i in idx]), _pointers(m), rows, cols, scales,

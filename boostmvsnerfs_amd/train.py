@@ -147,6 +147,8 @@ class MuonAdam(torch.optim.Optimizer):
             self._adam.param_groups = [g for g in self.param_groups if not g["muon"]]
 
     def load_state_dict(self, state_dict):
+        if [g.get("muon") for g in state_dict["param_groups"]] != [g["muon"] for g in self.param_groups]:
+            raise ValueError("MuonAdam: the state's groups are not this optimiser's (matrices, then the others)")
         super().load_state_dict(state_dict)
         # (torch casts a state to its parameter's type: a 16-bit weight's momentum is fp32)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]

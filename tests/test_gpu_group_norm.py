@@ -3,6 +3,8 @@
 Tolerances.  u = eps / 2 of the map's type is the rounding of a result; 32-bit arithmetic in between adds a few 2^-24 of the
 terms (x - mean) rstd w and b of z, and of the three terms of dx.  SiLU adds the 32-bit exponential's error (2 ulp + |z| 2^-23).
 dw and db are 64-bit sums of products with up to 4 roundings each of 2^-24."""
+import contextlib
+
 import pytest
 import torch
 
@@ -279,6 +281,35 @@ def test_group_norm_gradients_against_differences():
         scale = float((grad.double().cpu() * v).abs().sum())
         # 64-bit differences: h^2 f''' / 6 (h = 1e-5, a smooth function of unit scale) and rounding 1e-16 / h; fp32 gradients 2^-21
         assert abs(got - want) <= scale * (2 ** -20 + 1e-8), (k, got, want)
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["last", "planar"])
+def test_group_norm_with_saved_tensors_in_another_layout(layout):
+    """Hooks on saved tensors may hand the backward x in other strides (a copy to the host and back does)."""
+    from boostmvsnerfs_amd import autograd as A
+    x, r, w, b = _make(2, 8, (5, 7), torch.float32, layout)
+
+    def grads(hooks):
+        xg, wg, bg = _place(x, layout).requires_grad_(), w.cuda().requires_grad_(), b.cuda().requires_grad_()
+        with hooks:
+            y = A.GroupNormAct.apply(xg, 4, wg, bg, 1e-5, True)
+        return torch.autograd.grad(y, (xg, wg, bg), _place(r, layout))
+    want = grads(contextlib.nullcontext())
+    other = torch.autograd.graph.saved_tensors_hooks(
+        lambda t: t.cpu(), lambda t: t.cuda().transpose(1, -1).contiguous().transpose(1, -1) if t.dim() == 4 and layout == "planar"
+        else t.cuda().contiguous())
+    for hooks in (torch.autograd.graph.save_on_cpu(), other):
+        assert all(torch.equal(u, v) for u, v in zip(grads(hooks), want))
+
+
+@gpu
+def test_group_norm_keeps_no_answer_by_an_arguments_identity():
+    from boostmvsnerfs_amd import ops
+    x, eps = torch.randn(1, 4, 3, 3, device="cuda"), torch.tensor(1e-5)
+    a = ops.group_norm_fwd(x, 2, eps=eps)[0]
+    eps.fill_(3.0)
+    assert torch.equal(ops.group_norm_fwd(x, 2, eps=eps)[0], ops.group_norm_fwd(x, 2, eps=3.0)[0]) and not torch.equal(a, ops.group_norm_fwd(x, 2, eps=eps)[0])
 
 
 @gpu

@@ -145,6 +145,16 @@ def _converted(mod="enerf", group_size=8):
     return convert_group_norm(Network(), group_size)
 
 
+def test_another_optimisers_state_is_refused():
+    """Groups of one parameter each are as many in Adam's state: not loaded as if they were this one's."""
+    from boostmvsnerfs_amd.train import make_optimizer
+    net = torch.nn.Sequential(torch.nn.Linear(3, 4), torch.nn.Linear(4, 2))
+    adam, muon = make_optimizer(net), make_optimizer(net, optim="muon")
+    with pytest.raises(ValueError, match="groups"):
+        muon.load_state_dict(adam.state_dict())
+    muon.load_state_dict(copy.deepcopy(muon.state_dict()))
+
+
 @gpu
 def test_a_converted_regulariser_against_64_bits():
     """Outputs: 12 layers, each off by fp32 sums of at most 27 x 32 terms (a few 2^-22 of their size): 1e-4 in the 2-norm is

@@ -330,3 +330,7 @@ def test_refusals_on_the_gpu():
         ops.muon_step([m, m], [m.clone(), m.clone()], [m.clone(), m.clone()], 0.1)
     with pytest.raises(RuntimeError, match="overlaps"):
         ops.muon_step([m], [m], [m.clone()], 0.1)
+    wide = torch.zeros(8, 4, device="cuda").t()                # (goes through a copy)
+    for other in (wide, wide.t()):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            ops.muon_step([wide, other], [wide.clone(), other.clone()], [torch.zeros_like(wide), torch.zeros_like(other)], 0.1)
