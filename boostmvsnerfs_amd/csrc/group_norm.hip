@@ -762,7 +762,7 @@ static int gn_vec(long n, int size) {  // values per access: 16 bytes where the 
 // threads of a workgroup that holds `accesses` of them, kGnHold a thread; 0: too many
 static int gn_whole(long accesses) { return accesses <= 256 * kGnHold ? 256 : accesses <= 1024 * kGnHold ? 1024 : 0; }
 
-static GnPlan gn_plan(int N, int C, long S, int G, int dtype, int last) {
+static GnPlan gn_plan(int N, int C, long S, int G, int dtype, int last, bool backward) {
   GnPlan p{};
   GnArgs& a = p.a;
   a.N = N, a.C = C, a.S = S, a.G = G, a.cg = C / G, a.M = (long)a.cg * S;
@@ -800,15 +800,20 @@ static GnPlan gn_plan(int N, int C, long S, int G, int dtype, int last) {
         const int shared = ((g + 1) * a.cg - 1) / a.width - g * a.cg / a.width + 1;
         if (shared > a.slab_pieces) a.slab_pieces = shared;
       }
-    // rows of a chunk: about 1024 workgroups (four on a compute unit), of at least 2 accesses a thread
-    const long rpi = kGnThreads / wv, wgs = std::max(1l, 1024 / ((long)N * a.slabs));
+    // Rows of a chunk: 512 workgroups (two on a compute unit), of at least 2 accesses a thread.  What a workgroup does besides its
+    // rows -- joining the pieces, adding its rows' sums -- costs about as much as 8 accesses a thread, and more workgroups are more
+    // pieces to join: 3 x 32 x 128 x 160 backward 29.4 us with 1024, 17.6 with 512; 4 x 320 x 64 x 64 bf16 41.7, 30.6.  The forward's
+    // is less: 1024 where they have 7 accesses or more (3 x 8 x 512 x 640 23.4 -> 22.0 us, 3 x 32 x 512 x 640 72.8 -> 67.5).  And
+    // so few that their pieces need no launch of their own (1 x 256 x 128 x 128 bf16 forward 21 -> 16.4 us).
+    const long rpi = kGnThreads / wv, touched = std::min<long>((a.width + a.cg - 1) / a.cg + 1, G);
+    const long target = !backward && (long)N * a.slabs * S >= 7 * rpi * 1024 ? 1024 : 512;
+    const long wgs = std::max(1l, std::min(target / ((long)N * a.slabs), kGnMaxJoin / (touched * a.slab_pieces)));
     a.per = std::max(2 * rpi, ((S + wgs - 1) / wgs + rpi - 1) / rpi * rpi);
     const long chunks = (S + a.per - 1) / a.per;
     a.chunks = (int)chunks, a.pieces = a.chunks * a.slab_pieces, a.npc = a.chunks;
     a.pcn = (long)a.chunks * C, a.pck = C, a.pcc = 1;
     p.wgs = (long)N * a.slabs * a.chunks;
-    const long touched = (a.width + a.cg - 1) / a.cg + 1;
-    p.finish = std::min<long>(touched, G) * a.pieces > kGnMaxJoin;
+    p.finish = touched * a.pieces > kGnMaxJoin;
     // (one launch: the fewest channels that are whole groups and whole accesses; kGnHold passes of threads / accesses rows)
     if (unit <= kGnThreads) {
       p.held = unit * p.V;
@@ -939,7 +944,9 @@ static const char* gn_bad(const bmv_group_norm_spec* s) {
   if ((long)s->N * s->C > (1l << 24) || s->S > (1l << 40) / ((long)s->N * s->C)) return "the map is too large";
   return nullptr;
 }
-static GnPlan gn_plan_of(const bmv_group_norm_spec* s) { return gn_plan(s->N, s->C, s->S, s->G, s->dtype, s->channels_last); }
+static GnPlan gn_plan_of(const bmv_group_norm_spec* s, bool backward) {
+  return gn_plan(s->N, s->C, s->S, s->G, s->dtype, s->channels_last, backward);
+}
 
 }  // namespace bmv
 
@@ -950,7 +957,7 @@ extern "C" {
 long bmv_group_norm_workspace(const bmv_group_norm_spec* spec, int backward) {
   const char* bad = gn_bad(spec);
   BMV_REQUIRE(!bad, "bmv_group_norm_workspace: %s", bad);
-  const GnPlan p = gn_plan_of(spec);
+  const GnPlan p = gn_plan_of(spec, backward != 0);
   return 2 * (p.part + p.fin + (backward ? p.partc : 0));
 }
 
@@ -960,7 +967,7 @@ int bmv_group_norm_fwd(const bmv_group_norm_spec* spec, const void* x, const voi
   BMV_REQUIRE(!bad, "bmv_group_norm_fwd: %s", bad);
   BMV_REQUIRE(x && stats && workspace && y, "bmv_group_norm_fwd: null pointer");
   BMV_REQUIRE(gn_aligned(x) && gn_aligned(y) && gn_aligned(workspace), "bmv_group_norm_fwd: x, y and workspace begin at 16-byte addresses");
-  const GnPlan p = gn_plan_of(spec);
+  const GnPlan p = gn_plan_of(spec, false);
   GnArgs a = p.a;
   a.x = x, a.w = weight, a.b = bias, a.out = y, a.wdt = spec->param_dtype, a.eps = spec->eps, a.slope = spec->slope;
   a.mean = stats, a.rstd = stats + (long)a.N * a.G;
@@ -976,7 +983,7 @@ int bmv_group_norm_bwd(const bmv_group_norm_spec* spec, const void* x, const voi
   BMV_REQUIRE(x && dy && stats && workspace && dx, "bmv_group_norm_bwd: null pointer");
   BMV_REQUIRE(gn_aligned(x) && gn_aligned(dy) && gn_aligned(dx) && gn_aligned(workspace),
               "bmv_group_norm_bwd: x, dy, dx and workspace begin at 16-byte addresses");
-  const GnPlan p = gn_plan_of(spec);
+  const GnPlan p = gn_plan_of(spec, true);
   GnArgs a = p.a;
   a.x = x, a.dy = dy, a.w = weight, a.b = bias, a.out = dx, a.dw = dweight, a.db = dbias, a.wdt = spec->param_dtype, a.slope = spec->slope;
   a.mean = const_cast<double*>(stats), a.rstd = a.mean + (long)a.N * a.G;
