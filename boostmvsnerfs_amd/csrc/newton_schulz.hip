@@ -64,7 +64,7 @@ struct NsArgs {
   double* sq;           // partial sums of squares: [item][chunk], kNsList * sqn of them
   float* part;          // partial tiles
   int count, sqn, dtype, muon, nesterov, first, last, flip;
-  int least;            // short sides: columns of a workgroup at least
+  int least, spread;    // short sides: columns of a workgroup at least; slots of matrices that all XCDs share
   int full, run;        // a product's tiles that are a workgroup each; stages of a run of the others
   float a, b, c, eps, mu, nu, keep;      // nu: 1 - mu, rounded once
 };
@@ -534,12 +534,14 @@ __global__ void __launch_bounds__(256, 1) ns_block_kernel(NsArgs g) {
 // products are too small for the split of the operands to pay.
 // LDS rows are m + 4 floats (m a multiple of 16): rows 4 apart are 16 banks apart, which keeps both the 16-byte reads along k
 // (16 rows, one k) and the 4-byte reads across rows (16 values of rows 4 apart) free of conflicts.
-// T.  A step costs a workgroup 0.19 us (m = 128; 0.07 at 64) for each of its columns and 0.34 us (0.12) for each of the n / T
-// shares of A that it adds up, measured over 16, 32 and 64 columns: T^2 = 1.7 n or so for either, the power of two next to it --
-// unless the list then has more workgroups than fit the card at once: more columns each are cheaper than a second round.  (64
-// columns of more than 64 rows would be four blocks a wave: 10 % slower at 128 x 2048 than 32.)
-// Long sides: the shares that everybody adds up grow with n^2.  128 x 4096 285 us (through the large matrices' way 295),
+// T.  More columns cost a workgroup more, and every workgroup fewer shares of A to add up.  Five steps of 128 x 256 take 70 us
+// with 16 columns and 75 with 32, 128 x 512 103 and 89; 64 x 864 takes 51 us with 32 and 56 with 64, 64 x 1728 71 and 68.  A list
+// that has more workgroups than fit the card at once gets more columns each: cheaper than a second round.  (64 columns of more
+// than 64 rows would be four blocks a wave: 10 % slower at 128 x 2048 than 32.)
+// Long sides: the shares that everybody adds up grow with n^2.  128 x 4096 286 us (through the large matrices' way 295),
 // 128 x 8192 515 (438); 64 x 8192 130 (437).
+// A step's time: 128 x 128 10 us, 64 x 1728 12.5 us; the network of MVSNeRF, 29 matrices, 13.5 us.  4 us of it is one launch
+// behind another; the rest is a chain of shares, two products and the next share, of which the products are a quarter.
 constexpr int kNsShort = 128, kNsShortLong = 16384;      // short side, and long side (a quarter of it above 64 rows), up to which this way is taken
 __host__ __device__ __forceinline__ int ns_columns(int m, int n, int least) {
   const int t = n <= 288 ? 16 : n <= 1152 ? 32 : 64, u = t > least ? t : least;
@@ -563,15 +565,21 @@ __device__ __forceinline__ void ns_triangle(int b, int& i, int& j) {
   j = b - i * (i + 1) / 2;
 }
 
+// it.at of the matrices that have an XCD of their own: XCD << kNsXcd | slot
+constexpr int kNsXcd = 24;
+
 template <bool START>
 __global__ void __launch_bounds__(512) ns_short_kernel(NsArgs g) {
   extern __shared__ __align__(16) float sm[];
-  const int i = ns_find(g, blockIdx.x);
+  // (ns_place) workgroups go to the XCDs in turn: slot s of XCD x
+  const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, key = slot < g.spread ? slot : xcd << kNsXcd | slot, i = ns_find(g, key);
   const NsItem it = g.it[i];
   const NsShape shape(it.rows, it.cols);
   const NsShort s(shape, g.least);
+  const int wg = slot < g.spread ? (slot - it.at) * 8 + xcd : key - it.at;
+  if (wg >= s.parts) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, c16 = lane & 15;
-  const int wg = blockIdx.x - it.at, j0 = wg * s.T, nj = min(s.T, s.n - j0);
+  const int j0 = wg * s.T, nj = min(s.T, s.n - j0);
   float *xs = sm, *ys = xs + s.T * s.pitch, *as = ys + s.T * s.pitch;      // [column][row], [column][row], [row][row]
   float* x = reinterpret_cast<float*>(g.ws + it.ws);
   nsf4* in = reinterpret_cast<nsf4*>(x + s.x() + (g.flip ? s.share() : 0));
@@ -891,19 +899,50 @@ static void ns_fill(NsArgs& g, const NsLists& l, const int* idx, int n) {
   }
 }
 
-static void ns_run_short(NsArgs& g, int least, int steps, char* ws, hipStream_t st) {
-  long off = 0, wgs = 0;
-  int lds = 0;
-  g.ws = ws, g.least = least;
+// Which XCD computes which matrix; returns the workgroups of a launch.  Every workgroup of a matrix reads the shares of all others
+// of the launch before: on one XCD they are in its L2 (128 x 128 61.7 -> 55.2 us).  The matrices go to the XCDs by their work, the
+// largest first, each to the one that has least; one of more workgroups than an XCD has compute units is spread over all.
+static unsigned ns_place(NsArgs& g, int least) {
+  int parts[kNsList], order[kNsList], alone = 0, slots[8], most = 0;
+  long work[kNsList], load[8] = {};
+  g.spread = 0;
   for (int i = 0; i < g.count; ++i) {
     const NsShort s(NsShape(g.it[i].rows, g.it[i].cols), least);
-    g.it[i].ws = off, g.it[i].at = (int)wgs, off += s.bytes(), wgs += s.parts, lds = std::max(lds, s.lds());
+    parts[i] = s.parts;
+    if (s.parts > kNsUnits / 8) g.it[i].at = g.spread, g.spread += (s.parts + 7) / 8;
+    else {
+      // (0.01 us: a workgroup 2 us, and 0.0053 us for each block and column, 0.0094 for each block and share)
+      work[i] = (long)s.parts * (200 + s.blocks * (s.T / 2 + s.parts));
+      int k = alone++;
+      for (; k > 0 && work[order[k - 1]] < work[i]; --k) order[k] = order[k - 1];
+      order[k] = i;
+    }
+  }
+  for (int x = 0; x < 8; ++x) slots[x] = g.spread;
+  for (int k = 0; k < alone; ++k) {
+    const int i = order[k], x = (int)(std::min_element(load, load + 8) - load);
+    g.it[i].at = x << kNsXcd | slots[x];
+    load[x] += work[i], slots[x] += parts[i];
+  }
+  for (int x = 0; x < 8; ++x) most = std::max(most, slots[x]);
+  std::sort(g.it, g.it + g.count, [](const NsItem& a, const NsItem& b) { return a.at < b.at; });
+  return 8u * most;
+}
+
+static void ns_run_short(NsArgs& g, int least, int steps, char* ws, hipStream_t st) {
+  long off = 0;
+  int lds = 0;
+  g.ws = ws, g.least = least;
+  const dim3 grid(ns_place(g, least));
+  for (int i = 0; i < g.count; ++i) {
+    const NsShort s(NsShape(g.it[i].rows, g.it[i].cols), least);
+    g.it[i].ws = off, off += s.bytes(), lds = std::max(lds, s.lds());
   }
   g.flip = 1;                                             // (the first shares go to where step 0 reads)
-  hipLaunchKernelGGL(ns_short_kernel<true>, dim3((unsigned)wgs), dim3(512), lds, st, g);
+  hipLaunchKernelGGL(ns_short_kernel<true>, grid, dim3(512), lds, st, g);
   for (int k = 0; k < steps; ++k) {
     g.first = k == 0, g.last = k + 1 == steps, g.flip = k & 1;
-    hipLaunchKernelGGL(ns_short_kernel<false>, dim3((unsigned)wgs), dim3(512), lds, st, g);
+    hipLaunchKernelGGL(ns_short_kernel<false>, grid, dim3(512), lds, st, g);
   }
 }
 
