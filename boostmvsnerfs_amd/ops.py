@@ -1553,21 +1553,30 @@ NS_EPS = 1e-7
 
 
 def _matrices(tensors, name):
-    """(rows, cols) of each weight as a matrix: everything behind the first dimension is its columns.  (Lists of a network's
-    weights come here every step: one pass, names only for errors.)"""
-    sizes = []
+    """(rows, cols) of each weight as a matrix -- everything behind the first dimension is its columns --, and the indices of the
+    non-empty ones by (device index, dtype): a launch has one of each.  (Lists of a network's weights come here every step: one
+    pass, names only for errors.)"""
+    sizes, kinds, last = [], {}, None
     for i, t in enumerate(tensors):
-        if not (isinstance(t, torch.Tensor) and t.dtype in _FLOAT_CODES and t.is_cuda):
-            _gpu_float(t, f"{name}[{i}]")           # raises
+        kind = (t.get_device(), t.dtype) if isinstance(t, torch.Tensor) else None
+        if kind != last or kind is None:
+            if kind is None or kind[0] < 0 or kind[1] not in _FLOAT_CODES:
+                _gpu_float(t, f"{name}[{i}]")           # raises
+            last, idx = kind, kinds.setdefault(kind, [])
         shape = t.shape
-        if len(shape) < 2:
+        if len(shape) == 2:
+            rows, cols = shape
+        elif len(shape) > 2:
+            rows = shape[0]
+            cols = t.numel() // rows if rows else 0
+        else:
             raise ValueError(f"{name}[{i}]: expected a matrix (at least 2 dimensions), got {tuple(shape)}")
-        rows = shape[0]
-        cols = shape[1] if len(shape) == 2 else t.numel() // rows if rows else 0
         if rows > 65536 or cols > 65536:
             raise ValueError(f"{name}[{i}]: sides of up to 65536, got {rows} x {cols}")
         sizes.append((rows, cols))
-    return sizes
+        if rows and cols:
+            idx.append(i)
+    return sizes, [(k, v) for k, v in kinds.items() if v]
 
 
 def _ns_args(steps, coeffs, eps):
@@ -1579,15 +1588,6 @@ def _ns_args(steps, coeffs, eps):
     return int(steps), a, b, c, float(eps)
 
 
-def _by_kind(tensors, sizes):
-    """Indices of the non-empty tensors, by (device, dtype): a launch has one of each."""
-    kinds = {}
-    for i, t in enumerate(tensors):
-        if sizes[i][0] and sizes[i][1]:
-            kinds.setdefault((t.device, t.dtype), []).append(i)
-    return kinds.items()
-
-
 def _pointers(tensors):
     """Host array of the tensors' addresses; they stay referenced until the launch is enqueued (see _lib.dptr)."""
     _lib._held_list().extend(tensors)
@@ -1596,7 +1596,8 @@ def _pointers(tensors):
 
 def _sides(sizes, idx):
     n = C.c_int * len(idx)
-    return n(*[sizes[i][0] for i in idx]), n(*[sizes[i][1] for i in idx])
+    rows, cols = zip(*[sizes[i] for i in idx])
+    return n(*rows), n(*cols)
 
 
 def _ns_workspace(lib, count, rows, cols, dtype, device):
@@ -1615,17 +1616,18 @@ def newton_schulz(mats, steps=5, coeffs=NS_COEFFS, eps=NS_EPS):
         return newton_schulz([mats], steps, coeffs, eps)[0]
     mats = list(mats)
     steps, a, b, c, eps = _ns_args(steps, coeffs, eps)
-    sizes = _matrices(mats, "mats")
+    sizes, kinds = _matrices(mats, "mats")
     mats = [t if t.is_contiguous() else t.contiguous() for t in mats]
     out = [torch.empty_like(t) for t in mats]
     lib = _lib.load()
-    for (device, dtype), idx in _by_kind(mats, sizes):
+    for (_, dtype), idx in kinds:
         with _on_device_of(mats[idx[0]]):
             n = len(idx)
             rows, cols = _sides(sizes, idx)
-            ws = _ns_workspace(lib, n, rows, cols, dtype, device)
+            ws = _ns_workspace(lib, n, rows, cols, dtype, mats[idx[0]].device)
+            src, dst = (mats, out) if n == len(mats) else ([mats[i] for i in idx], [out[i] for i in idx])
             with _region("newton_schulz"):
-                rc = lib.bmv_newton_schulz(n, _pointers([mats[i] for i in idx]), _pointers([out[i] for i in idx]), rows, cols,
+                rc = lib.bmv_newton_schulz(n, _pointers(src), _pointers(dst), rows, cols,
                                            _FLOAT_CODES[dtype], steps, a, b, c, eps, ws.data_ptr(), ws.numel(), stream())
             _lib.check(rc, "newton_schulz")
     return out
@@ -1654,16 +1656,16 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
     if not 0 <= momentum < 1:
         raise ValueError(f"momentum: expected 0 <= momentum < 1, got {momentum}")
     lr, keep = float(lr), 1.0 - float(lr) * float(weight_decay)
-    sizes = _matrices(params, "params")
+    sizes, kinds = _matrices(params, "params")
     for i, (p, g, m) in enumerate(zip(params, grads, momenta)):
-        if not (isinstance(g, torch.Tensor) and g.shape == p.shape and g.dtype == p.dtype and g.device == p.device):
+        if not (isinstance(g, torch.Tensor) and g.shape == p.shape and g.dtype == p.dtype and g.get_device() == p.get_device()):
             _gpu_float(g, f"grads[{i}]", p)
             raise ValueError(f"grads[{i}]: expected {tuple(p.shape)} {p.dtype}, got {tuple(g.shape)} {g.dtype}")
-        if not (isinstance(m, torch.Tensor) and m.shape == p.shape and m.dtype == torch.float32 and m.device == p.device):
+        if not (isinstance(m, torch.Tensor) and m.shape == p.shape and m.dtype == torch.float32 and m.get_device() == p.get_device()):
             _gpu_float(m, f"momenta[{i}]", p)
             raise ValueError(f"momenta[{i}]: expected {tuple(p.shape)} float32, got {tuple(m.shape)} {m.dtype}")
     lib = _lib.load()
-    for (device, dtype), idx in _by_kind(params, sizes):
+    for (_, dtype), idx in kinds:
         with torch.no_grad(), _on_device_of(params[idx[0]]):
             n = len(idx)
             rows, cols = _sides(sizes, idx)
@@ -1672,7 +1674,7 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
             if any(a is not params[i] or b is not momenta[i] for a, b, i in zip(p, m, idx)):      # (copies do not overlap)
                 if len({t.data_ptr() for i in idx for t in (params[i], momenta[i])}) < 2 * n:
                     raise RuntimeError("muon_step: a weight or a momentum overlaps another tensor (is one listed twice?)")
-            ws = _ns_workspace(lib, n, rows, cols, dtype, device)
+            ws = _ns_workspace(lib, n, rows, cols, dtype, p[0].device)
             with _region("muon_step"):
                 rc = lib.bmv_muon_step(n, _pointers(p), _pointers([_c(grads[i]) for i in idx]), _pointers(m), rows, cols, scales,
                                        _FLOAT_CODES[dtype], float(momentum), int(bool(nesterov)), keep, steps, a, b, c, eps,
