@@ -442,19 +442,21 @@ __global__ void __launch_bounds__(256) ns_join_kernel(NsArgs g) {
   ns_finish<P, STAGE>(g, it, s, p, ti * kNsTile + (quarter >> 1) * 64, tj * kNsTile + (quarter & 1) * 64, ti == tj, tile);
 }
 
-// The same products 64 x 64 a workgroup, whole and in one launch: a wave has 32 x 32, a stage is 32 k-values.  Twice the bytes an
-// operation, and a compute unit holds one workgroup whose stages wait for memory -- so up to kBufs - 1 of them are on their way --,
-// but no partial tiles and no joining launch.
+// The same products 64 x 64 a workgroup, whole and in one launch: twice the bytes an operation, but no partial tiles and no joining
+// launch.  A compute unit has one workgroup, so nothing else hides its waits: each of the four waves takes every fourth block of 16
+// k-values for all of the 64 x 64, through a ring of stages of its own that it fills and reads without any barrier -- half the LDS
+// reads of waves that share stages and have 32 x 32 each, and none waits for another.  Their four sums meet at the end.
 template <int P>
-constexpr int kNsBlockBufs = P == 3 ? 6 : 8;
+constexpr int kNsBlockBufs = P == 3 ? 3 : 4;
 template <int P>
-constexpr int kNsBlockLds = kNsBlockBufs<P> * 2 * 2 * P * 1024 * 2;      // stages of two operands' two blocks of P pieces
+constexpr int kNsBlockLds = 4 * kNsBlockBufs<P> * 2 * P * 1024 * 2;      // waves, stages, operands' pieces of 64 rows of 16 k-values
 template <int P, int STAGE>
 __global__ void __launch_bounds__(256, 1) ns_block_kernel(NsArgs g) {
-  constexpr int kB = 2, kBufs = kNsBlockBufs<P>;
+  constexpr int kBufs = kNsBlockBufs<P>;
   constexpr int kPart = 1024;                             // elements of a piece of a block: 64 rows of 16 k-values
-  constexpr int kHalf = kB * P * kPart, kStage = 2 * kHalf, kLoads = kStage * 2 / 1024 / 4;
-  static_assert(kBufs * kStage * 2 == kNsBlockLds<P> && 64 * kNsPitch * 4 <= kNsBlockLds<P>, "LDS");
+  constexpr int kHalf = P * kPart, kStage = 2 * kHalf, kLoads = kStage * 2 / 1024;
+  constexpr int kSum = 64 * kNsPitch;
+  static_assert(4 * kBufs * kStage * 2 == kNsBlockLds<P> && (kSum + 3 * 1024) * 4 <= kBufs * kStage * 2 && kSum % 4 == 0, "LDS");
   extern __shared__ __align__(16) __bf16 stages_[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t = xcd_contiguous(blockIdx.x, gridDim.x), i = ns_find(g, t);
@@ -463,47 +465,48 @@ __global__ void __launch_bounds__(256, 1) ns_block_kernel(NsArgs g) {
   const NsPlanes<P> p(g.ws + it.ws, s);
   int ti, tj;
   ns_tile(t - it.at, 2 * s.mt(), 2 * s.nt(), STAGE != kNsApply, ti, tj);
-  const int K = STAGE == kNsGram ? s.np : s.mp, count = K / (kNsK * kB);
+  const int K = STAGE == kNsGram ? s.np : s.mp, count = K / (kNsK * 4);
   // a panel's half: rows 64 (t & 1) ... of every block's pieces
-  const long panel = (long)(K / kNsK) * (P * kNsCell);
-  const __bf16* L = (STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : p.q) + (ti >> 1) * panel + (ti & 1) * kPart;
-  const __bf16* R = (STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : (g.flip ? p.xt1 : p.xt)) + (tj >> 1) * panel + (tj & 1) * kPart;
+  const long panel = (long)(K / kNsK) * (P * kNsCell), mine = (long)wave * (P * kNsCell) + lane * 8;
+  const __bf16* L = (STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : p.q) + (ti >> 1) * panel + (ti & 1) * kPart + mine;
+  const __bf16* R = (STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : (g.flip ? p.xt1 : p.xt)) + (tj >> 1) * panel + (tj & 1) * kPart + mine;
+  __bf16* ring = stages_ + wave * (kBufs * kStage);
   auto fill = [&](int k) {
-    __bf16* to = stages_ + k % kBufs * kStage;
+    __bf16* to = ring + k % kBufs * kStage;
+    const long at = (long)k * (4 * P * kNsCell);
 #pragma unroll
-    for (int h = 0; h < kLoads; ++h) {
-      const int c = wave + 4 * h, d = c % (kLoads * 2);   // (1 KB = half a piece of a block; L's first, then R's)
-      const __bf16* from = (c < kLoads * 2 ? L : R) + (long)k * (kB * P * kNsCell) + (d >> 1) * kNsCell + (d & 1) * 512;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + lane * 8),
+    for (int c = 0; c < kLoads; ++c) {                    // (1 KB = half a piece of a block; L's first, then R's)
+      const int d = c % (kLoads / 2);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((c < kLoads / 2 ? L : R) + at + (d >> 1) * kNsCell + (d & 1) * 512),
                                        (__attribute__((address_space(3))) void*)(to + c * 512), 16, 0, 0);
     }
   };
-  const int lr = (wave >> 1) * 32 + (lane & 31), rr = (wave & 1) * 32 + (lane & 31), oct = lane >> 5;
-  auto read = [&](int k, int b, int operand, int q, int row) {
-    return *reinterpret_cast<const nsb8*>(stages_ + k % kBufs * kStage + operand * kHalf + (b * P + q) * kPart + row * kNsK + ((oct ^ row >> 3) & 1) * 8);
-  };
-  nsf16 acc = {}, low = {};
-  nsb8 lf[2][kB][P], rf[2][kB][P];                        // operands of the stage that is multiplied, and of the next
+  const int row = lane & 31, oct = lane >> 5, cell = row * kNsK + ((oct ^ row >> 3) & 1) * 8;      // (32 rows on: the same cell)
+  nsf16 acc[2][2] = {}, low[2][2] = {};
+  nsb8 lf[2][2][P], rf[2][2][P];                          // operands of the stage that is multiplied, and of the next
   auto fetch = [&](int k, int into) {
+    const __bf16* b = ring + k % kBufs * kStage + cell;
 #pragma unroll
-    for (int b = 0; b < kB; ++b)
+    for (int q = 0; q < P; ++q)
 #pragma unroll
-      for (int q = 0; q < P; ++q) lf[into][b][q] = read(k, b, 0, q, lr), rf[into][b][q] = read(k, b, 1, q, rr);
+      for (int e = 0; e < 2; ++e) {
+        lf[into][e][q] = *reinterpret_cast<const nsb8*>(b + q * kPart + e * 32 * kNsK);
+        rf[into][e][q] = *reinterpret_cast<const nsb8*>(b + kHalf + q * kPart + e * 32 * kNsK);
+      }
   };
-  // stage k is in LDS for everybody (behind it up to kBufs - 2 may be on their way), and nobody reads stage k - 1 any more
+  // stage k is in LDS (behind it up to kBufs - 2 may be on their way), and the operands of stage k - 1 in registers
   auto arrive = [&](int k) {
-    if (k + kBufs - 2 < count) asm volatile("s_waitcnt vmcnt(%0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::"n"((kBufs - 2) * kLoads) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (k + kBufs - 2 < count) asm volatile("s_waitcnt vmcnt(%0)\n\ts_waitcnt lgkmcnt(0)" ::"n"((kBufs - 2) * kLoads) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)" ::: "memory");
   };
   for (int k = 0; k < kBufs - 1 && k < count; ++k) fill(k);
   arrive(0);
   if (kBufs - 1 < count) fill(kBufs - 1);
   fetch(0, 0);
-  for (int k = 0; k < count; k += 2)                      // (an even number of stages: k is a multiple of 128)
+  for (int k = 0; k < count; k += 2)                      // (an even number of stages: K is a multiple of 128)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      // the next stage's operands are read under this one's products: all four waves would otherwise first read, then multiply
-      // (behind the last stage: that one again, unused)
+      // the next stage's operands are read under this one's products (behind the last stage: that one again, unused)
       arrive(k + u + 1);
       if (k + u + kBufs < count) fill(k + u + kBufs);
       fetch(min(k + u + 1, count - 1), u ^ 1);
@@ -512,15 +515,39 @@ __global__ void __launch_bounds__(256, 1) ns_block_kernel(NsArgs g) {
 #pragma unroll
         for (int q = sum; q >= 0; --q)
 #pragma unroll
-          for (int b = 0; b < kB; ++b)
-            if (sum) low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[u][b][q], rf[u][b][sum - q], low, 0, 0, 0);
-            else acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[u][b][q], rf[u][b][sum - q], acc, 0, 0, 0);
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+              if (sum) low[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[u][e][q], rf[u][f][sum - q], low[e][f], 0, 0, 0);
+              else acc[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[u][e][q], rf[u][f][sum - q], acc[e][f], 0, 0, 0);
+    }
+  // Wave w finishes the 32 x 32 block w of the sums: the others' shares of it come through their rings, behind the tile's space
+  arrive(count);
+  constexpr int kRing = kBufs * kStage / 2, kOut = kSum;  // floats
+  float* tile = reinterpret_cast<float*>(stages_);
+  nsf4 own[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      nsf4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = acc[b >> 1][b & 1][4 * r + j] + low[b >> 1][b & 1][4 * r + j];
+      if (b == wave) own[r] = v;
+      else *reinterpret_cast<nsf4*>(tile + wave * kRing + kOut + ((b - wave - 1 & 3) * 4 + r) * 256 + lane * 4) = v;
     }
   __syncthreads();
-  float* tile = reinterpret_cast<float*>(stages_);
 #pragma unroll
-  for (int r = 0; r < 16; ++r)
-    tile[((wave >> 1) * 32 + 8 * (r >> 2) + 4 * oct + (r & 3)) * kNsPitch + (wave & 1) * 32 + (lane & 31)] = acc[r] + low[r];
+  for (int d = 1; d < 4; ++d) {
+    const int from = wave + d & 3;                        // (its shares: blocks from + 1, from + 2, from + 3)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) own[r] += *reinterpret_cast<const nsf4*>(tile + from * kRing + kOut + ((wave - from - 1 & 3) * 4 + r) * 256 + lane * 4);
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      tile[((wave >> 1) * 32 + 8 * r + 4 * oct + j) * kNsPitch + (wave & 1) * 32 + row] = own[r][j];
   __syncthreads();
   ns_finish<P, STAGE>(g, it, s, p, ti * 64, tj * 64, ti == tj, tile);
 }
@@ -841,7 +868,7 @@ static long ns_workspace(int count, const int* rows, const int* cols, int dtype,
 // a compute unit walks.  fp32: 6.3 us and 0.4 us for 32 k-values, against 14 ... 25 us for cut tiles and the launch that joins
 // them: 333 x 1000 (k = 1024) 18.9 us (cut 20.5), 1024 x 1024 21.5 (27), 512 x 2048 (k = 2048) 31.9 (24).  bf16: 4.5 and 0.24 us,
 // 1024 x 1024 14 us (24), k = 2048 20 (18).
-constexpr int kNsBlockK = 1024;
+constexpr int kNsBlockK = 2048;
 template <int P, int STAGE>
 static bool ns_blocks(NsArgs& g, hipStream_t st) {
   long blocks = 0, most = 0;

@@ -45,7 +45,7 @@ Knob g_knobs[] = {
     {"BMV_SWEEP_QUAD_L1", "quad-planar sweep: default tuning variant where the source maps have the volume's resolution"},
     {"BMV_DETERMINISTIC", "1 = the host takes the *_fixed scatter entry points (order-independent fixed-point accumulation): bit-reproducible gradients"},
     {"BMV_NS_SHORT", "Newton-Schulz iteration: short side up to which a step is one launch (default and at most 128; 0 = none)"},
-    {"BMV_NS_BLOCK_K", "Newton-Schulz products: k-values a compute unit walks, up to which 64 x 64 blocks run whole (default 1024; 0 = always tiles of 128 x 128, cut along k)"},
+    {"BMV_NS_BLOCK_K", "Newton-Schulz products: k-values a compute unit walks, up to which 64 x 64 blocks run whole (default 2048; 0 = always tiles of 128 x 128, cut along k)"},
     {"BMV_FPN_TOPDOWN_SPLIT", "FPN top-down step: workgroups sharing the output channels of a pixel (1, 2, 4)"},
 };
 constexpr int kNumKnobs = sizeof(g_knobs) / sizeof(g_knobs[0]);
