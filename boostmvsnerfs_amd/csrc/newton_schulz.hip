@@ -20,10 +20,15 @@
 // What a stage of a product loads is one run of memory per operand, moved to LDS by 16-byte DMA with no registers and next to
 // no address arithmetic.  A and Q are symmetric: only tiles on and below the diagonal are computed.
 //
-// Work.  A product's tiles of 128 x 128 are as many workgroups while they fill the card; the rest (all of them, for matrices
-// of a few hundred) is cut along k into equal runs of stages over all compute units, whose partial tiles the joining launch
-// adds in a fixed order.  That launch also applies the polynomial, splits the values and writes both orientations.
-// A stage of the whole list is one launch: a workgroup finds its matrix in a table of the kernel arguments.
+// Work.  Matrices of up to 1000 or so: a product is one launch of 64 x 64 blocks (ns_block_kernel).  Above, its tiles of 128 x 128
+// are as many workgroups while they fill the card; the rest is cut along k into equal runs of stages over all compute units, whose
+// partial tiles the joining launch adds in a fixed order.  That launch also applies the polynomial, splits the values and writes
+// both orientations.  A product of the whole list is one launch: a workgroup finds its matrix in a table of the kernel arguments.
+//
+// What bounds it.  4096 x 4096 fp32: Q X takes 612 us, 1347 TFLOP/s of bf16 products -- a large product of the library reaches
+// 1247 on this card --, with the matrix pipe 66 % busy at the 1.9 GHz that its power leaves.  Joins are 10 ... 20 % on top
+// (4096 x 4096: 100 of 1365 us a step) and move their bytes at 4 ... 5 TB/s.  Below 1000 or so it is the chain: 15 launches, of
+// which 7.5 us each are start, first operands and end.
 //
 // Matrices with a short side of up to 128 (every layer of the networks here) go another way, one launch a step: see below.
 #include <algorithm>
@@ -107,6 +112,7 @@ __device__ __forceinline__ long ns_cell(int r, int k, int K) {
 __device__ __forceinline__ int ns_find(const NsArgs& g, int at) {
   static_assert(kNsList <= 64, "a lane each");
   const int lane = threadIdx.x & 63;
+  if (g.count == 1) return 0;                             // (0.2 us of a launch)
   return __popcll(__ballot(lane < g.count && g.it[min(lane, kNsList - 1)].at <= at)) - 1;
 }
 
@@ -864,10 +870,10 @@ static long ns_workspace(int count, const int* rows, const int* cols, int dtype,
   return most;
 }
 
-// 64 x 64 blocks, where a round of them on all compute units is cheaper than tiles, a cut along k and a join: that goes by the k
-// a compute unit walks.  fp32: 6.3 us and 0.4 us for 32 k-values, against 14 ... 25 us for cut tiles and the launch that joins
-// them: 333 x 1000 (k = 1024) 18.9 us (cut 20.5), 1024 x 1024 21.5 (27), 512 x 2048 (k = 2048) 31.9 (24).  bf16: 4.5 and 0.24 us,
-// 1024 x 1024 14 us (24), k = 2048 20 (18).
+// 64 x 64 blocks, where rounds of them on all compute units are cheaper than tiles, a cut along k and a join: that goes by the k
+// a compute unit walks.  A launch of them is 7.5 us and 0.2 (bf16: 0.13) us for 32 k-values -- k = 384 9.9 us, 1024 13.7 ... 19.3
+// by how many blocks share the caches --, cut tiles and the launch that joins them 14 ... 25.  Five steps with blocks up to 2048
+// and up to 1024: 1024 x 2048 402 us and 428, bf16 294 and 328, 768 x 2048 334 and 350, 512 x 2048 251 and 246.
 constexpr int kNsBlockK = 2048;
 template <int P, int STAGE>
 static bool ns_blocks(NsArgs& g, hipStream_t st) {
