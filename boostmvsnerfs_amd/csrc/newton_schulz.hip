@@ -448,57 +448,82 @@ __global__ void __launch_bounds__(256) ns_join_kernel(NsArgs g) {
   ns_finish<P, STAGE>(g, it, s, p, ti * kNsTile + (quarter >> 1) * 64, tj * kNsTile + (quarter & 1) * 64, ti == tj, tile);
 }
 
-// The same products 64 x 64 a workgroup, whole and in one launch: twice the bytes an operation, but no partial tiles and no joining
+// The same products whole and in one launch, 32 E x 64 a workgroup: more bytes an operation, but no partial tiles and no joining
 // launch.  A compute unit has one workgroup, so nothing else hides its waits: each of the four waves takes every fourth block of 16
-// k-values for all of the 64 x 64, through a ring of stages of its own that it fills and reads without any barrier -- half the LDS
-// reads of waves that share stages and have 32 x 32 each, and none waits for another.  Their four sums meet at the end.
-template <int P>
-constexpr int kNsBlockBufs = P == 3 ? 3 : 4;
-template <int P>
-constexpr int kNsBlockLds = 4 * kNsBlockBufs<P> * 2 * P * 1024 * 2;      // waves, stages, operands' pieces of 64 rows of 16 k-values
-template <int P, int STAGE>
+// k-values for all of the 32 E x 64, through a ring of stages of its own that it fills and reads without any barrier -- half the LDS
+// reads of waves that share stages, and none waits for another.  Their four sums meet at the end.  E = 4 (two pieces: one sum for
+// all products, which costs 2^-24 where the pieces leave 2^-17 out; symmetric products) is a third more operations for each byte.
+template <int P, int E>
+constexpr int kNsBlockBufs = P == 2 && E == 2 ? 4 : 3;
+template <int P, int E>
+constexpr int kNsBlockLds = 4 * kNsBlockBufs<P, E> * P * (E + 2) * 1024; // waves, stages, pieces of 32 E + 64 rows of 16 k-values
+__host__ __device__ __forceinline__ int ns_block_count(const NsShape& s, int stage, int E) {
+  if (E == 4) return s.mt() * (s.mt() + 1);               // (symmetric products only)
+  return stage == kNsApply ? 4 * s.mt() * s.nt() : s.mt() * (2 * s.mt() + 1);
+}
+// block t of 128 x 64 of a symmetric product: its rows' panel and its half panel of columns, up to the panel's last.  Super-rows of 4.
+__device__ __forceinline__ void ns_block_tall(int t, int mt, int& i, int& j) {
+  int sr = 0;
+  while (16 * (sr + 1) * (sr + 1) + 4 * (sr + 1) <= t) ++sr;      // (blocks above super-row sr: 16 sr^2 + 4 sr)
+  t -= 16 * sr * sr + 4 * sr;
+  const int h = min(4, mt - 4 * sr);
+  if (t < 8 * sr * h) {
+    i = 4 * sr + t % h, j = t / h;
+    return;
+  }
+  t -= 8 * sr * h;
+  int l = 0;
+  while ((l + 1) * (l + 2) <= t) ++l;
+  i = 4 * sr + l, j = 8 * sr + t - l * (l + 1);
+}
+template <int P, int STAGE, int E>
 __global__ void __launch_bounds__(256, 1) ns_block_kernel(NsArgs g) {
-  constexpr int kBufs = kNsBlockBufs<P>;
-  constexpr int kPart = 1024;                             // elements of a piece of a block: 64 rows of 16 k-values
-  constexpr int kHalf = P * kPart, kStage = 2 * kHalf, kLoads = kStage * 2 / 1024;
-  constexpr int kSum = 64 * kNsPitch;
-  static_assert(4 * kBufs * kStage * 2 == kNsBlockLds<P> && (kSum + 3 * 1024) * 4 <= kBufs * kStage * 2 && kSum % 4 == 0, "LDS");
+  constexpr int kBufs = kNsBlockBufs<P, E>;
+  constexpr int kLeft = P * E * 512, kStage = kLeft + P * 1024, kLoads = P * (E + 2);      // elements of the left operand's part, of a stage; 1 KB DMAs
+  constexpr bool kLow = E == 2;                           // sums of their own for the small products
+  constexpr int kSum = 64 * kNsPitch, kOwn = E / 2;       // floats of a 64 x 64 tile; 32 x 32 blocks that a wave finishes
+  constexpr bool kApart = (kSum + 3 * kOwn * 1024) * 4 <= kBufs * kStage * 2;      // the finished tile and the shares have room beside each other
+  static_assert(4 * kBufs * kStage * 2 == kNsBlockLds<P, E> && 3 * kOwn * 4096 <= kBufs * kStage * 2 && kSum % 4 == 0, "LDS");
   extern __shared__ __align__(16) __bf16 stages_[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = xcd_contiguous(blockIdx.x, gridDim.x), i = ns_find(g, t);
+  // an XCD has an eighth of every matrix' blocks, one run of them
+  const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, i = ns_find(g, slot);
   const NsItem it = g.it[i];
   const NsShape s(it.rows, it.cols);
+  const int blocks = ns_block_count(s, STAGE, E), t = xcd * ((blocks + 7) / 8) + slot - it.at;
+  if (t >= blocks || slot - it.at >= (blocks + 7) / 8) return;
   const NsPlanes<P> p(g.ws + it.ws, s);
   int ti, tj;
-  ns_tile(t - it.at, 2 * s.mt(), 2 * s.nt(), STAGE != kNsApply, ti, tj);
+  if (E == 2) ns_tile(t, 2 * s.mt(), 2 * s.nt(), STAGE != kNsApply, ti, tj);
+  else ns_block_tall(t, s.mt(), ti, tj);
   const int K = STAGE == kNsGram ? s.np : s.mp, count = K / (kNsK * 4);
-  // a panel's half: rows 64 (t & 1) ... of every block's pieces
+  // (a half panel: rows 64 (t & 1) ... of every block's pieces)
   const long panel = (long)(K / kNsK) * (P * kNsCell), mine = (long)wave * (P * kNsCell) + lane * 8;
-  const __bf16* L = (STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : p.q) + (ti >> 1) * panel + (ti & 1) * kPart + mine;
-  const __bf16* R = (STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : (g.flip ? p.xt1 : p.xt)) + (tj >> 1) * panel + (tj & 1) * kPart + mine;
+  const __bf16* L = (STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : p.q) + (E == 2 ? (ti >> 1) * panel + (ti & 1) * 1024 : ti * panel) + mine;
+  const __bf16* R = (STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : (g.flip ? p.xt1 : p.xt)) + (tj >> 1) * panel + (tj & 1) * 1024 + mine;
   __bf16* ring = stages_ + wave * (kBufs * kStage);
   auto fill = [&](int k) {
     __bf16* to = ring + k % kBufs * kStage;
     const long at = (long)k * (4 * P * kNsCell);
 #pragma unroll
-    for (int c = 0; c < kLoads; ++c) {                    // (1 KB = half a piece of a block; L's first, then R's)
-      const int d = c % (kLoads / 2);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((c < kLoads / 2 ? L : R) + at + (d >> 1) * kNsCell + (d & 1) * 512),
+    for (int c = 0; c < kLoads; ++c) {                    // (1 KB = 32 rows of a piece of a block; L's first, then R's)
+      const int d = c < P * E ? c / E * kNsCell + c % E * 512 : (c - P * E) / 2 * kNsCell + (c - P * E) % 2 * 512;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((c < P * E ? L : R) + at + d),
                                        (__attribute__((address_space(3))) void*)(to + c * 512), 16, 0, 0);
     }
   };
   const int row = lane & 31, oct = lane >> 5, cell = row * kNsK + ((oct ^ row >> 3) & 1) * 8;      // (32 rows on: the same cell)
-  nsf16 acc[2][2] = {}, low[2][2] = {};
-  nsb8 lf[2][2][P], rf[2][2][P];                          // operands of the stage that is multiplied, and of the next
+  nsf16 acc[E][2] = {}, low[kLow ? E : 1][2] = {};
+  nsb8 lf[2][E][P], rf[2][2][P];                          // operands of the stage that is multiplied, and of the next
   auto fetch = [&](int k, int into) {
     const __bf16* b = ring + k % kBufs * kStage + cell;
 #pragma unroll
-    for (int q = 0; q < P; ++q)
+    for (int q = 0; q < P; ++q) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        lf[into][e][q] = *reinterpret_cast<const nsb8*>(b + q * kPart + e * 32 * kNsK);
-        rf[into][e][q] = *reinterpret_cast<const nsb8*>(b + kHalf + q * kPart + e * 32 * kNsK);
-      }
+      for (int e = 0; e < E; ++e) lf[into][e][q] = *reinterpret_cast<const nsb8*>(b + (q * E + e) * 512);
+#pragma unroll
+      for (int f = 0; f < 2; ++f) rf[into][f][q] = *reinterpret_cast<const nsb8*>(b + kLeft + (q * 2 + f) * 512);
+    }
   };
   // stage k is in LDS (behind it up to kBufs - 2 may be on their way), and the operands of stage k - 1 in registers
   auto arrive = [&](int k) {
@@ -521,41 +546,54 @@ __global__ void __launch_bounds__(256, 1) ns_block_kernel(NsArgs g) {
 #pragma unroll
         for (int q = sum; q >= 0; --q)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+          for (int e = 0; e < E; ++e)
 #pragma unroll
-            for (int f = 0; f < 2; ++f)
-              if (sum) low[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[u][e][q], rf[u][f][sum - q], low[e][f], 0, 0, 0);
-              else acc[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[u][e][q], rf[u][f][sum - q], acc[e][f], 0, 0, 0);
+            for (int f = 0; f < 2; ++f) {
+              nsf16& to = kLow && sum ? low[kLow ? e : 0][f] : acc[e][f];
+              to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[u][e][q], rf[u][f][sum - q], to, 0, 0, 0);
+            }
     }
-  // Wave w finishes the 32 x 32 block w of the sums: the others' shares of it come through their rings, behind the tile's space
+  // Wave w finishes kOwn 32 x 32 blocks of the sums, from w kOwn on: the others' shares of them come through their rings
   arrive(count);
-  constexpr int kRing = kBufs * kStage / 2, kOut = kSum;  // floats
+  constexpr int kRing = kBufs * kStage / 2, kOut = kApart ? kSum : 0;      // floats
   float* tile = reinterpret_cast<float*>(stages_);
-  nsf4 own[4];
+  nsf4 own[kOwn][4];
 #pragma unroll
-  for (int b = 0; b < 4; ++b)
+  for (int b = 0; b < 2 * E; ++b)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       nsf4 v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = acc[b >> 1][b & 1][4 * r + j] + low[b >> 1][b & 1][4 * r + j];
-      if (b == wave) own[r] = v;
-      else *reinterpret_cast<nsf4*>(tile + wave * kRing + kOut + ((b - wave - 1 & 3) * 4 + r) * 256 + lane * 4) = v;
+      for (int j = 0; j < 4; ++j) v[j] = acc[b >> 1][b & 1][4 * r + j] + (kLow ? low[kLow ? b >> 1 : 0][b & 1][4 * r + j] : 0.f);
+      if (b / kOwn == wave) own[b % kOwn][r] = v;
+      else *reinterpret_cast<nsf4*>(tile + wave * kRing + kOut + (((b / kOwn - wave - 1 & 3) * kOwn + b % kOwn) * 4 + r) * 256 + lane * 4) = v;
     }
   __syncthreads();
 #pragma unroll
   for (int d = 1; d < 4; ++d) {
-    const int from = wave + d & 3;                        // (its shares: blocks from + 1, from + 2, from + 3)
+    const int from = wave + d & 3;                        // (its shares: blocks of wave from + 1, from + 2, from + 3)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) own[r] += *reinterpret_cast<const nsf4*>(tile + from * kRing + kOut + ((wave - from - 1 & 3) * 4 + r) * 256 + lane * 4);
+    for (int o = 0; o < kOwn; ++o)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        own[o][r] += *reinterpret_cast<const nsf4*>(tile + from * kRing + kOut + (((wave - from - 1 & 3) * kOwn + o) * 4 + r) * 256 + lane * 4);
   }
+  if (!kApart) __syncthreads();
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+  for (int o = 0; o < kOwn; ++o) {
+    const int b = wave * kOwn + o;                        // row block b / 2, column block b % 2
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      tile[((wave >> 1) * 32 + 8 * r + 4 * oct + j) * kNsPitch + (wave & 1) * 32 + row] = own[r][j];
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        tile[(b >> 2) * kSum + ((b >> 1 & 1) * 32 + 8 * r + 4 * oct + j) * kNsPitch + (b & 1) * 32 + row] = own[o][r][j];
+  }
   __syncthreads();
-  ns_finish<P, STAGE>(g, it, s, p, ti * 64, tj * 64, ti == tj, tile);
+#pragma unroll
+  for (int h = 0; h < E / 2; ++h) {
+    const int rb = ti * (E / 2) + h;                      // (symmetric, 128 x 64: the upper half may lie above the diagonal)
+    if (STAGE == kNsApply || rb >= tj) ns_finish<P, STAGE>(g, it, s, p, rb * 64, tj * 64, rb == tj, tile + h * kSum);
+  }
 }
 
 // ---- short sides of up to 128 ------------------------------------------------------------------------------------------------
@@ -875,21 +913,46 @@ static long ns_workspace(int count, const int* rows, const int* cols, int dtype,
 // by how many blocks share the caches --, cut tiles and the launch that joins them 14 ... 25.  Five steps with blocks up to 2048
 // and up to 1024: 1024 x 2048 402 us and 428, bf16 294 and 328, 768 x 2048 334 and 350, 512 x 2048 251 and 246.
 constexpr int kNsBlockK = 2048;
+template <int P, int STAGE, int E>
+static void ns_block_launch(NsArgs& g, hipStream_t st) {
+  // (the longest first: an item's blocks begin in the order of the list)
+  std::stable_sort(g.it, g.it + g.count, [](const NsItem& a, const NsItem& b) {
+    auto k = [](const NsItem& i) { const NsShape s(i.rows, i.cols); return STAGE == kNsGram ? s.np : s.mp; };
+    return k(a) > k(b);
+  });
+  int slots = 0;
+  for (int i = 0; i < g.count; ++i) g.it[i].at = slots, slots += (ns_block_count(NsShape(g.it[i].rows, g.it[i].cols), STAGE, E) + 7) / 8;
+  hipLaunchKernelGGL((ns_block_kernel<P, STAGE, E>), dim3(8u * slots), dim3(256), (kNsBlockLds<P, E>), st, g);
+}
+// 128 x 64 blocks for symmetric products of two pieces that are too large for those: where they keep the compute units busy for
+// kNsTallBusy of the longest one's time, and that is no longer than kNsTallK k-values.  Five steps with them and with tiles (bf16):
+// 1500 x 1500 445 us and 492, 3000 x 3000 2055 and 2255, eight of 768 x 768 562 and 600, two of 1024 x 4096 with four of 1024 x 1024
+// 1030 and 1131.  Below that share tiles' cut along k is better (A of 1024 x 4096, 28 % busy: 38 us and 28), above that length
+// their traffic is (4096 x 4096: 2 % slower).  Q X has whole tiles for all compute units sooner: 3 ... 6 % slower with these.
+constexpr int kNsTallBusy = 60, kNsTallK = 10240;
 template <int P, int STAGE>
 static bool ns_blocks(NsArgs& g, hipStream_t st) {
-  long blocks = 0, most = 0;
+  long blocks = 0, most = 0, work = 0, least = 1 << 20;
   for (int i = 0; i < g.count; ++i) {
     const NsShape s(g.it[i].rows, g.it[i].cols);
-    blocks += STAGE == kNsApply ? 4l * s.mt() * s.nt() : (long)s.mt() * (2 * s.mt() + 1);
-    most = std::max<long>(most, STAGE == kNsGram ? s.np : s.mp);
+    const long k = STAGE == kNsGram ? s.np : s.mp;
+    blocks += ns_block_count(s, STAGE, 2), work += k * ns_block_count(s, STAGE, 4);
+    most = std::max(most, k), least = std::min(least, k);
   }
-  if ((blocks + kNsUnits - 1) / kNsUnits * most > tuning("BMV_NS_BLOCK_K", kNsBlockK)) return false;
-  for (int i = 0, at = 0; i < g.count; ++i) {
-    const NsShape s(g.it[i].rows, g.it[i].cols);
-    g.it[i].at = at, at += STAGE == kNsApply ? 4 * s.mt() * s.nt() : s.mt() * (2 * s.mt() + 1);
+  const long limit = tuning("BMV_NS_BLOCK_K", kNsBlockK);
+  if ((blocks + kNsUnits - 1) / kNsUnits * most <= limit) {
+    ns_block_launch<P, STAGE, 2>(g, st);
+    return true;
   }
-  hipLaunchKernelGGL((ns_block_kernel<P, STAGE>), dim3((unsigned)blocks), dim3(256), kNsBlockLds<P>, st, g);
-  return true;
+  if constexpr (P == 2 && STAGE != kNsApply) {
+    // k-values of the compute unit that has most, in rounds of the shortest blocks
+    const long span = std::max(most, (work + kNsUnits * least - 1) / (kNsUnits * least) * least);
+    if (limit > 0 && span <= kNsTallK && work * 100 >= span * kNsUnits * kNsTallBusy) {
+      ns_block_launch<P, STAGE, 4>(g, st);
+      return true;
+    }
+  }
+  return false;
 }
 
 template <int P, int STAGE>
@@ -1010,12 +1073,14 @@ static bool ns_lds() {
   if (ready.load(std::memory_order_acquire) & bit) return true;
   const std::pair<const void*, int> f[] = {{(const void*)ns_short_kernel<true>, kLds},
                                            {(const void*)ns_short_kernel<false>, kLds},
-                                           {(const void*)ns_block_kernel<3, kNsGram>, kNsBlockLds<3>},
-                                           {(const void*)ns_block_kernel<3, kNsPoly>, kNsBlockLds<3>},
-                                           {(const void*)ns_block_kernel<3, kNsApply>, kNsBlockLds<3>},
-                                           {(const void*)ns_block_kernel<2, kNsGram>, kNsBlockLds<2>},
-                                           {(const void*)ns_block_kernel<2, kNsPoly>, kNsBlockLds<2>},
-                                           {(const void*)ns_block_kernel<2, kNsApply>, kNsBlockLds<2>}};
+                                           {(const void*)ns_block_kernel<3, kNsGram, 2>, kNsBlockLds<3, 2>},
+                                           {(const void*)ns_block_kernel<3, kNsPoly, 2>, kNsBlockLds<3, 2>},
+                                           {(const void*)ns_block_kernel<3, kNsApply, 2>, kNsBlockLds<3, 2>},
+                                           {(const void*)ns_block_kernel<2, kNsGram, 2>, kNsBlockLds<2, 2>},
+                                           {(const void*)ns_block_kernel<2, kNsPoly, 2>, kNsBlockLds<2, 2>},
+                                           {(const void*)ns_block_kernel<2, kNsApply, 2>, kNsBlockLds<2, 2>},
+                                           {(const void*)ns_block_kernel<2, kNsGram, 4>, kNsBlockLds<2, 4>},
+                                           {(const void*)ns_block_kernel<2, kNsPoly, 4>, kNsBlockLds<2, 4>}};
   for (const auto& k : f)
     if (hipFuncSetAttribute(k.first, hipFuncAttributeMaxDynamicSharedMemorySize, k.second) != hipSuccess) return false;
   ready.fetch_or(bit, std::memory_order_release);

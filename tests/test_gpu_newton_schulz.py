@@ -128,6 +128,26 @@ def test_newton_schulz_large_matrices():
 
 
 @gpu
+def test_newton_schulz_lists_that_fill_the_card():
+    """bf16 symmetric products in blocks of 128 x 64, which are taken where the list keeps the compute units busy: panels of one
+    to four, sides on and off their borders, tall and wide, two lengths of k.  And a large matrix alone."""
+    from boostmvsnerfs_amd import _lib, ops
+    sizes = [(129, 140), (256, 256), (257, 400), (300, 150), (384, 129), (130, 131), (400, 512), (511, 385)]
+    mats = [_grad(*sizes[i % len(sizes)], seed=i).bfloat16() for i in range(64)]
+    on_gpu = [v.cuda() for v in mats]
+    _lib.set_tuning("BMV_NS_BLOCK_K", 1)
+    try:
+        out, again = ops.newton_schulz(on_gpu), ops.newton_schulz(on_gpu)
+    finally:
+        _lib.set_tuning("BMV_NS_BLOCK_K", None)
+    for got, twice, u in zip(out, again, mats):
+        assert torch.equal(got, twice)
+        _check(got, u)
+    u = _grad(1500, 1450, 9).bfloat16()
+    _check(ops.newton_schulz(u.cuda()), u)
+
+
+@gpu
 def test_newton_schulz_orthogonalises():
     """After enough steps of the classical cubic (1.5, -0.5, 0) the result is the orthogonal factor itself."""
     from boostmvsnerfs_amd import ops
