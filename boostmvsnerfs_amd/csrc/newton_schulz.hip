@@ -126,13 +126,31 @@ __device__ __forceinline__ void ns_write(void* p, long i, int dtype, float v) {
   else if (dtype == 1) static_cast<__bf16*>(p)[i] = (__bf16)v;
   else static_cast<_Float16*>(p)[i] = (_Float16)v;
 }
-// what the iteration starts from, before its norm is divided out; `fresh`: the momentum is moved first
-__device__ __forceinline__ float ns_start(const NsArgs& g, const NsItem& it, long i, bool fresh) {
-  const float v = ns_read(it.src, i, g.dtype);
-  if (!g.muon) return v;
-  float m = it.buf[i];
-  if (fresh) m = g.mu * m + g.nu * v, it.buf[i] = m;
-  return g.nesterov ? g.nu * v + g.mu * m : m;
+// N values of what the iteration starts from, before its norm is divided out; `fresh`: the momentum is moved first.  at(j): the
+// index of value j, or -1 for a zero.  (All loads before the first use: a branch or a conversion between them waits for each.)
+template <int DT, bool MUON, int N, typename F>
+__device__ __forceinline__ void ns_start(const NsArgs& g, const NsItem& it, bool fresh, F at, float* v) {
+  using T = std::conditional_t<DT == 0, float, std::conditional_t<DT == 1, __bf16, _Float16>>;
+  long i[N];
+  T raw[N];
+  float m[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) i[j] = at(j);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    raw[j] = static_cast<const T*>(it.src)[max(i[j], 0l)];
+    if (MUON) m[j] = it.buf[max(i[j], 0l)];
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    float x = (float)raw[j];
+    if (MUON) {
+      if (fresh) m[j] = g.mu * m[j] + g.nu * x;
+      if (fresh && i[j] >= 0) it.buf[i[j]] = m[j];
+      x = g.nesterov ? g.nu * x + g.mu * m[j] : m[j];
+    }
+    v[j] = i[j] >= 0 ? x : 0.f;
+  }
 }
 __device__ __forceinline__ void ns_result(const NsArgs& g, const NsItem& it, long i, float x) {
   ns_write(it.dst, i, g.dtype, g.muon ? ns_read(it.dst, i, g.dtype) * g.keep - it.scale * x : x);
@@ -177,6 +195,7 @@ __device__ __forceinline__ void ns_store_block(const float* t, int r0, int c0, _
 }
 
 // ---- the start: momentum and sum of squares; then scaled, split, both orientations --------------------------------------
+template <int DT, bool MUON>
 __global__ void __launch_bounds__(256) ns_norm_kernel(NsArgs g) {
   const int i = ns_find(g, blockIdx.x);
   const NsItem it = g.it[i];
@@ -185,11 +204,10 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(NsArgs g) {
   double s = 0.;
   for (int k = 0; k < kNsChunk / 256; k += 8) {
     float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    ns_start<DT, MUON, 8>(g, it, true, [&](int j) {
       const long at = base + (k + j) * 256 + threadIdx.x;
-      v[j] = at < numel ? ns_start(g, it, at, true) : 0.f;
-    }
+      return at < numel ? at : -1l;
+    }, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) s += (double)v[j] * (double)v[j];
   }
@@ -201,8 +219,9 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(NsArgs g) {
   if (threadIdx.x == 0) g.sq[(long)i * g.sqn + wg] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
 }
 
-template <int P>
+template <int DT, bool MUON>
 __global__ void __launch_bounds__(256) ns_split_kernel(NsArgs g) {
+  constexpr int P = DT == 1 ? 2 : 3;
   const int i = ns_find(g, blockIdx.x);
   const NsItem it = g.it[i];
   const NsShape s(it.rows, it.cols);
@@ -220,12 +239,18 @@ __global__ void __launch_bounds__(256) ns_split_kernel(NsArgs g) {
   __syncthreads();
   const double norm = sqrt((sh[0] + sh[1]) + (sh[2] + sh[3]));
   const float scale = (float)(1. / (norm > (double)g.eps || norm != norm ? norm : (double)g.eps));
-#pragma unroll 8
-  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-    const int hi = e >> 6, lo = e & 63;                  // the source's row and column inside the tile
-    const int r = (s.tall ? j0 : k0) + hi, c = (s.tall ? k0 : j0) + lo;
-    const float v = r < it.rows && c < it.cols ? ns_start(g, it, (long)r * it.cols + c, false) * scale : 0.f;
-    tile[s.tall ? lo * kNsPitch + hi : hi * kNsPitch + lo] = v;
+#pragma unroll
+  for (int k = 0; k < 16; k += 8) {
+    float v[8];
+    ns_start<DT, MUON, 8>(g, it, false, [&](int j) {
+      const int e = threadIdx.x + 256 * (k + j), r = (s.tall ? j0 : k0) + (e >> 6), c = (s.tall ? k0 : j0) + (e & 63);
+      return r < it.rows && c < it.cols ? (long)r * it.cols + c : -1l;
+    }, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int e = threadIdx.x + 256 * (k + j), hi = e >> 6, lo = e & 63;      // the source's row and column inside the tile
+      tile[s.tall ? lo * kNsPitch + hi : hi * kNsPitch + lo] = v[j] * scale;
+    }
   }
   __syncthreads();
   ns_store_block<P>(tile, k0, j0, p.x, s.np, p.xt, s.mp);
@@ -639,7 +664,8 @@ __device__ __forceinline__ void ns_triangle(int b, int& i, int& j) {
 // it.at of the matrices that have an XCD of their own: XCD << kNsXcd | slot
 constexpr int kNsXcd = 24;
 
-template <bool START>
+// (DT, MUON: the start's alone; the steps' kernel is one for all)
+template <bool START, int DT, bool MUON>
 __global__ void __launch_bounds__(512) ns_short_kernel(NsArgs g) {
   extern __shared__ __align__(16) float sm[];
   // (ns_place) workgroups go to the XCDs in turn: slot s of XCD x
@@ -658,17 +684,19 @@ __global__ void __launch_bounds__(512) ns_short_kernel(NsArgs g) {
   // columns of the tile as rows of m values, 16 bytes a lane, two columns a wave
   const int k4 = lane & 31, jw = wave * 2 + (lane >> 5);
   if (START) {
-    if (shape.tall) {
-#pragma unroll 8
-      for (int j = wave; j < s.T; j += 8)
-        for (int k = lane; k < s.mp; k += 64) xs[j * s.pitch + k] = j < nj && k < s.m ? ns_start(g, it, (long)(j0 + j) * it.cols + k, true) : 0.f;
-    } else {
-      const int sh = 31 - __clz(s.T);
-#pragma unroll 8
-      for (int e = threadIdx.x; e < s.mp << sh; e += 512) {
-        const int k = e >> sh, j = e & (s.T - 1);
-        xs[j * s.pitch + k] = j < nj && k < s.m ? ns_start(g, it, (long)k * it.cols + j0 + j, true) : 0.f;
-      }
+    // 8 values a thread at a time: of a column (tall: one wave a column) or of a row
+    const int sh = 31 - __clz(s.T), all = shape.tall ? s.T * 128 : s.mp << sh;
+    for (int e0 = threadIdx.x; e0 < all; e0 += 8 * 512) {
+      float v[8];
+      int to[8];
+      ns_start<DT, MUON, 8>(g, it, true, [&](int u) {
+        const int e = e0 + 512 * u, j = shape.tall ? e >> 7 : e & (s.T - 1), k = shape.tall ? e & 127 : e >> sh;
+        to[u] = e < all && k < s.mp ? j * s.pitch + k : -1;
+        return e < all && j < nj && k < s.m ? (shape.tall ? (long)(j0 + j) * it.cols + k : (long)k * it.cols + j0 + j) : -1l;
+      }, v);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (to[u] >= 0) xs[to[u]] = v[u];
     }
     __syncthreads();
   } else {
@@ -995,6 +1023,18 @@ static void ns_fill(NsArgs& g, const NsLists& l, const int* idx, int n) {
   }
 }
 
+// f with the call's type and kind as constants
+template <typename F>
+static void ns_typed(const NsArgs& g, F f) {
+  auto kind = [&](auto dt) {
+    if (g.muon) f(dt, std::true_type{});
+    else f(dt, std::false_type{});
+  };
+  if (g.dtype == 0) kind(std::integral_constant<int, 0>{});
+  else if (g.dtype == 1) kind(std::integral_constant<int, 1>{});
+  else kind(std::integral_constant<int, 2>{});
+}
+
 // Which XCD computes which matrix; returns the workgroups of a launch.  Every workgroup of a matrix reads the shares of all others
 // of the launch before: on one XCD they are in its L2 (128 x 128 61.7 -> 55.2 us).  The matrices go to the XCDs by their work, the
 // largest first, each to the one that has least; one of more workgroups than an XCD has compute units is spread over all.
@@ -1035,10 +1075,10 @@ static void ns_run_short(NsArgs& g, int least, int steps, char* ws, hipStream_t 
     g.it[i].ws = off, off += s.bytes(), lds = std::max(lds, s.lds());
   }
   g.flip = 1;                                             // (the first shares go to where step 0 reads)
-  hipLaunchKernelGGL(ns_short_kernel<true>, grid, dim3(512), lds, st, g);
+  ns_typed(g, [&](auto dt, auto muon) { hipLaunchKernelGGL((ns_short_kernel<true, decltype(dt)::value, decltype(muon)::value>), grid, dim3(512), lds, st, g); });
   for (int k = 0; k < steps; ++k) {
     g.first = k == 0, g.last = k + 1 == steps, g.flip = k & 1;
-    hipLaunchKernelGGL(ns_short_kernel<false>, grid, dim3(512), lds, st, g);
+    hipLaunchKernelGGL((ns_short_kernel<false, 0, false>), grid, dim3(512), lds, st, g);
   }
 }
 
@@ -1052,9 +1092,9 @@ static void ns_run_long(NsArgs& g, const NsRoom& room, int steps, char* ws, hipS
     it.ws = off, it.at = (int)chunks;
     off += ns_bytes(NsShape(it.rows, it.cols), P), chunks += ns_chunks(it.rows, it.cols);
   }
-  hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)chunks), dim3(256), 0, st, g);
+  ns_typed(g, [&](auto dt, auto muon) { hipLaunchKernelGGL((ns_norm_kernel<decltype(dt)::value, decltype(muon)::value>), dim3((unsigned)chunks), dim3(256), 0, st, g); });
   for (int i = 0; i < g.count; ++i) g.it[i].at = (int)blocks, blocks += NsShape(g.it[i].rows, g.it[i].cols).big() / (64 * 64);
-  hipLaunchKernelGGL(ns_split_kernel<P>, dim3((unsigned)blocks), dim3(256), 0, st, g);
+  ns_typed(g, [&](auto dt, auto muon) { hipLaunchKernelGGL((ns_split_kernel<decltype(dt)::value, decltype(muon)::value>), dim3((unsigned)blocks), dim3(256), 0, st, g); });
   for (int k = 0; k < steps; ++k) {
     g.last = k + 1 == steps, g.flip = k & 1;
     ns_product<P, kNsGram>(g, st);
@@ -1071,8 +1111,13 @@ static bool ns_lds() {
   if (hipGetDevice(&dev) != hipSuccess) return false;
   const unsigned long bit = dev < 64 ? 1ul << dev : 0;
   if (ready.load(std::memory_order_acquire) & bit) return true;
-  const std::pair<const void*, int> f[] = {{(const void*)ns_short_kernel<true>, kLds},
-                                           {(const void*)ns_short_kernel<false>, kLds},
+  const std::pair<const void*, int> f[] = {{(const void*)ns_short_kernel<true, 0, false>, kLds},
+                                           {(const void*)ns_short_kernel<true, 1, false>, kLds},
+                                           {(const void*)ns_short_kernel<true, 2, false>, kLds},
+                                           {(const void*)ns_short_kernel<true, 0, true>, kLds},
+                                           {(const void*)ns_short_kernel<true, 1, true>, kLds},
+                                           {(const void*)ns_short_kernel<true, 2, true>, kLds},
+                                           {(const void*)ns_short_kernel<false, 0, false>, kLds},
                                            {(const void*)ns_block_kernel<3, kNsGram, 2>, kNsBlockLds<3, 2>},
                                            {(const void*)ns_block_kernel<3, kNsPoly, 2>, kNsBlockLds<3, 2>},
                                            {(const void*)ns_block_kernel<3, kNsApply, 2>, kNsBlockLds<3, 2>},
