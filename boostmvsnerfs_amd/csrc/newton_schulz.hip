@@ -116,16 +116,6 @@ __device__ __forceinline__ int ns_find(const NsArgs& g, int at) {
   return __popcll(__ballot(lane < g.count && g.it[min(lane, kNsList - 1)].at <= at)) - 1;
 }
 
-__device__ __forceinline__ float ns_read(const void* p, long i, int dtype) {
-  if (dtype == 0) return static_cast<const float*>(p)[i];
-  if (dtype == 1) return (float)static_cast<const __bf16*>(p)[i];
-  return (float)static_cast<const _Float16*>(p)[i];
-}
-__device__ __forceinline__ void ns_write(void* p, long i, int dtype, float v) {
-  if (dtype == 0) static_cast<float*>(p)[i] = v;
-  else if (dtype == 1) static_cast<__bf16*>(p)[i] = (__bf16)v;
-  else static_cast<_Float16*>(p)[i] = (_Float16)v;
-}
 // N values of what the iteration starts from, before its norm is divided out; `fresh`: the momentum is moved first.  at(j): the
 // index of value j, or -1 for a zero.  (All loads before the first use: a branch or a conversion between them waits for each.)
 template <int DT, bool MUON, int N, typename F>
@@ -152,8 +142,25 @@ __device__ __forceinline__ void ns_start(const NsArgs& g, const NsItem& it, bool
     v[j] = i[j] >= 0 ? x : 0.f;
   }
 }
-__device__ __forceinline__ void ns_result(const NsArgs& g, const NsItem& it, long i, float x) {
-  ns_write(it.dst, i, g.dtype, g.muon ? ns_read(it.dst, i, g.dtype) * g.keep - it.scale * x : x);
+// N results, value j of index at(j) (-1: none): the iterate itself, or the weight that it steps, rounded once
+template <int N, typename F>
+__device__ __forceinline__ void ns_results(const NsArgs& g, const NsItem& it, F at, const float* x) {
+  long i[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) i[j] = at(j);
+  auto run = [&](auto* dst) {
+    std::remove_pointer_t<decltype(dst)> w[N];
+    if (g.muon) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) w[j] = dst[max(i[j], 0l)];
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i[j] >= 0) dst[i[j]] = (std::remove_pointer_t<decltype(dst)>)(g.muon ? (float)w[j] * g.keep - it.scale * x[j] : x[j]);
+  };
+  if (g.dtype == 0) run(static_cast<float*>(it.dst));
+  else if (g.dtype == 1) run(static_cast<__bf16*>(it.dst));
+  else run(static_cast<_Float16*>(it.dst));
 }
 
 // x = p[0] + p[1] + p[2], exactly: every piece is the nearest bf16 to what the pieces before it leave (to nearest, not
@@ -314,12 +321,18 @@ __device__ __forceinline__ void ns_finish(const NsArgs& g, const NsItem& it, con
     __syncthreads();
   }
   if (STAGE == kNsApply && g.last) {
-#pragma unroll 4
-    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-      const int hi_ = e >> 6, lo_ = e & 63;               // row and column of the source inside the block
-      const int r = (s.tall ? col0 : row0) + hi_, c = (s.tall ? row0 : col0) + lo_;
-      if (r < it.rows && c < it.cols)
-        ns_result(g, it, (long)r * it.cols + c, tile[s.tall ? lo_ * kNsPitch + hi_ : hi_ * kNsPitch + lo_]);
+#pragma unroll
+    for (int k = 0; k < 16; k += 8) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int e = threadIdx.x + 256 * (k + j), hi = e >> 6, lo = e & 63;      // row and column of the source inside the block
+        v[j] = tile[s.tall ? lo * kNsPitch + hi : hi * kNsPitch + lo];
+      }
+      ns_results<8>(g, it, [&](int j) {
+        const int e = threadIdx.x + 256 * (k + j), r = (s.tall ? col0 : row0) + (e >> 6), c = (s.tall ? row0 : col0) + (e & 63);
+        return r < it.rows && c < it.cols ? (long)r * it.cols + c : -1l;
+      }, v);
     }
     return;
   }
@@ -803,15 +816,18 @@ __global__ void __launch_bounds__(512) ns_short_kernel(NsArgs g) {
     if (tiles <= 8) step(std::integral_constant<int, 1>{});
     else step(std::integral_constant<int, 2>{});
     if (g.last) {
-      if (shape.tall) {
-        for (int j = wave; j < nj; j += 8)
-          for (int k = lane; k < s.m; k += 64) ns_result(g, it, (long)(j0 + j) * it.cols + k, xs[j * s.pitch + k]);
-      } else {
-        const int sh = 31 - __clz(s.T);
-        for (int e = threadIdx.x; e < s.m << sh; e += 512) {
-          const int k = e >> sh, j = e & (s.T - 1);
-          if (j < nj) ns_result(g, it, (long)k * it.cols + j0 + j, xs[j * s.pitch + k]);
+      const int sh = 31 - __clz(s.T), all = shape.tall ? nj * 128 : s.m << sh;
+      for (int e0 = threadIdx.x; e0 < all; e0 += 8 * 512) {
+        float v[8];
+        long at[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int e = min(e0 + 512 * u, all - 1), j = shape.tall ? e >> 7 : e & (s.T - 1), k = shape.tall ? e & 127 : e >> sh;
+          const bool on = e0 + 512 * u < all && j < nj && k < s.m;
+          at[u] = on ? (shape.tall ? (long)(j0 + j) * it.cols + k : (long)k * it.cols + j0 + j) : -1l;
+          v[u] = on ? xs[j * s.pitch + k] : 0.f;
         }
+        ns_results<8>(g, it, [&](int u) { return at[u]; }, v);
       }
       return;
     }
