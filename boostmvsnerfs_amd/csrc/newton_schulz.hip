@@ -1014,10 +1014,10 @@ static void ns_product(NsArgs& g, hipStream_t st) {
     const long end = i + 1 < g.count ? g.it[i + 1].at : tiles, begin = std::max<long>(g.it[i].at, g.full);
     if (end > begin) units += (end - begin) * ns_stages<P>(s, STAGE);
   }
-  // A run for every compute unit (two for each hide more latency, but a partial tile is 64 KB through memory: 1024 x 1024 bf16
-  // 366 -> 308 us, 1024 x 4096 492 -> 450), but not too short for the same reason: of at least 8 stages, or 4 where even those are
-  // few (256 x 256 185 us, with 8 212; 512 x 2048 fp32 with 4 365 us, with 8 300).  Panels are multiples of 8 stages long.
-  g.run = (int)std::max<long>((units + kNsUnits - 1) / kNsUnits, units <= 2 * kNsUnits ? 4 : 8);
+  // A run for every compute unit (two for each hide more latency, but a partial tile is 64 KB through memory: 1024 x 4096 bf16 432 us,
+  // one 409; 512 x 4096 fp32 331, 319), but of at least 256 k-values for the same reason: 160 x 8192 fp32 283 us, with 128 322 and
+  // with 384 295; bf16 242, with 128 290 and with 384 243; 256 x 4096 bf16 175, 198 and 190.  Panels are multiples of 128 long.
+  g.run = (int)std::max<long>((units + kNsUnits - 1) / kNsUnits, 256 / (kNsK * kNsBlocks<P>));
   hipLaunchKernelGGL((ns_product_kernel<P, STAGE>), dim3((unsigned)(g.full + (units + g.run - 1) / g.run)), dim3(256), 0, st, g);
   hipLaunchKernelGGL((ns_join_kernel<P, STAGE>), dim3((unsigned)(4 * tiles)), dim3(256), 0, st, g);
 }
