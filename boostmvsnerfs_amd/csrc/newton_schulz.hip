@@ -647,11 +647,13 @@ __global__ void __launch_bounds__(256, 1) ns_block_kernel(NsArgs g) {
 // with 16 columns and 75 with 32, 128 x 512 103 and 89; 64 x 864 takes 51 us with 32 and 56 with 64, 64 x 1728 71 and 68.  A list
 // that has more workgroups than fit the card at once gets more columns each: cheaper than a second round.  (64 columns of more
 // than 64 rows would be four blocks a wave: 10 % slower at 128 x 2048 than 32.)
-// Long sides: the shares that everybody adds up grow with n^2.  128 x 4096 286 us (through the large matrices' way 295),
-// 128 x 8192 515 (438); 64 x 8192 130 (437).
+// Long sides: the shares that everybody adds up grow with n^2.  Above 64 rows up to 2048 (128 x 2048 181 us, through the large
+// matrices' way 187; 128 x 3000 229 and 174), bf16 up to 1024 (128 x 1024 123 and 118, 96 x 1024 106 and 117; 128 x 2048 181 and
+// 144); below them 64 x 8192 takes 134 us (226), 64 x 16384 218 (320, bf16 287).
 // A step's time: 128 x 128 10 us, 64 x 1728 12.5 us; the network of MVSNeRF, 29 matrices, 13.5 us.  4 us of it is one launch
 // behind another; the rest is a chain of shares, two products and the next share, of which the products are a quarter.
-constexpr int kNsShort = 128, kNsShortLong = 16384;      // short side, and long side (a quarter of it above 64 rows), up to which this way is taken
+constexpr int kNsShort = 128;                            // short side, and long side (below), up to which this way is taken
+__host__ __device__ __forceinline__ int ns_short_long(int m, int dtype) { return m <= 64 ? 16384 : dtype == 1 ? 1024 : 2048; }
 __host__ __device__ __forceinline__ int ns_columns(int m, int n, int least) {
   const int t = n <= 288 ? 16 : n <= 1152 ? 32 : 64, u = t > least ? t : least;
   return m > 64 && u > 32 ? 32 : u;
@@ -894,9 +896,9 @@ static int ns_chunks(int rows, int cols) { return (int)(((long)rows * cols + kNs
 
 // limit: of the short side, what BMV_NS_SHORT is at the call (read once: the workspace's layout goes by it)
 static int ns_limit() { return std::min(kNsShort, tuning("BMV_NS_SHORT", kNsShort)); }
-static bool ns_is_short(int rows, int cols, int limit) {
+static bool ns_is_short(int rows, int cols, int dtype, int limit) {
   const int m = std::min(rows, cols);
-  return m <= limit && std::max(rows, cols) <= (m > 64 ? kNsShortLong / 4 : kNsShortLong);
+  return m <= limit && std::max(rows, cols) <= ns_short_long(m, dtype);
 }
 // Workspace of a part of the list (indices): the short ones' X and shares, or the others' pieces, then the norm's partial
 // sums, then partial tiles
@@ -933,14 +935,14 @@ struct NsRoom {
   long bytes() const { return pieces + (long)kNsList * sqn * sizeof(double) + (tiles + kNsSlots) * (kNsTile * kNsTile * 4l); }
 };
 // the list's indices: the short ones, then the others
-static std::vector<int> ns_order(int count, const int* rows, const int* cols, int limit, int& shorts) {
+static std::vector<int> ns_order(int count, const int* rows, const int* cols, int dtype, int limit, int& shorts) {
   std::vector<int> v;
   v.reserve(count);
   for (int i = 0; i < count; ++i)
-    if (ns_is_short(rows[i], cols[i], limit)) v.push_back(i);
+    if (ns_is_short(rows[i], cols[i], dtype, limit)) v.push_back(i);
   shorts = (int)v.size();
   for (int i = 0; i < count; ++i)
-    if (!ns_is_short(rows[i], cols[i], limit)) v.push_back(i);
+    if (!ns_is_short(rows[i], cols[i], dtype, limit)) v.push_back(i);
   return v;
 }
 // a list is done in parts of kNsList, which share the workspace
@@ -1150,7 +1152,7 @@ static bool ns_lds() {
 
 static const char* ns_run(NsArgs g, int count, const NsLists& l, int dtype, int steps, void* workspace, long bytes, hipStream_t st) {
   int shorts;
-  const std::vector<int> v = ns_order(count, l.rows, l.cols, ns_limit(), shorts);
+  const std::vector<int> v = ns_order(count, l.rows, l.cols, dtype, ns_limit(), shorts);
   if (ns_workspace(count, l.rows, l.cols, dtype, v, shorts) > bytes) return "the workspace is too small";
   if (!ns_lds()) return "LDS refused";
   char* ws = static_cast<char*>(workspace);
@@ -1180,7 +1182,7 @@ long bmv_newton_schulz_workspace(int count, const int* rows, const int* cols, in
   BMV_REQUIRE(dtype >= 0 && dtype <= 2, "bmv_newton_schulz_workspace: unknown type %d", dtype);
   return ns_no_throw([&]() -> long {
     int shorts;
-    const std::vector<int> v = ns_order(count, rows, cols, ns_limit(), shorts);
+    const std::vector<int> v = ns_order(count, rows, cols, dtype, ns_limit(), shorts);
     return ns_workspace(count, rows, cols, dtype, v, shorts);
   });
 }

@@ -64,7 +64,7 @@ def _check(got, u, steps=5, coeffs=COEFFS, eps=1e-7):
 
 
 SHAPES = [(1, 1), (1, 7), (9, 1), (2, 2), (3, 64), (8, 27), (16, 200), (35, 4), (64, 24), (33, 32), (63, 65), (64, 64), (64, 1728),
-          (65, 40), (80, 100), (127, 129), (128, 63), (8, 4000), (128, 4096), (128, 4097), (33, 1000), (5, 16384), (17, 16385), (60, 1153), (112, 288), (112, 289), (96, 1200), (128, 128), (128, 515), (129, 129), (130, 1000), (333, 257), (256, 384), (700, 90)]
+          (65, 40), (80, 100), (127, 129), (128, 63), (8, 4000), (128, 1024), (1025, 100), (128, 2048), (97, 2049), (128, 4097), (33, 1000), (5, 16384), (17, 16385), (60, 1153), (112, 288), (112, 289), (96, 1200), (128, 128), (128, 515), (129, 129), (130, 1000), (333, 257), (256, 384), (700, 90)]
 
 
 @pytest.fixture(params=["short", "blocks", "tiles"])
