@@ -749,6 +749,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_pl_bwd_apply_kernel(GnArgs a) {
 
 // ---- host ------------------------------------------------------------------------------------------------------------
 constexpr int kGnMaxJoin = 1024;      // double2 that a workgroup of the apply launch joins; above, one more launch does
+constexpr int kGnFew = 384;           // workgroups, fewer of which cost more than that launch
 
 struct GnPlan {
   GnArgs a;
@@ -811,7 +812,8 @@ static GnPlan gn_plan(int N, int C, long S, int G, int dtype, int last, bool bac
     // so few that their pieces need no launch of their own (1 x 256 x 128 x 128 bf16 forward 21 -> 16.4 us).
     const long rpi = kGnThreads / wv, touched = std::min<long>((a.width + a.cg - 1) / a.cg + 1, G);
     const long target = !backward && (long)N * a.slabs * S >= 7 * rpi * 1024 ? 1024 : 512;
-    const long wgs = std::max(1l, std::min(target / ((long)N * a.slabs), kGnMaxJoin / (touched * a.slab_pieces)));
+    const long few = kGnMaxJoin / (touched * a.slab_pieces), most = target / ((long)N * a.slabs);
+    const long wgs = std::max(1l, few * N * a.slabs >= kGnFew ? std::min(most, few) : most);
     a.per = std::max(2 * rpi, ((S + wgs - 1) / wgs + rpi - 1) / rpi * rpi);
     const long chunks = (S + a.per - 1) / a.per;
     a.chunks = (int)chunks, a.pieces = a.chunks * a.slab_pieces, a.npc = a.chunks;
