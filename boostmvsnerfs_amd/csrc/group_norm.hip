@@ -749,7 +749,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_pl_bwd_apply_kernel(GnArgs a) {
 
 // ---- host ------------------------------------------------------------------------------------------------------------
 constexpr int kGnMaxJoin = 1024;      // double2 that a workgroup of the apply launch joins; above, one more launch does
-constexpr int kGnFew = 384;           // workgroups, fewer of which cost more than that launch
+constexpr int kGnFew = 384;           // workgroups, fewer of which cost more than that launch (200416 x 19 fp16, 19 groups: 80 us with 53, 33)
 
 struct GnPlan {
   GnArgs a;
