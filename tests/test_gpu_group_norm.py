@@ -130,7 +130,8 @@ def test_group_norm_matches_the_formula(shape, dtype, layout):
 @pytest.mark.parametrize("layout", ["last", "planar"])
 def test_group_norm_many_chunks_and_the_finishing_launch(layout):
     """Maps whose partial sums come from hundreds of workgroups (with the launch that joins them in front of the second pass)."""
-    for N, C, sp, G, dtype in ((1, 8, (640, 517), 1, torch.float32), (2, 64, (131, 128), 64, torch.bfloat16), (1, 256, (96, 97), 1, torch.float32)):
+    for N, C, sp, G, dtype in ((1, 8, (640, 517), 1, torch.float32), (2, 64, (131, 128), 64, torch.bfloat16), (1, 256, (96, 97), 1, torch.float32), (1, 19, (200, 150), 19, torch.float16),
+                               (3, 30, (131, 97), 30, torch.float32)):
         x, dy, w, b = _make(N, C, sp, dtype, layout, seed=3)
         _check(x, dy, G, w, b, True, layout)
 
