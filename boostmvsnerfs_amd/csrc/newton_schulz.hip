@@ -10,8 +10,7 @@
 // three bf16 pieces (hi + mid + lo: its 24 significand bits exactly) and the six products that are not below 2^-25, sums in
 // fp32: 2.5 PFLOP/s / 6 against the 0.157 of the fp32 matrix instructions.  |U|_F is a 64-bit sum.
 //
-// bf16 matrices (half a step of a result: 2^-9) get two pieces (2^-17) and three products, half the work: what the steps make
-// of that error is a few 1e-4 of the result at most, beside 1.7e-3 that its one rounding costs.  fp16 (2^-12) keeps three.
+// All types: a bf16 or fp16 matrix' result is the fp32 result of the same values, rounded once.
 //
 // Layout.  Every operand is kept as its pieces from the moment it is computed (one split per value, not one per use), in the
 // orientation in which its k axis is contiguous, so all three products are L R^T: A from X (k = n), A A from the symmetric A
@@ -48,6 +47,7 @@ using nsf16 = __attribute__((ext_vector_type(16))) float;
 
 constexpr int kNsList = 40;      // matrices per launch (the table travels in the kernel arguments)
 constexpr int kNsTile = 128;     // output tile of a workgroup; matrices are padded to it with zeros
+constexpr int kNsP = 3;          // bf16 pieces of an operand
 constexpr int kNsK = 16;         // k-values of a stage
 constexpr int kNsCell = 2048;    // elements of a piece of a block: 128 rows of 16 k-values
 constexpr int kNsChunk = 8192;   // elements of a workgroup of the norm
@@ -89,23 +89,21 @@ struct NsShape {
   __host__ __device__ int nt() const { return np / kNsTile; }
   __host__ __device__ long triangle() const { return (long)mt() * (mt() + 1) / 2; }
 };
-// the operands of a matrix, P pieces each
-template <int P>
+// the operands of a matrix, kNsP pieces each
 struct NsPlanes {
   __bf16 *x, *xt, *xt1, *a, *q;      // xt, xt1: X^T before and after a step, in turn
   __device__ NsPlanes(char* ws, const NsShape& s) {
     x = reinterpret_cast<__bf16*>(ws);
-    xt = x + P * s.big(), xt1 = xt + P * s.big(), a = xt1 + P * s.big(), q = a + P * s.sym();
+    xt = x + kNsP * s.big(), xt1 = xt + kNsP * s.big(), a = xt1 + kNsP * s.big(), q = a + kNsP * s.sym();
   }
 };
-static long ns_bytes(const NsShape& s, int pieces) { return (3 * s.big() + 2 * s.sym()) * 2 * pieces; }
+static long ns_bytes(const NsShape& s) { return (3 * s.big() + 2 * s.sym()) * 2 * kNsP; }
 
 // the 8 k-values k ... k + 7 (k % 8 == 0) of row r, piece 0, of an operand with K k-values; piece q is kNsCell * q behind.
 // The two 16-byte cells of a row in a block are in turn swapped every 8 rows: the 16 lanes of a phase of ds_read_b128 (rows at
 // one k) then touch all 64 banks once.
-template <int P>
 __device__ __forceinline__ long ns_cell(int r, int k, int K) {
-  return ((long)(r >> 7) * (K / kNsK) + k / kNsK) * (P * kNsCell) + (r & 127) * kNsK + (((k >> 3) ^ (r >> 3)) & 1) * 8;
+  return ((long)(r >> 7) * (K / kNsK) + k / kNsK) * (kNsP * kNsCell) + (r & 127) * kNsK + (((k >> 3) ^ (r >> 3)) & 1) * 8;
 }
 
 // the matrix that holds `at`: the last whose first is not behind it (one load a lane instead of a chain of them)
@@ -117,7 +115,8 @@ __device__ __forceinline__ int ns_find(const NsArgs& g, int at) {
 }
 
 // N values of what the iteration starts from, before its norm is divided out; `fresh`: the momentum is moved first.  at(j): the
-// index of value j, or -1 for a zero.  (All loads before the first use: a branch or a conversion between them waits for each.)
+// index of value j, or -1 for a zero.  (All loads before the first use: a branch or a conversion between them waits for each.
+// Fused products are written out: the same roundings for all types.)
 template <int DT, bool MUON, int N, typename F>
 __device__ __forceinline__ void ns_start(const NsArgs& g, const NsItem& it, bool fresh, F at, float* v) {
   using T = std::conditional_t<DT == 0, float, std::conditional_t<DT == 1, __bf16, _Float16>>;
@@ -135,14 +134,15 @@ __device__ __forceinline__ void ns_start(const NsArgs& g, const NsItem& it, bool
   for (int j = 0; j < N; ++j) {
     float x = (float)raw[j];
     if (MUON) {
-      if (fresh) m[j] = g.mu * m[j] + g.nu * x;
+      if (fresh) m[j] = fmaf(g.mu, m[j], g.nu * x);
       if (fresh && i[j] >= 0) it.buf[i[j]] = m[j];
-      x = g.nesterov ? g.nu * x + g.mu * m[j] : m[j];
+      x = g.nesterov ? fmaf(g.mu, m[j], g.nu * x) : m[j];
     }
     v[j] = i[j] >= 0 ? x : 0.f;
   }
 }
-// N results, value j of index at(j) (-1: none): the iterate itself, or the weight that it steps, rounded once
+// N results, value j of index at(j) (-1: none): the iterate itself, or the weight that it steps, rounded once (the fused product is
+// written out: one order of the roundings for all types)
 template <int N, typename F>
 __device__ __forceinline__ void ns_results(const NsArgs& g, const NsItem& it, F at, const float* x) {
   long i[N];
@@ -156,7 +156,7 @@ __device__ __forceinline__ void ns_results(const NsArgs& g, const NsItem& it, F 
     }
 #pragma unroll
     for (int j = 0; j < N; ++j)
-      if (i[j] >= 0) dst[i[j]] = (std::remove_pointer_t<decltype(dst)>)(g.muon ? (float)w[j] * g.keep - it.scale * x[j] : x[j]);
+      if (i[j] >= 0) dst[i[j]] = (std::remove_pointer_t<decltype(dst)>)(g.muon ? fmaf(-it.scale, x[j], (float)w[j] * g.keep) : x[j]);
   };
   if (g.dtype == 0) run(static_cast<float*>(it.dst));
   else if (g.dtype == 1) run(static_cast<__bf16*>(it.dst));
@@ -164,25 +164,23 @@ __device__ __forceinline__ void ns_results(const NsArgs& g, const NsItem& it, F 
 }
 
 // x = p[0] + p[1] + p[2], exactly: every piece is the nearest bf16 to what the pieces before it leave (to nearest, not
-// truncated: what the dropped products of the pieces amount to is then below 2^-25 and of either sign, not 2^-21 of one);
-// two pieces leave 2^-17 out.  Eight consecutive values as P 16-byte stores.
-template <int P>
+// truncated: what the dropped products of the pieces amount to is then below 2^-25 and of either sign, not 2^-21 of one).
+// Eight consecutive values as kNsP 16-byte stores.
 __device__ __forceinline__ void ns_store8(__bf16* p, const float* v) {
-  nsb8 o[P];
+  nsb8 o[kNsP];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     float r = v[j];
 #pragma unroll
-    for (int q = 0; q < P; ++q) o[q][j] = (__bf16)r, r -= (float)o[q][j];
+    for (int q = 0; q < kNsP; ++q) o[q][j] = (__bf16)r, r -= (float)o[q][j];
   }
 #pragma unroll
-  for (int q = 0; q < P; ++q) *reinterpret_cast<nsb8*>(p + q * kNsCell) = o[q];
+  for (int q = 0; q < kNsP; ++q) *reinterpret_cast<nsb8*>(p + q * kNsCell) = o[q];
 }
 
 // A 64 x 64 block of values in LDS, rows r0 ..., columns c0 ... of a matrix, as cells of the operand whose k axis is the
 // columns (out, K = its columns) and of its transpose (outt, Kt); either may be null.
 constexpr int kNsPitch = 65;
-template <int P>
 __device__ __forceinline__ void ns_store_block(const float* t, int r0, int c0, __bf16* out, int K, __bf16* outt, int Kt) {
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -191,12 +189,12 @@ __device__ __forceinline__ void ns_store_block(const float* t, int r0, int c0, _
     if (out) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = t[line * kNsPitch + k + j];
-      ns_store8<P>(out + ns_cell<P>(r0 + line, c0 + k, K), v);
+      ns_store8(out + ns_cell(r0 + line, c0 + k, K), v);
     }
     if (outt) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = t[(k + j) * kNsPitch + line];
-      ns_store8<P>(outt + ns_cell<P>(c0 + line, r0 + k, Kt), v);
+      ns_store8(outt + ns_cell(c0 + line, r0 + k, Kt), v);
     }
   }
 }
@@ -228,11 +226,10 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(NsArgs g) {
 
 template <int DT, bool MUON>
 __global__ void __launch_bounds__(256) ns_split_kernel(NsArgs g) {
-  constexpr int P = DT == 1 ? 2 : 3;
   const int i = ns_find(g, blockIdx.x);
   const NsItem it = g.it[i];
   const NsShape s(it.rows, it.cols);
-  const NsPlanes<P> p(g.ws + it.ws, s);
+  const NsPlanes p(g.ws + it.ws, s);
   const int wg = blockIdx.x - it.at, nt = s.np / 64;
   const int k0 = wg / nt * 64, j0 = wg % nt * 64;       // rows and columns of X
   __shared__ float tile[64 * kNsPitch];                  // [row of X][column of X]
@@ -260,7 +257,7 @@ __global__ void __launch_bounds__(256) ns_split_kernel(NsArgs g) {
     }
   }
   __syncthreads();
-  ns_store_block<P>(tile, k0, j0, p.x, s.np, p.xt, s.mp);
+  ns_store_block(tile, k0, j0, p.x, s.np, p.xt, s.mp);
 }
 
 // ---- the products --------------------------------------------------------------------------------------------------------
@@ -289,25 +286,21 @@ __device__ __forceinline__ void ns_tile(int t, int mt, int nt, bool symmetric, i
   i = 8 * sr + col + t, j = 8 * sr + col;
 }
 __device__ __forceinline__ int ns_tiles(const NsShape& s, int stage) { return stage == kNsApply ? s.mt() * s.nt() : (int)s.triangle(); }
-// blocks of 16 k-values of a stage: two where a block has only 12 matrix instructions for a barrier (two pieces)
-template <int P>
-constexpr int kNsBlocks = P == 2 ? 2 : 1;
-template <int P>
-__host__ __device__ __forceinline__ int ns_stages(const NsShape& s, int stage) { return (stage == kNsGram ? s.np : s.mp) / (kNsK * kNsBlocks<P>); }
+__host__ __device__ __forceinline__ int ns_stages(const NsShape& s, int stage) { return (stage == kNsGram ? s.np : s.mp) / kNsK; }
 
 // A finished 64 x 64 block of a product in LDS, by its workgroup: the polynomial (kNsPoly), then both orientations as pieces, or
 // the result
-template <int P, int STAGE>
-__device__ __forceinline__ void ns_finish(const NsArgs& g, const NsItem& it, const NsShape& s, const NsPlanes<P>& p, int row0, int col0,
+template <int STAGE>
+__device__ __forceinline__ void ns_finish(const NsArgs& g, const NsItem& it, const NsShape& s, const NsPlanes& p, int row0, int col0,
                                           bool diagonal, float* tile) {
   if (STAGE == kNsPoly) {                                 // a I + b A + c A A, in place
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int k = threadIdx.x + 256 * e, r = k >> 1 & 63, c = (k >> 7) * 16 + (k & 1) * 8;
-      const __bf16* ap = p.a + ns_cell<P>(row0 + r, col0 + c, s.mp);
+      const __bf16* ap = p.a + ns_cell(row0 + r, col0 + c, s.mp);
       float av[8] = {};
 #pragma unroll
-      for (int q = P - 1; q >= 0; --q) {
+      for (int q = kNsP - 1; q >= 0; --q) {
         const nsb8 piece = *reinterpret_cast<const nsb8*>(ap + q * kNsCell);
 #pragma unroll
         for (int j = 0; j < 8; ++j) av[j] += (float)piece[j];
@@ -337,18 +330,18 @@ __device__ __forceinline__ void ns_finish(const NsArgs& g, const NsItem& it, con
     return;
   }
   __bf16* out = STAGE == kNsGram ? p.a : STAGE == kNsPoly ? p.q : p.x;
-  if (STAGE == kNsApply) ns_store_block<P>(tile, row0, col0, out, s.np, g.flip ? p.xt : p.xt1, s.mp);
-  else ns_store_block<P>(tile, row0, col0, out, s.mp, diagonal ? nullptr : out, s.mp);
+  if (STAGE == kNsApply) ns_store_block(tile, row0, col0, out, s.np, g.flip ? p.xt : p.xt1, s.mp);
+  else ns_store_block(tile, row0, col0, out, s.mp, diagonal ? nullptr : out, s.mp);
 }
 
 // A workgroup = 128 x 128 of L R^T, four waves of 64 x 64 (2 x 2 accumulators of v_mfma_f32_32x32x16_bf16, twice: hi hi goes to
 // accumulators of its own, because the other products are 2^-8 of it and adding them into the large sums would round those
 // once more for each).  Three stages of 16 k-values in LDS: one being multiplied, two on their way.  The finished tile leaves
 // in the order of the accumulators, 16 bytes a lane; the joining launch knows that order.
-template <int P, int STAGE>
+template <int STAGE>
 __global__ void __launch_bounds__(256, 2) ns_product_kernel(NsArgs g) {
-  constexpr int kB = kNsBlocks<P>, kBufs = kB == 1 ? 3 : 2;
-  constexpr int kHalf = kB * P * kNsCell;                 // elements of an operand's stage
+  constexpr int kBufs = 3;
+  constexpr int kHalf = kNsP * kNsCell;                   // elements of an operand's stage
   constexpr int kStage = 2 * kHalf;                       // L's, then R's
   constexpr int kLoads = kStage * 2 / 1024 / 4;           // 1 KB DMAs of a wave for a stage
   __shared__ __align__(16) __bf16 lds[kBufs * kStage];
@@ -361,7 +354,7 @@ __global__ void __launch_bounds__(256, 2) ns_product_kernel(NsArgs g) {
   while (left > 0) {
     const NsItem it = g.it[i];
     const NsShape s(it.rows, it.cols);
-    const int stages = ns_stages<P>(s, STAGE), tiles = ns_tiles(s, STAGE);
+    const int stages = ns_stages(s, STAGE), tiles = ns_tiles(s, STAGE);
     if (!whole) {                                         // go to the tile that holds the next unit
       const long jump = min(skip / stages, (long)(it.at + tiles - t));
       t += (int)jump, skip -= jump * stages;
@@ -374,7 +367,7 @@ __global__ void __launch_bounds__(256, 2) ns_product_kernel(NsArgs g) {
     skip = 0, left -= whole ? left : count;
     int ti, tj;
     ns_tile(t - it.at, s.mt(), s.nt(), STAGE != kNsApply, ti, tj);
-    const NsPlanes<P> p(g.ws + it.ws, s);
+    const NsPlanes p(g.ws + it.ws, s);
     const __bf16* L = STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : p.q;
     const __bf16* R = STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : (g.flip ? p.xt1 : p.xt);
     L += ((long)ti * stages + first) * kHalf, R += ((long)tj * stages + first) * kHalf;
@@ -389,37 +382,34 @@ __global__ void __launch_bounds__(256, 2) ns_product_kernel(NsArgs g) {
       }
     };
     const int lr = (wave >> 1) * 64 + (lane & 31), rr = (wave & 1) * 64 + (lane & 31), oct = lane >> 5;
-    auto read = [&](int k, int b, int operand, int q, int row) {
-      return *reinterpret_cast<const nsb8*>(lds + k % kBufs * kStage + operand * kHalf + (b * P + q) * kNsCell + row * kNsK + ((oct ^ row >> 3) & 1) * 8);
+    auto read = [&](int k, int operand, int q, int row) {
+      return *reinterpret_cast<const nsb8*>(lds + k % kBufs * kStage + operand * kHalf + q * kNsCell + row * kNsK + ((oct ^ row >> 3) & 1) * 8);
     };
     nsf16 acc[2][2] = {}, low[2][2] = {};
     fill(0);
-    if (kBufs == 3 && count > 1) fill(1);
+    if (count > 1) fill(1);
     for (int k = 0; k < count; ++k) {
       // this wave's part of stage k is in LDS (of the newer loads only those of stage k + 1 may be on their way), then
       // everybody's, and nobody reads stage k - 1 any more
-      if (kBufs == 3 && k + 1 < count) asm volatile("s_waitcnt vmcnt(%0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads) : "memory");
+      if (k + 1 < count) asm volatile("s_waitcnt vmcnt(%0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::"n"(kLoads) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       if (k + kBufs - 1 < count) fill(k + kBufs - 1);
+      nsb8 lf[2][kNsP], rf[2][kNsP];
 #pragma unroll
-      for (int b = 0; b < kB; ++b) {
-        nsb8 lf[2][P], rf[2][P];
+      for (int q = kNsP - 1; q >= 0; --q)
 #pragma unroll
-        for (int q = P - 1; q >= 0; --q)
+        for (int e = 0; e < 2; ++e) lf[e][q] = read(k, 0, q, lr + 32 * e), rf[e][kNsP - 1 - q] = read(k, 1, kNsP - 1 - q, rr + 32 * e);
+      // the products of pieces whose numbers add up to at most kNsP - 1, small ones first
 #pragma unroll
-          for (int e = 0; e < 2; ++e) lf[e][q] = read(k, b, 0, q, lr + 32 * e), rf[e][P - 1 - q] = read(k, b, 1, P - 1 - q, rr + 32 * e);
-        // the products of pieces whose numbers add up to at most P - 1, small ones first
+      for (int sum = kNsP - 1; sum >= 0; --sum)
 #pragma unroll
-        for (int sum = P - 1; sum >= 0; --sum)
+        for (int q = sum; q >= 0; --q)
 #pragma unroll
-          for (int q = sum; q >= 0; --q)
+          for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-              for (int f = 0; f < 2; ++f)
-                if (sum) low[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[e][q], rf[f][sum - q], low[e][f], 0, 0, 0);
-                else acc[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[e][q], rf[f][sum - q], acc[e][f], 0, 0, 0);
-      }
+            for (int f = 0; f < 2; ++f)
+              if (sum) low[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[e][q], rf[f][sum - q], low[e][f], 0, 0, 0);
+              else acc[e][f] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[e][q], rf[f][sum - q], acc[e][f], 0, 0, 0);
     }
     // slot: a whole tile's number; behind those, run + tile, which grows by one from each run's piece of a tile to the next
     const long slot = whole ? t : t + (long)(blockIdx.x - g.full);
@@ -446,14 +436,14 @@ __global__ void __launch_bounds__(256, 2) ns_product_kernel(NsArgs g) {
 
 // A workgroup = a wave's 64 x 64 quarter of a tile: its partial sums in the order of the runs, then the polynomial
 // (kNsPoly), then both orientations as pieces, or the result.
-template <int P, int STAGE>
+template <int STAGE>
 __global__ void __launch_bounds__(256) ns_join_kernel(NsArgs g) {
   __shared__ float tile[64 * kNsPitch];
   const int t = blockIdx.x >> 2, quarter = blockIdx.x & 3, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i = ns_find(g, t);
   const NsItem it = g.it[i];
   const NsShape s(it.rows, it.cols);
-  const NsPlanes<P> p(g.ws + it.ws, s);
+  const NsPlanes p(g.ws + it.ws, s);
   int ti, tj;
   ns_tile(t - it.at, s.mt(), s.nt(), STAGE != kNsApply, ti, tj);
   // the slots that hold this tile: its own number, or one for each run that has stages of it
@@ -463,9 +453,9 @@ __global__ void __launch_bounds__(256) ns_join_kernel(NsArgs g) {
     for (int k = 0; k < i; ++k) {
       const NsShape o(g.it[k].rows, g.it[k].cols);
       const int begin = max(g.it[k].at, g.full), end = g.it[k].at + ns_tiles(o, STAGE);
-      if (end > begin) unit += (long)(end - begin) * ns_stages<P>(o, STAGE);
+      if (end > begin) unit += (long)(end - begin) * ns_stages(o, STAGE);
     }
-    const int stages = ns_stages<P>(s, STAGE);
+    const int stages = ns_stages(s, STAGE);
     unit += (long)(t - max(it.at, g.full)) * stages;
     lo = t + unit / g.run, hi = t + (unit + stages - 1) / g.run;
   }
@@ -483,82 +473,60 @@ __global__ void __launch_bounds__(256) ns_join_kernel(NsArgs g) {
     for (int j = 0; j < 4; ++j)
       tile[((wave >> 1) * 32 + 8 * r + 4 * (lane >> 5) + j) * kNsPitch + (wave & 1) * 32 + (lane & 31)] = v[r][j];
   __syncthreads();
-  ns_finish<P, STAGE>(g, it, s, p, ti * kNsTile + (quarter >> 1) * 64, tj * kNsTile + (quarter & 1) * 64, ti == tj, tile);
+  ns_finish<STAGE>(g, it, s, p, ti * kNsTile + (quarter >> 1) * 64, tj * kNsTile + (quarter & 1) * 64, ti == tj, tile);
 }
 
-// The same products whole and in one launch, 32 E x 64 a workgroup: more bytes an operation, but no partial tiles and no joining
+// The same products whole and in one launch, 64 x 64 a workgroup: more bytes an operation, but no partial tiles and no joining
 // launch.  A compute unit has one workgroup, so nothing else hides its waits: each of the four waves takes every fourth block of 16
-// k-values for all of the 32 E x 64, through a ring of stages of its own that it fills and reads without any barrier -- half the LDS
-// reads of waves that share stages, and none waits for another.  Their four sums meet at the end.  E = 4 (two pieces: one sum for
-// all products, which costs 2^-24 where the pieces leave 2^-17 out; symmetric products) is a third more operations for each byte.
-template <int P, int E>
-constexpr int kNsBlockBufs = P == 2 && E == 2 ? 4 : 3;
-template <int P, int E>
-constexpr int kNsBlockLds = 4 * kNsBlockBufs<P, E> * P * (E + 2) * 1024; // waves, stages, pieces of 32 E + 64 rows of 16 k-values
-__host__ __device__ __forceinline__ int ns_block_count(const NsShape& s, int stage, int E) {
-  if (E == 4) return s.mt() * (s.mt() + 1);               // (symmetric products only)
+// k-values for all of the 64 x 64, through a ring of stages of its own that it fills and reads without any barrier -- half the LDS
+// reads of waves that share stages, and none waits for another.  Their four sums meet at the end.
+constexpr int kNsBlockBufs = 3;
+constexpr int kNsBlockLds = 4 * kNsBlockBufs * kNsP * 4 * 1024;      // waves, stages, pieces of 64 + 64 rows of 16 k-values
+__host__ __device__ __forceinline__ int ns_block_count(const NsShape& s, int stage) {
   return stage == kNsApply ? 4 * s.mt() * s.nt() : s.mt() * (2 * s.mt() + 1);
 }
-// block t of 128 x 64 of a symmetric product: its rows' panel and its half panel of columns, up to the panel's last.  Super-rows of 4.
-__device__ __forceinline__ void ns_block_tall(int t, int mt, int& i, int& j) {
-  int sr = 0;
-  while (16 * (sr + 1) * (sr + 1) + 4 * (sr + 1) <= t) ++sr;      // (blocks above super-row sr: 16 sr^2 + 4 sr)
-  t -= 16 * sr * sr + 4 * sr;
-  const int h = min(4, mt - 4 * sr);
-  if (t < 8 * sr * h) {
-    i = 4 * sr + t % h, j = t / h;
-    return;
-  }
-  t -= 8 * sr * h;
-  int l = 0;
-  while ((l + 1) * (l + 2) <= t) ++l;
-  i = 4 * sr + l, j = 8 * sr + t - l * (l + 1);
-}
-template <int P, int STAGE, int E>
+template <int STAGE>
 __global__ void __launch_bounds__(256, 1) ns_block_kernel(NsArgs g) {
-  constexpr int kBufs = kNsBlockBufs<P, E>;
-  constexpr int kLeft = P * E * 512, kStage = kLeft + P * 1024, kLoads = P * (E + 2);      // elements of the left operand's part, of a stage; 1 KB DMAs
-  constexpr bool kLow = E == 2;                           // sums of their own for the small products
-  constexpr int kSum = 64 * kNsPitch, kOwn = E / 2;       // floats of a 64 x 64 tile; 32 x 32 blocks that a wave finishes
-  constexpr bool kApart = (kSum + 3 * kOwn * 1024) * 4 <= kBufs * kStage * 2;      // the finished tile and the shares have room beside each other
-  static_assert(4 * kBufs * kStage * 2 == kNsBlockLds<P, E> && 3 * kOwn * 4096 <= kBufs * kStage * 2 && kSum % 4 == 0, "LDS");
+  constexpr int kBufs = kNsBlockBufs;
+  constexpr int kLeft = kNsP * 1024, kStage = 2 * kLeft, kLoads = 4 * kNsP;      // elements of an operand's part, of a stage; 1 KB DMAs
+  constexpr int kSum = 64 * kNsPitch;                     // floats of the finished tile, beside which the shares have room
+  static_assert(4 * kBufs * kStage * 2 == kNsBlockLds && (kSum + 3 * 1024) * 4 <= kBufs * kStage * 2 && kSum % 4 == 0, "LDS");
   extern __shared__ __align__(16) __bf16 stages_[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // an XCD has an eighth of every matrix' blocks, one run of them
   const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, i = ns_find(g, slot);
   const NsItem it = g.it[i];
   const NsShape s(it.rows, it.cols);
-  const int blocks = ns_block_count(s, STAGE, E), t = xcd * ((blocks + 7) / 8) + slot - it.at;
+  const int blocks = ns_block_count(s, STAGE), t = xcd * ((blocks + 7) / 8) + slot - it.at;
   if (t >= blocks || slot - it.at >= (blocks + 7) / 8) return;
-  const NsPlanes<P> p(g.ws + it.ws, s);
+  const NsPlanes p(g.ws + it.ws, s);
   int ti, tj;
-  if (E == 2) ns_tile(t, 2 * s.mt(), 2 * s.nt(), STAGE != kNsApply, ti, tj);
-  else ns_block_tall(t, s.mt(), ti, tj);
+  ns_tile(t, 2 * s.mt(), 2 * s.nt(), STAGE != kNsApply, ti, tj);
   const int K = STAGE == kNsGram ? s.np : s.mp, count = K / (kNsK * 4);
   // (a half panel: rows 64 (t & 1) ... of every block's pieces)
-  const long panel = (long)(K / kNsK) * (P * kNsCell), mine = (long)wave * (P * kNsCell) + lane * 8;
-  const __bf16* L = (STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : p.q) + (E == 2 ? (ti >> 1) * panel + (ti & 1) * 1024 : ti * panel) + mine;
+  const long panel = (long)(K / kNsK) * (kNsP * kNsCell), mine = (long)wave * (kNsP * kNsCell) + lane * 8;
+  const __bf16* L = (STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : p.q) + (ti >> 1) * panel + (ti & 1) * 1024 + mine;
   const __bf16* R = (STAGE == kNsGram ? p.x : STAGE == kNsPoly ? p.a : (g.flip ? p.xt1 : p.xt)) + (tj >> 1) * panel + (tj & 1) * 1024 + mine;
   __bf16* ring = stages_ + wave * (kBufs * kStage);
   auto fill = [&](int k) {
     __bf16* to = ring + k % kBufs * kStage;
-    const long at = (long)k * (4 * P * kNsCell);
+    const long at = (long)k * (4 * kNsP * kNsCell);
 #pragma unroll
     for (int c = 0; c < kLoads; ++c) {                    // (1 KB = 32 rows of a piece of a block; L's first, then R's)
-      const int d = c < P * E ? c / E * kNsCell + c % E * 512 : (c - P * E) / 2 * kNsCell + (c - P * E) % 2 * 512;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((c < P * E ? L : R) + at + d),
+      const int h = c % (2 * kNsP), d = h / 2 * kNsCell + h % 2 * 512;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((c < 2 * kNsP ? L : R) + at + d),
                                        (__attribute__((address_space(3))) void*)(to + c * 512), 16, 0, 0);
     }
   };
   const int row = lane & 31, oct = lane >> 5, cell = row * kNsK + ((oct ^ row >> 3) & 1) * 8;      // (32 rows on: the same cell)
-  nsf16 acc[E][2] = {}, low[kLow ? E : 1][2] = {};
-  nsb8 lf[2][E][P], rf[2][2][P];                          // operands of the stage that is multiplied, and of the next
+  nsf16 acc[2][2] = {}, low[2][2] = {};                   // (low: sums of their own for the small products)
+  nsb8 lf[2][2][kNsP], rf[2][2][kNsP];                    // operands of the stage that is multiplied, and of the next
   auto fetch = [&](int k, int into) {
     const __bf16* b = ring + k % kBufs * kStage + cell;
 #pragma unroll
-    for (int q = 0; q < P; ++q) {
+    for (int q = 0; q < kNsP; ++q) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) lf[into][e][q] = *reinterpret_cast<const nsb8*>(b + (q * E + e) * 512);
+      for (int e = 0; e < 2; ++e) lf[into][e][q] = *reinterpret_cast<const nsb8*>(b + (q * 2 + e) * 512);
 #pragma unroll
       for (int f = 0; f < 2; ++f) rf[into][f][q] = *reinterpret_cast<const nsb8*>(b + kLeft + (q * 2 + f) * 512);
     }
@@ -580,58 +548,46 @@ __global__ void __launch_bounds__(256, 1) ns_block_kernel(NsArgs g) {
       if (k + u + kBufs < count) fill(k + u + kBufs);
       fetch(min(k + u + 1, count - 1), u ^ 1);
 #pragma unroll
-      for (int sum = P - 1; sum >= 0; --sum)
+      for (int sum = kNsP - 1; sum >= 0; --sum)
 #pragma unroll
         for (int q = sum; q >= 0; --q)
 #pragma unroll
-          for (int e = 0; e < E; ++e)
+          for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int f = 0; f < 2; ++f) {
-              nsf16& to = kLow && sum ? low[kLow ? e : 0][f] : acc[e][f];
+              nsf16& to = sum ? low[e][f] : acc[e][f];
               to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lf[u][e][q], rf[u][f][sum - q], to, 0, 0, 0);
             }
     }
-  // Wave w finishes kOwn 32 x 32 blocks of the sums, from w kOwn on: the others' shares of them come through their rings
+  // Wave w finishes 32 x 32 block w of the sums: the others' shares of it come through their rings
   arrive(count);
-  constexpr int kRing = kBufs * kStage / 2, kOut = kApart ? kSum : 0;      // floats
+  constexpr int kRing = kBufs * kStage / 2;               // floats
   float* tile = reinterpret_cast<float*>(stages_);
-  nsf4 own[kOwn][4];
+  nsf4 own[4];
 #pragma unroll
-  for (int b = 0; b < 2 * E; ++b)
+  for (int b = 0; b < 4; ++b)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       nsf4 v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = acc[b >> 1][b & 1][4 * r + j] + (kLow ? low[kLow ? b >> 1 : 0][b & 1][4 * r + j] : 0.f);
-      if (b / kOwn == wave) own[b % kOwn][r] = v;
-      else *reinterpret_cast<nsf4*>(tile + wave * kRing + kOut + (((b / kOwn - wave - 1 & 3) * kOwn + b % kOwn) * 4 + r) * 256 + lane * 4) = v;
+      for (int j = 0; j < 4; ++j) v[j] = acc[b >> 1][b & 1][4 * r + j] + low[b >> 1][b & 1][4 * r + j];
+      if (b == wave) own[r] = v;
+      else *reinterpret_cast<nsf4*>(tile + wave * kRing + kSum + ((b - wave - 1 & 3) * 4 + r) * 256 + lane * 4) = v;
     }
   __syncthreads();
 #pragma unroll
   for (int d = 1; d < 4; ++d) {
-    const int from = wave + d & 3;                        // (its shares: blocks of wave from + 1, from + 2, from + 3)
-#pragma unroll
-    for (int o = 0; o < kOwn; ++o)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        own[o][r] += *reinterpret_cast<const nsf4*>(tile + from * kRing + kOut + (((wave - from - 1 & 3) * kOwn + o) * 4 + r) * 256 + lane * 4);
-  }
-  if (!kApart) __syncthreads();
-#pragma unroll
-  for (int o = 0; o < kOwn; ++o) {
-    const int b = wave * kOwn + o;                        // row block b / 2, column block b % 2
+    const int from = wave + d & 3;                        // (its shares: blocks from + 1, from + 2, from + 3)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        tile[(b >> 2) * kSum + ((b >> 1 & 1) * 32 + 8 * r + 4 * oct + j) * kNsPitch + (b & 1) * 32 + row] = own[o][r][j];
+      own[r] += *reinterpret_cast<const nsf4*>(tile + from * kRing + kSum + ((wave - from - 1 & 3) * 4 + r) * 256 + lane * 4);
   }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) tile[((wave >> 1) * 32 + 8 * r + 4 * oct + j) * kNsPitch + (wave & 1) * 32 + row] = own[r][j];
   __syncthreads();
-#pragma unroll
-  for (int h = 0; h < E / 2; ++h) {
-    const int rb = ti * (E / 2) + h;                      // (symmetric, 128 x 64: the upper half may lie above the diagonal)
-    if (STAGE == kNsApply || rb >= tj) ns_finish<P, STAGE>(g, it, s, p, rb * 64, tj * 64, rb == tj, tile + h * kSum);
-  }
+  ns_finish<STAGE>(g, it, s, p, ti * 64, tj * 64, ti == tj, tile);
 }
 
 // ---- short sides of up to 128 ------------------------------------------------------------------------------------------------
@@ -648,12 +604,11 @@ __global__ void __launch_bounds__(256, 1) ns_block_kernel(NsArgs g) {
 // that has more workgroups than fit the card at once gets more columns each: cheaper than a second round.  (64 columns of more
 // than 64 rows would be four blocks a wave: 10 % slower at 128 x 2048 than 32.)
 // Long sides: the shares that everybody adds up grow with n^2.  Above 64 rows up to 2048 (128 x 2048 181 us, through the large
-// matrices' way 187; 128 x 3000 229 and 174), bf16 up to 1024 (128 x 1024 123 and 118, 96 x 1024 106 and 117; 128 x 2048 181 and
-// 144); below them 64 x 8192 takes 134 us (226), 64 x 16384 218 (320, bf16 287).
+// matrices' way 187; 128 x 3000 229 and 174); below them 64 x 8192 takes 134 us (226), 64 x 16384 218 (320).
 // A step's time: 128 x 128 10 us, 64 x 1728 12.5 us; the network of MVSNeRF, 29 matrices, 13.5 us.  4 us of it is one launch
 // behind another; the rest is a chain of shares, two products and the next share, of which the products are a quarter.
 constexpr int kNsShort = 128;                            // short side, and long side (below), up to which this way is taken
-__host__ __device__ __forceinline__ int ns_short_long(int m, int dtype) { return m <= 64 ? 16384 : dtype == 1 ? 1024 : 2048; }
+__host__ __device__ __forceinline__ int ns_short_long(int m) { return m <= 64 ? 16384 : 2048; }
 __host__ __device__ __forceinline__ int ns_columns(int m, int n, int least) {
   const int t = n <= 288 ? 16 : n <= 1152 ? 32 : 64, u = t > least ? t : least;
   return m > 64 && u > 32 ? 32 : u;
@@ -896,9 +851,9 @@ static int ns_chunks(int rows, int cols) { return (int)(((long)rows * cols + kNs
 
 // limit: of the short side, what BMV_NS_SHORT is at the call (read once: the workspace's layout goes by it)
 static int ns_limit() { return std::min(kNsShort, tuning("BMV_NS_SHORT", kNsShort)); }
-static bool ns_is_short(int rows, int cols, int dtype, int limit) {
+static bool ns_is_short(int rows, int cols, int limit) {
   const int m = std::min(rows, cols);
-  return m <= limit && std::max(rows, cols) <= ns_short_long(m, dtype);
+  return m <= limit && std::max(rows, cols) <= ns_short_long(m);
 }
 // Workspace of a part of the list (indices): the short ones' X and shares, or the others' pieces, then the norm's partial
 // sums, then partial tiles
@@ -924,42 +879,41 @@ static long ns_short_room(const int* rows, const int* cols, const int* idx, int 
 struct NsRoom {
   long pieces = 0, tiles = 0;
   int sqn = 1;
-  NsRoom(const int* rows, const int* cols, const int* idx, int n, int p) {
+  NsRoom(const int* rows, const int* cols, const int* idx, int n) {
     for (int k = 0; k < n; ++k) {
       const int i = idx[k];
       const NsShape s(rows[i], cols[i]);
-      pieces += ns_bytes(s, p), tiles += (long)s.mt() * s.nt();      // (no fewer than the symmetric products')
+      pieces += ns_bytes(s), tiles += (long)s.mt() * s.nt();      // (no fewer than the symmetric products')
       sqn = std::max(sqn, ns_chunks(rows[i], cols[i]));
     }
   }
   long bytes() const { return pieces + (long)kNsList * sqn * sizeof(double) + (tiles + kNsSlots) * (kNsTile * kNsTile * 4l); }
 };
 // the list's indices: the short ones, then the others
-static std::vector<int> ns_order(int count, const int* rows, const int* cols, int dtype, int limit, int& shorts) {
+static std::vector<int> ns_order(int count, const int* rows, const int* cols, int limit, int& shorts) {
   std::vector<int> v;
   v.reserve(count);
   for (int i = 0; i < count; ++i)
-    if (ns_is_short(rows[i], cols[i], dtype, limit)) v.push_back(i);
+    if (ns_is_short(rows[i], cols[i], limit)) v.push_back(i);
   shorts = (int)v.size();
   for (int i = 0; i < count; ++i)
-    if (!ns_is_short(rows[i], cols[i], dtype, limit)) v.push_back(i);
+    if (!ns_is_short(rows[i], cols[i], limit)) v.push_back(i);
   return v;
 }
 // a list is done in parts of kNsList, which share the workspace
-static long ns_workspace(int count, const int* rows, const int* cols, int dtype, const std::vector<int>& v, int shorts) {
+static long ns_workspace(int count, const int* rows, const int* cols, const std::vector<int>& v, int shorts) {
   long most = 0;
   for (int b = 0; b < shorts; b += kNsList) most = std::max(most, ns_short_room(rows, cols, &v[b], std::min(shorts - b, kNsList)));
-  for (int b = shorts; b < count; b += kNsList)
-    most = std::max(most, NsRoom(rows, cols, &v[b], std::min(count - b, kNsList), dtype == 1 ? 2 : 3).bytes());
+  for (int b = shorts; b < count; b += kNsList) most = std::max(most, NsRoom(rows, cols, &v[b], std::min(count - b, kNsList)).bytes());
   return most;
 }
 
 // 64 x 64 blocks, where rounds of them on all compute units are cheaper than tiles, a cut along k and a join: that goes by the k
-// a compute unit walks.  A launch of them is 7.5 us and 0.2 (bf16: 0.13) us for 32 k-values -- k = 384 9.9 us, 1024 13.7 ... 19.3
+// a compute unit walks.  A launch of them is 7.5 us and 0.2 us for 32 k-values -- k = 384 9.9 us, 1024 13.7 ... 19.3
 // by how many blocks share the caches --, cut tiles and the launch that joins them 14 ... 25.  Five steps with blocks up to 2048
-// and up to 1024: 1024 x 2048 402 us and 428, bf16 294 and 328, 768 x 2048 334 and 350, 512 x 2048 251 and 246.
+// and up to 1024: 1024 x 2048 402 us and 428, 768 x 2048 334 and 350, 512 x 2048 251 and 246.
 constexpr int kNsBlockK = 2048;
-template <int P, int STAGE, int E>
+template <int STAGE>
 static void ns_block_launch(NsArgs& g, hipStream_t st) {
   // (the longest first: an item's blocks begin in the order of the list)
   std::stable_sort(g.it, g.it + g.count, [](const NsItem& a, const NsItem& b) {
@@ -967,43 +921,24 @@ static void ns_block_launch(NsArgs& g, hipStream_t st) {
     return k(a) > k(b);
   });
   int slots = 0;
-  for (int i = 0; i < g.count; ++i) g.it[i].at = slots, slots += (ns_block_count(NsShape(g.it[i].rows, g.it[i].cols), STAGE, E) + 7) / 8;
-  hipLaunchKernelGGL((ns_block_kernel<P, STAGE, E>), dim3(8u * slots), dim3(256), (kNsBlockLds<P, E>), st, g);
+  for (int i = 0; i < g.count; ++i) g.it[i].at = slots, slots += (ns_block_count(NsShape(g.it[i].rows, g.it[i].cols), STAGE) + 7) / 8;
+  hipLaunchKernelGGL((ns_block_kernel<STAGE>), dim3(8u * slots), dim3(256), kNsBlockLds, st, g);
 }
-// 128 x 64 blocks for symmetric products of two pieces that are too large for those: where they keep the compute units busy for
-// kNsTallBusy of the longest one's time, and that is no longer than kNsTallK k-values.  Five steps with them and with tiles (bf16):
-// 1500 x 1500 445 us and 492, 3000 x 3000 2055 and 2255, eight of 768 x 768 562 and 600, two of 1024 x 4096 with four of 1024 x 1024
-// 1030 and 1131.  Below that share tiles' cut along k is better (A of 1024 x 4096, 28 % busy: 38 us and 28), above that length
-// their traffic is (4096 x 4096: 2 % slower).  Q X has whole tiles for all compute units sooner: 3 ... 6 % slower with these.
-constexpr int kNsTallBusy = 60, kNsTallK = 10240;
-template <int P, int STAGE>
+template <int STAGE>
 static bool ns_blocks(NsArgs& g, hipStream_t st) {
-  long blocks = 0, most = 0, work = 0, least = 1 << 20;
+  long blocks = 0, most = 0;
   for (int i = 0; i < g.count; ++i) {
     const NsShape s(g.it[i].rows, g.it[i].cols);
-    const long k = STAGE == kNsGram ? s.np : s.mp;
-    blocks += ns_block_count(s, STAGE, 2), work += k * ns_block_count(s, STAGE, 4);
-    most = std::max(most, k), least = std::min(least, k);
+    blocks += ns_block_count(s, STAGE), most = std::max<long>(most, STAGE == kNsGram ? s.np : s.mp);
   }
-  const long limit = tuning("BMV_NS_BLOCK_K", kNsBlockK);
-  if ((blocks + kNsUnits - 1) / kNsUnits * most <= limit) {
-    ns_block_launch<P, STAGE, 2>(g, st);
-    return true;
-  }
-  if constexpr (P == 2 && STAGE != kNsApply) {
-    // k-values of the compute unit that has most, in rounds of the shortest blocks
-    const long span = std::max(most, (work + kNsUnits * least - 1) / (kNsUnits * least) * least);
-    if (limit > 0 && span <= kNsTallK && work * 100 >= span * kNsUnits * kNsTallBusy) {
-      ns_block_launch<P, STAGE, 4>(g, st);
-      return true;
-    }
-  }
-  return false;
+  if ((blocks + kNsUnits - 1) / kNsUnits * most > tuning("BMV_NS_BLOCK_K", kNsBlockK)) return false;
+  ns_block_launch<STAGE>(g, st);
+  return true;
 }
 
-template <int P, int STAGE>
+template <int STAGE>
 static void ns_product(NsArgs& g, hipStream_t st) {
-  if (ns_blocks<P, STAGE>(g, st)) return;
+  if (ns_blocks<STAGE>(g, st)) return;
   long tiles = 0, units = 0;
   for (int i = 0; i < g.count; ++i) {
     const NsShape s(g.it[i].rows, g.it[i].cols);
@@ -1014,14 +949,14 @@ static void ns_product(NsArgs& g, hipStream_t st) {
   for (int i = 0; i < g.count; ++i) {
     const NsShape s(g.it[i].rows, g.it[i].cols);
     const long end = i + 1 < g.count ? g.it[i + 1].at : tiles, begin = std::max<long>(g.it[i].at, g.full);
-    if (end > begin) units += (end - begin) * ns_stages<P>(s, STAGE);
+    if (end > begin) units += (end - begin) * ns_stages(s, STAGE);
   }
-  // A run for every compute unit (two for each hide more latency, but a partial tile is 64 KB through memory: 1024 x 4096 bf16 432 us,
-  // one 409; 512 x 4096 fp32 331, 319), but of at least 256 k-values for the same reason: 160 x 8192 fp32 283 us, with 128 322 and
-  // with 384 295; bf16 242, with 128 290 and with 384 243; 256 x 4096 bf16 175, 198 and 190.  Panels are multiples of 128 long.
-  g.run = (int)std::max<long>((units + kNsUnits - 1) / kNsUnits, 256 / (kNsK * kNsBlocks<P>));
-  hipLaunchKernelGGL((ns_product_kernel<P, STAGE>), dim3((unsigned)(g.full + (units + g.run - 1) / g.run)), dim3(256), 0, st, g);
-  hipLaunchKernelGGL((ns_join_kernel<P, STAGE>), dim3((unsigned)(4 * tiles)), dim3(256), 0, st, g);
+  // A run for every compute unit (two for each hide more latency, but a partial tile is 64 KB through memory: 512 x 4096 331 us, one
+  // 319), but of at least 256 k-values for the same reason: 160 x 8192 283 us, with 128 322 and with 384 295.  Panels are multiples
+  // of 128 long.
+  g.run = (int)std::max<long>((units + kNsUnits - 1) / kNsUnits, 256 / kNsK);
+  hipLaunchKernelGGL((ns_product_kernel<STAGE>), dim3((unsigned)(g.full + (units + g.run - 1) / g.run)), dim3(256), 0, st, g);
+  hipLaunchKernelGGL((ns_join_kernel<STAGE>), dim3((unsigned)(4 * tiles)), dim3(256), 0, st, g);
 }
 
 struct NsLists {
@@ -1100,7 +1035,6 @@ static void ns_run_short(NsArgs& g, int least, int steps, char* ws, hipStream_t 
   }
 }
 
-template <int P>
 static void ns_run_long(NsArgs& g, const NsRoom& room, int steps, char* ws, hipStream_t st) {
   g.ws = ws, g.sqn = room.sqn, g.sq = reinterpret_cast<double*>(ws + room.pieces);
   g.part = reinterpret_cast<float*>(g.sq + (long)kNsList * g.sqn);
@@ -1108,16 +1042,16 @@ static void ns_run_long(NsArgs& g, const NsRoom& room, int steps, char* ws, hipS
   for (int i = 0; i < g.count; ++i) {
     NsItem& it = g.it[i];
     it.ws = off, it.at = (int)chunks;
-    off += ns_bytes(NsShape(it.rows, it.cols), P), chunks += ns_chunks(it.rows, it.cols);
+    off += ns_bytes(NsShape(it.rows, it.cols)), chunks += ns_chunks(it.rows, it.cols);
   }
   ns_typed(g, [&](auto dt, auto muon) { hipLaunchKernelGGL((ns_norm_kernel<decltype(dt)::value, decltype(muon)::value>), dim3((unsigned)chunks), dim3(256), 0, st, g); });
   for (int i = 0; i < g.count; ++i) g.it[i].at = (int)blocks, blocks += NsShape(g.it[i].rows, g.it[i].cols).big() / (64 * 64);
   ns_typed(g, [&](auto dt, auto muon) { hipLaunchKernelGGL((ns_split_kernel<decltype(dt)::value, decltype(muon)::value>), dim3((unsigned)blocks), dim3(256), 0, st, g); });
   for (int k = 0; k < steps; ++k) {
     g.last = k + 1 == steps, g.flip = k & 1;
-    ns_product<P, kNsGram>(g, st);
-    ns_product<P, kNsPoly>(g, st);
-    ns_product<P, kNsApply>(g, st);
+    ns_product<kNsGram>(g, st);
+    ns_product<kNsPoly>(g, st);
+    ns_product<kNsApply>(g, st);
   }
 }
 
@@ -1136,24 +1070,19 @@ static bool ns_lds() {
                                            {(const void*)ns_short_kernel<true, 1, true>, kLds},
                                            {(const void*)ns_short_kernel<true, 2, true>, kLds},
                                            {(const void*)ns_short_kernel<false, 0, false>, kLds},
-                                           {(const void*)ns_block_kernel<3, kNsGram, 2>, kNsBlockLds<3, 2>},
-                                           {(const void*)ns_block_kernel<3, kNsPoly, 2>, kNsBlockLds<3, 2>},
-                                           {(const void*)ns_block_kernel<3, kNsApply, 2>, kNsBlockLds<3, 2>},
-                                           {(const void*)ns_block_kernel<2, kNsGram, 2>, kNsBlockLds<2, 2>},
-                                           {(const void*)ns_block_kernel<2, kNsPoly, 2>, kNsBlockLds<2, 2>},
-                                           {(const void*)ns_block_kernel<2, kNsApply, 2>, kNsBlockLds<2, 2>},
-                                           {(const void*)ns_block_kernel<2, kNsGram, 4>, kNsBlockLds<2, 4>},
-                                           {(const void*)ns_block_kernel<2, kNsPoly, 4>, kNsBlockLds<2, 4>}};
+                                           {(const void*)ns_block_kernel<kNsGram>, kNsBlockLds},
+                                           {(const void*)ns_block_kernel<kNsPoly>, kNsBlockLds},
+                                           {(const void*)ns_block_kernel<kNsApply>, kNsBlockLds}};
   for (const auto& k : f)
     if (hipFuncSetAttribute(k.first, hipFuncAttributeMaxDynamicSharedMemorySize, k.second) != hipSuccess) return false;
   ready.fetch_or(bit, std::memory_order_release);
   return true;
 }
 
-static const char* ns_run(NsArgs g, int count, const NsLists& l, int dtype, int steps, void* workspace, long bytes, hipStream_t st) {
+static const char* ns_run(NsArgs g, int count, const NsLists& l, int steps, void* workspace, long bytes, hipStream_t st) {
   int shorts;
-  const std::vector<int> v = ns_order(count, l.rows, l.cols, dtype, ns_limit(), shorts);
-  if (ns_workspace(count, l.rows, l.cols, dtype, v, shorts) > bytes) return "the workspace is too small";
+  const std::vector<int> v = ns_order(count, l.rows, l.cols, ns_limit(), shorts);
+  if (ns_workspace(count, l.rows, l.cols, v, shorts) > bytes) return "the workspace is too small";
   if (!ns_lds()) return "LDS refused";
   char* ws = static_cast<char*>(workspace);
   for (int b = 0; b < shorts; b += kNsList) {
@@ -1164,8 +1093,7 @@ static const char* ns_run(NsArgs g, int count, const NsLists& l, int dtype, int 
   for (int b = shorts; b < count; b += kNsList) {
     const int n = std::min(count - b, kNsList);
     ns_fill(g, l, &v[b], n);
-    if (dtype == 1) ns_run_long<2>(g, NsRoom(l.rows, l.cols, &v[b], n, 2), steps, ws, st);
-    else ns_run_long<3>(g, NsRoom(l.rows, l.cols, &v[b], n, 3), steps, ws, st);
+    ns_run_long(g, NsRoom(l.rows, l.cols, &v[b], n), steps, ws, st);
   }
   return nullptr;
 }
@@ -1182,8 +1110,8 @@ long bmv_newton_schulz_workspace(int count, const int* rows, const int* cols, in
   BMV_REQUIRE(dtype >= 0 && dtype <= 2, "bmv_newton_schulz_workspace: unknown type %d", dtype);
   return ns_no_throw([&]() -> long {
     int shorts;
-    const std::vector<int> v = ns_order(count, rows, cols, dtype, ns_limit(), shorts);
-    return ns_workspace(count, rows, cols, dtype, v, shorts);
+    const std::vector<int> v = ns_order(count, rows, cols, ns_limit(), shorts);
+    return ns_workspace(count, rows, cols, v, shorts);
   });
 }
 
@@ -1201,7 +1129,7 @@ int bmv_newton_schulz(int count, const void* const* src, void* const* dst, const
     NsArgs g{};
     g.dtype = dtype, g.a = a, g.b = b, g.c = c, g.eps = eps;
     const NsLists l{src, dst, nullptr, rows, cols, nullptr};
-    bad = ns_run(g, count, l, dtype, steps, workspace, workspace_bytes, as_stream(stream));
+    bad = ns_run(g, count, l, steps, workspace, workspace_bytes, as_stream(stream));
     BMV_REQUIRE(!bad, "bmv_newton_schulz: %s", bad);
     BMV_LAUNCH_END("bmv_newton_schulz");
   });
@@ -1224,7 +1152,7 @@ int bmv_muon_step(int count, void* const* params, const void* const* grads, floa
     NsArgs g{};
     g.dtype = dtype, g.a = a, g.b = b, g.c = c, g.eps = eps, g.muon = 1, g.nesterov = nesterov, g.mu = (float)momentum, g.nu = (float)(1. - momentum), g.keep = (float)keep;
     const NsLists l{grads, params, momenta, rows, cols, scales};
-    bad = ns_run(g, count, l, dtype, steps, workspace, workspace_bytes, as_stream(stream));
+    bad = ns_run(g, count, l, steps, workspace, workspace_bytes, as_stream(stream));
     BMV_REQUIRE(!bad, "bmv_muon_step: %s", bad);
     BMV_LAUNCH_END("bmv_muon_step");
   });

@@ -1611,7 +1611,8 @@ def newton_schulz(mats, steps=5, coeffs=NS_COEFFS, eps=NS_EPS):
     """Orthogonalise matrices: X = M / max(|M|_F, eps), then `steps` times A = X X^T, X = a X + (b A + c A A) X with
     `coeffs` = (a, b, c) -- singular values towards 1, singular vectors kept.  `mats`: a tensor, or a list of tensors (one set
     of launches for all), of 2 dimensions or more (what is behind the first is flattened: convolution kernels), fp32, bf16 or
-    fp16.  Computed at fp32 accuracy (bf16: with 17-bit operands).  -> new tensors of the same shapes and types."""
+    fp16.  Computed at fp32 accuracy whatever the
+    type, rounded once.  -> new tensors of the same shapes and types."""
     if torch.is_tensor(mats):
         return newton_schulz([mats], steps, coeffs, eps)[0]
     mats = list(mats)

@@ -368,7 +368,7 @@ int bmv_group_norm_bwd(const bmv_group_norm_spec* spec, const void* x, const voi
 /* ---- orthogonalised updates of weight matrices (training; beside the reference's Adam, lib/train/optimizer.py:12-28)
  * Newton-Schulz iteration of `count` matrices src[i] (rows[i], cols[i]), row-major, contiguous, all of `dtype` (0 fp32, 1 bf16,
  * 2 fp16) -> dst[i]: X = src / max(|src|_F, eps), then `steps` times A = X X^T, X = a X + (b A + c A A) X (on the transpose
- * where rows > cols).  operands of 24 bits (bf16: 17), one rounding at the end; a non-finite value (up to 128 rows: also a
+ * where rows > cols).  operands of 24 bits whatever the type, one rounding at the end; a non-finite value (up to 128 rows: also a
  * norm whose square leaves fp32) makes its matrix NaN and leaves the others alone.  Reproducible; a matrix' last bits depend on what else is in the list (where sums are cut).  The arrays are
  * HOST arrays, read before the call returns; eps >= 1e-12, sides up to 65536.
  * workspace: bmv_newton_schulz_workspace(...) bytes or more, beginning at a 256-byte border; the call refuses one that is too

@@ -99,6 +99,29 @@ def test_newton_schulz_matches_the_formula(dtype, way):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_sixteen_bit_matrices_are_computed_as_fp32_ones(dtype, way):
+    """A 16-bit matrix' result is the fp32 result of the same values rounded once, a 16-bit weight's step the fp32 step rounded
+    once: bit for bit, because the way, the operands and the order of the sums go by the sizes alone."""
+    from boostmvsnerfs_amd import ops
+    mats = [_grad(m, n, seed=i).to(dtype).cuda() for i, (m, n) in enumerate(SHAPES)]
+    for steps in (5, 8):
+        for got, want in zip(ops.newton_schulz(mats, steps=steps), ops.newton_schulz([v.float() for v in mats], steps=steps)):
+            assert torch.equal(got, want.to(dtype)), (steps, got.shape)
+    for m, n in ((700, 90), (333, 1000), (1024, 1100)):                     # ... alone as well
+        u = _grad(m, n, 7).to(dtype).cuda()
+        assert torch.equal(ops.newton_schulz(u), ops.newton_schulz(u.float()).to(dtype)), (m, n)
+    g = torch.Generator().manual_seed(3)
+    params = [torch.randn(v.shape, generator=g).to(dtype).cuda() for v in mats]
+    momenta = [1e-2 * torch.randn(v.shape, generator=g).cuda() for v in mats]
+    p32, m32 = [p.float() for p in params], [m.clone() for m in momenta]
+    ops.muon_step(params, mats, momenta, 0.02, weight_decay=0.01)
+    ops.muon_step(p32, [v.float() for v in mats], m32, 0.02, weight_decay=0.01)
+    for p, m, q, k in zip(params, momenta, p32, m32):
+        assert torch.equal(m, k) and torch.equal(p, q.to(dtype)), p.shape
+
+
+@gpu
 def test_newton_schulz_is_as_exact_as_the_iteration_in_fp32(way):
     """Within four times the error of the same iteration in fp32 products (four: two roundings for its one at the operands'
     pieces, and the spread of one random error against another), on flat and on decaying spectra."""
