@@ -6,11 +6,11 @@
 //   g = dy act'(z);  db_c = sum g;  dw_c = sum g xhat;  dx = rstd (g w - (sum_g g w + xhat sum_g g w xhat) / M)
 //   act(v) = v > 0 ? v : slope v (1 none, 0 ReLU, 0.01 leaky ReLU), or v / (1 + exp(-v)) (SiLU)
 //
-// Numbers.  Sums are 64-bit (mean and variance as sum x and sum x^2: x^2 of a 32-bit x is exact in 64 bits, so the difference
-// loses 1e-16 (mean / std)^2 and no pivot is needed).  That is not only for long sums: act' of the ReLUs jumps at z = 0, so
-// the backward has to decide the sign of z as the exact value has it.  It computes z in 32 bits and, where |z| is within
-// 2^-18 of its terms (a few values in a million), again in 64 with the saved 64-bit statistics.  x - mean is taken as
-// (x - mh) - ml with mean = mh + ml, so a large common offset costs no accuracy.
+// Numbers.  Sums are 64-bit; the backward adds four terms at a time in 32 bits first.  Mean and variance are sum x and sum x^2: x^2
+// of a 32-bit x is exact in 64 bits, so the difference loses 1e-16 (mean / std)^2 and no pivot is needed.  That is not only for
+// long sums: act' of the ReLUs jumps at z = 0, so the backward has to decide the sign of z as the exact value has it.  It
+// computes z in 32 bits and, where |z| is within 2^-18 of its terms (a few values in a million), again in 64 with the saved 64-bit
+// statistics.  x - mean is taken as (x - mh) - ml with mean = mh + ml, so a large common offset costs no accuracy.
 //
 // What bounds it: bytes, and for small maps the launches.  Two launches each way: sums of a chunk per workgroup -> partials; then
 // every workgroup joins the partials of the groups it touches (always in the same order: bit-reproducible, no atomics) and writes
@@ -700,16 +700,17 @@ __global__ void __launch_bounds__(kGnThreads) gn_pl_bwd_reduce_kernel(GnArgs a) 
         const long iu = i + u * TPU * V < t.end ? i + u * TPU * V : i;
         v[u] = gn_load<T, V>(p + iu), e[u] = gn_load<T, V>(pd + iu);
       }
-      float fs = 0.f, fq = 0.f;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int j = 0; j < V; ++j) {
+        float fs = 0.f, fq = 0.f;                         // (four terms in 32 bits, their sum in 64, as in gn_cl_bwd_reduce_kernel)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
+        for (int u = 0; u < U; ++u) {
           const float x = (float)v[u].v[j], d = (x - mh) - ml;
           const float gr = gn_grad<SILU>((float)e[u].v[j], x, d, sc, b, w, a.slope, mean, rstd);
           if (i + u * TPU * V < t.end) fs += gr, fq += gr * d;
         }
-      s += (double)fs, q += (double)fq;
+        s += (double)fs, q += (double)fq;
+      }
     }
   }
   double2 v = gn_unit_sum<TPU>(s, q);

@@ -188,6 +188,24 @@ def test_group_norm_other_strides_and_offsets():
 
 
 @gpu
+@pytest.mark.parametrize("layout", ["last", "planar"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_group_norm_gradient_sums_leave_32_bits_after_four_terms(dtype, layout):
+    """Large terms among many of 2^-24 of them, which a long sum in 32 bits loses all.  Without an activation g is dy itself, so
+    db's error is the sums' alone: three roundings of at most 2^-24 of four terms of one sign, and the result's one (the
+    64-bit sums and second-order terms are in the last 2^-4 of a 2^-24)."""
+    from boostmvsnerfs_amd import ops
+    x = torch.randn(1, 2, 32, 64, generator=torch.Generator().manual_seed(1)).to(dtype)
+    i = torch.arange(2048)
+    dy = torch.where((i % 8 == 0) & (i < 512), 2.0 ** 10, 2.0 ** -14).to(dtype).view(1, 1, 32, 64).expand(1, 2, 32, 64).contiguous()
+    xg, dyg, w, b = _place(x, layout), _place(dy, layout), torch.ones(2).cuda(), torch.zeros(2).cuda()
+    _, mean, rstd = ops.group_norm_fwd(xg, 1, w, b)
+    db = ops.group_norm_bwd(xg, dyg, 1, w, b, mean, rstd)[2]
+    want = dy.double().sum((0, 2, 3))
+    _close(db, want, (4 + 2 ** -4) * E32 * want, "db")
+
+
+@gpu
 def test_group_norm_decides_the_sign_at_zero_as_64_bits_do():
     """Values whose exact z is a few 1e-9 off zero, either side: a 32-bit z cannot tell them apart, dx would be off by dy."""
     g = torch.Generator().manual_seed(5)
