@@ -6,11 +6,13 @@
 //   g = dy act'(z);  db_c = sum g;  dw_c = sum g xhat;  dx = rstd (g w - (sum_g g w + xhat sum_g g w xhat) / M)
 //   act(v) = v > 0 ? v : slope v (1 none, 0 ReLU, 0.01 leaky ReLU), or v / (1 + exp(-v)) (SiLU)
 //
-// Numbers.  Sums are 64-bit; the backward adds four terms at a time in 32 bits first.  Mean and variance are sum x and sum x^2: x^2
-// of a 32-bit x is exact in 64 bits, so the difference loses 1e-16 (mean / std)^2 and no pivot is needed.  That is not only for
-// long sums: act' of the ReLUs jumps at z = 0, so the backward has to decide the sign of z as the exact value has it.  It
-// computes z in 32 bits and, where |z| is within 2^-18 of its terms (a few values in a million), again in 64 with the saved 64-bit
-// statistics.  x - mean is taken as (x - mh) - ml with mean = mh + ml, so a large common offset costs no accuracy.
+// Numbers.  Sums are 64-bit; the backward adds four terms at a time in 32 bits first.  Mean and variance are sum d and sum d^2 of
+// d = x - pivot, the pivot the group's first value: (mean - pivot)^2 <= M var whatever the values are, so the difference that
+// gives the variance loses at most M 2^-52 of it.  (Of x itself it would lose (mean / std)^2 2^-52: half a percent at an offset of 5e6
+// standard deviations, which fp32 maps can hold.)  64 bits are not only for long sums: act' of the ReLUs jumps at z = 0, so
+// the backward has to decide the sign of z as the exact value has it.  It computes z in 32 bits and, where |z| is within 2^-18 of
+// its terms (a few values in a million), again in 64 with the saved 64-bit statistics.  x - mean is taken as (x - mh) - ml with
+// mean = mh + ml, so a large common offset costs no accuracy.
 //
 // What bounds it: bytes, and for small maps the launches.  Two launches each way: sums of a chunk per workgroup -> partials; then
 // every workgroup joins the partials of the groups it touches (always in the same order: bit-reproducible, no atomics) and writes
@@ -90,9 +92,19 @@ __device__ __forceinline__ double2 gn_join(const double2* __restrict__ p, int pi
 struct GnStat {
   double mean, rstd;
 };
-__device__ __forceinline__ GnStat gn_stat(double2 s, double M, double eps) {
-  const double mean = s.x / M, var = s.y / M - mean * mean;
-  return {mean, 1. / sqrt((var > 0. || var != var ? var : 0.) + eps)};
+// (s: of the differences from the pivot)
+__device__ __forceinline__ GnStat gn_stat(double2 s, double pivot, double M, double eps) {
+  const double d = s.x / M, var = s.y / M - d * d;
+  return {pivot + d, 1. / sqrt((var > 0. || var != var ? var : 0.) + eps)};
+}
+// the pivot of group g of sample n
+template <typename T>
+__device__ __forceinline__ double gn_pivot_cl(const GnArgs& a, int n, int g) {
+  return (double)(float)static_cast<const T*>(a.x)[(long)n * a.S * a.C + g * a.cg];
+}
+template <typename T>
+__device__ __forceinline__ double gn_pivot_pl(const GnArgs& a, int n, int g) {
+  return (double)(float)static_cast<const T*>(a.x)[((long)n * a.C + g * a.cg) * a.S];
 }
 
 // z > 0 as the exact z has it (see above)
@@ -227,7 +239,11 @@ __global__ void __launch_bounds__(kGnThreads) gn_cl_stats_kernel(GnArgs a) {
   const GnCl t = gn_cl<V>(a, blockIdx.x);
   if (t.on) {
     constexpr int A = E == 1 ? 1 : V;                // accumulators
-    double s[V] = {}, q[V] = {};
+    double s[V] = {}, q[V] = {}, pv[V];
+    int gs[V];
+    gn_group_of<V>(t.c, a.cg, gs);
+#pragma unroll
+    for (int j = 0; j < A; ++j) pv[j] = gn_pivot_cl<T>(a, t.n, gs[j]);
     const T* p = static_cast<const T*>(a.x) + (long)t.n * a.S * a.C + t.c;
     constexpr int U = 4;
     for (long r = t.begin + t.r0; r < t.end; r += U * t.rpi) {
@@ -239,7 +255,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_cl_stats_kernel(GnArgs a) {
         if (r + u * t.rpi >= t.end) break;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const double f = (double)(float)v[u].v[j];
+          const double f = (double)(float)v[u].v[j] - pv[A == 1 ? 0 : j];
           s[A == 1 ? 0 : j] += f, q[A == 1 ? 0 : j] += f * f;
         }
       }
@@ -281,7 +297,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_cl_apply_kernel(GnArgs a) {
   const int g0 = t.c0 / a.cg, g1 = (t.c0 + t.nch - 1) / a.cg;
   for (int g = g0 + (threadIdx.x >> 6); g <= g1; g += kGnWaves) {
     const long i = (long)t.n * a.G + g;
-    const GnStat s = gn_stat(gn_join(a.part + i * a.pieces, a.pieces), (double)a.M, a.eps);
+    const GnStat s = gn_stat(gn_join(a.part + i * a.pieces, a.pieces), gn_pivot_cl<T>(a, t.n, g), (double)a.M, a.eps);
     if ((threadIdx.x & 63) == 0) {
       st[g - g0] = s;
       if (t.k == 0) a.mean[i] = s.mean, a.rstd[i] = s.rstd;     // (slabs that share a group write the same value)
@@ -329,16 +345,20 @@ __global__ void __launch_bounds__(TH) gn_cl_whole_kernel(GnArgs a) {
   const long off = (long)t.n * a.S * a.C + t.c;
   const T* p = static_cast<const T*>(a.x) + off;
   GnVec<T, V> v[R];
-  double s[V] = {}, q[V] = {};
+  double s[V] = {}, q[V] = {}, pv[V];
+  int gs[V];
   if (t.on) {
+    gn_group_of<V>(t.c, a.cg, gs);
 #pragma unroll
     for (int u = 0; u < R; ++u) v[u] = gn_load<T, V>(p + min((long)t.r0 + u * t.rpi, a.S - 1) * a.C);
+#pragma unroll
+    for (int j = 0; j < (E == 1 ? 1 : V); ++j) pv[j] = gn_pivot_cl<T>(a, t.n, gs[j]);
 #pragma unroll
     for (int u = 0; u < R; ++u) {
       if (t.r0 + u * t.rpi >= a.S) break;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const double f = (double)(float)v[u].v[j];
+        const double f = (double)(float)v[u].v[j] - pv[E == 1 ? 0 : j];
         s[E == 1 ? 0 : j] += f, q[E == 1 ? 0 : j] += f * f;
       }
     }
@@ -351,7 +371,7 @@ __global__ void __launch_bounds__(TH) gn_cl_whole_kernel(GnArgs a) {
     double2 sum = {0., 0.};
 #pragma unroll
     for (int i = 0; i < TH / 64; ++i) sum.x += sh[i].x, sum.y += sh[i].y;
-    const GnStat m = gn_stat(sum, (double)a.M, a.eps);
+    const GnStat m = gn_stat(sum, gn_pivot_cl<T>(a, t.n, g0), (double)a.M, a.eps);
     if (threadIdx.x == 0) st[0] = m, a.mean[(long)t.n * a.G + g0] = m.mean, a.rstd[(long)t.n * a.G + g0] = m.rstd;
   } else {
     if (t.on) {
@@ -360,7 +380,7 @@ __global__ void __launch_bounds__(TH) gn_cl_whole_kernel(GnArgs a) {
     }
     gn_cl_rows<TH>(t, t.wv * E, sh);
     gn_cl_groups<V, E, TH>(a, t, sh, [&](int g, double x, double y) {
-      const GnStat m = gn_stat({x, y}, (double)a.M, a.eps);
+      const GnStat m = gn_stat({x, y}, gn_pivot_cl<T>(a, t.n, g), (double)a.M, a.eps);
       st[g - g0] = m;
       a.mean[(long)t.n * a.G + g] = m.mean, a.rstd[(long)t.n * a.G + g] = m.rstd;
     });
@@ -368,8 +388,6 @@ __global__ void __launch_bounds__(TH) gn_cl_whole_kernel(GnArgs a) {
   __syncthreads();
   if (!t.on) return;
   float mh[V], ml[V], sc[V], b[V];
-  int gs[V];
-  gn_group_of<V>(t.c, a.cg, gs);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const GnStat m = st[gs[j] - g0];
@@ -581,6 +599,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_pl_stats_kernel(GnArgs a) {
   double s = 0., q = 0.;
   if (t.on) {
     const T* p = static_cast<const T*>(a.x) + t.plane * a.S;
+    const double pivot = gn_pivot_pl<T>(a, t.n, t.c / a.cg);
     constexpr int U = 4;
     long i = t.begin + t.t * V;
     for (; i + (U - 1) * TPU * V < t.end; i += U * TPU * V) {
@@ -591,7 +610,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_pl_stats_kernel(GnArgs a) {
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const double f = (double)(float)v[u].v[j];
+          const double f = (double)(float)v[u].v[j] - pivot;
           s += f, q += f * f;
         }
     }
@@ -599,7 +618,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_pl_stats_kernel(GnArgs a) {
       const GnVec<T, V> v = gn_load<T, V>(p + i);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const double f = (double)(float)v.v[j];
+        const double f = (double)(float)v.v[j] - pivot;
         s += f, q += f * f;
       }
     }
@@ -618,7 +637,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_pl_apply_kernel(GnArgs a) {
   if (!t.on) return;                                 // (workgroup-units: the whole workgroup)
   const int g = t.c / a.cg;
   const long ig = (long)t.n * a.G + g;
-  const GnStat s = gn_stat(gn_join(a.part + ig * a.pieces, a.pieces), (double)a.M, a.eps);
+  const GnStat s = gn_stat(gn_join(a.part + ig * a.pieces, a.pieces), gn_pivot_pl<T>(a, t.n, g), (double)a.M, a.eps);
   if (t.t == 0 && t.k == 0 && t.c == g * a.cg) a.mean[ig] = s.mean, a.rstd[ig] = s.rstd;
   const float mh = (float)s.mean, ml = (float)(s.mean - (double)mh);
   const float sc = (float)(s.rstd * (double)gn_param<T>(a.w, t.c, a.wdt, 1.f)), b = gn_param<T>(a.b, t.c, a.wdt, 0.f);
@@ -644,6 +663,7 @@ __global__ void __launch_bounds__(TH) gn_pl_whole_kernel(GnArgs a) {
   const T* p = static_cast<const T*>(a.x) + off;
   GnVec<T, V> v[R];
   double s = 0., q = 0.;
+  const double pivot = (double)(float)p[0];
 #pragma unroll
   for (int u = 0; u < R; ++u) v[u] = gn_load<T, V>(p + (long)min((int)threadIdx.x + u * TH, nv - 1) * V);
 #pragma unroll
@@ -651,7 +671,7 @@ __global__ void __launch_bounds__(TH) gn_pl_whole_kernel(GnArgs a) {
     if ((int)threadIdx.x + u * TH >= nv) break;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const double f = (double)(float)v[u].v[j];
+      const double f = (double)(float)v[u].v[j] - pivot;
       s += f, q += f * f;
     }
   }
@@ -661,7 +681,7 @@ __global__ void __launch_bounds__(TH) gn_pl_whole_kernel(GnArgs a) {
   s = q = 0.;
 #pragma unroll
   for (int i = 0; i < TH / 64; ++i) s += sh[i].x, q += sh[i].y;
-  const GnStat m = gn_stat({s, q}, (double)a.M, a.eps);
+  const GnStat m = gn_stat({s, q}, pivot, (double)a.M, a.eps);
   if (threadIdx.x == 0) a.mean[blockIdx.x] = m.mean, a.rstd[blockIdx.x] = m.rstd;
   const float mh = (float)m.mean, ml = (float)(m.mean - (double)mh);
   T* o = static_cast<T*>(a.out) + off;

@@ -153,6 +153,23 @@ def test_group_norm_of_a_large_common_offset():
 
 
 @gpu
+@pytest.mark.parametrize("layout", ["last", "planar"])
+def test_group_norm_of_offsets_that_fp32_only_just_holds(layout):
+    """mean / std = 5e6: sum x^2 / M - mean^2 in 64 bits would be off by 2^-52 (mean / std)^2 of the variance, half a percent.
+    Small maps (one launch), middle and large ones (two launches, with the joining one)."""
+    from boostmvsnerfs_amd import ops
+    for N, C, sp, G in ((2, 8, (9, 11), 2), (1, 6, (5, 7), 2), (2, 12, (5, 9), 4), (2, 8, (64, 65), 2), (1, 30, (90, 31), 5), (1, 19, (150, 100), 19), (1, 8, (300, 200), 1)):
+        x, dy, w, b = _make(N, C, sp, torch.float32, layout, seed=4, offset=0.0)
+        x = 3e5 + 0.05 * x
+        ref = x.double().reshape(N, G, -1) - 3e5                      # (exact)
+        _, mean, rstd = ops.group_norm_fwd(_place(x, layout), G, w.cuda(), b.cuda())
+        # 64-bit sums of d = x - pivot over M <= 480000 values lose at most M 2^-52 of the variance, half of that of rstd
+        _close(rstd, 1 / (ref.var(2, unbiased=False) + 1e-5).sqrt(), 1e-10 * rstd.double().cpu(), "rstd")
+        _close(mean - 3e5, ref.mean(2), 1e-9, "mean")               # (the mean itself is rounded by 2^-53 of 3e5)
+        _check(x, dy, G, w, b, 0.01, layout)
+
+
+@gpu
 def test_group_norm_constant_groups_and_zero_eps():
     x = torch.full((2, 4, 6, 5), 3.0)
     _, dy, w, b = _make(2, 4, (6, 5), torch.float32, "last")
