@@ -116,35 +116,43 @@ class MuonAdam(torch.optim.Optimizer):
     `matrices` / `others`: parameters, or param groups (the reference's one-group-per-parameter layout works for both).  A
     matrix has 2 dimensions or more (convolution kernels are flattened behind the first) and is fp32, bf16 or fp16, contiguous
     or not; its state is `momentum_buffer`, fp32.  Groups of matrices carry lr, momentum, nesterov, weight_decay (decoupled),
-    scale (ops.muon_step) and steps; schedulers see all groups.  Learning rates are plain numbers."""
+    scale (ops.muon_step) and steps; schedulers see all groups.  Learning rates are plain numbers.  Groups added later say which
+    they are (`muon`, True where it is not given)."""
 
     def __init__(self, matrices, others=(), lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, scale="shape", steps=5,
                  adam_lr=5e-4, adam_weight_decay=0.0, adam_eps=1e-8):
-        if scale not in ops.MUON_SCALES:
-            raise ValueError(f"scale: expected one of {sorted(ops.MUON_SCALES)}, got {scale!r}")
+        self._adam = GroupedAdam([{"params": []}], lr=adam_lr, weight_decay=adam_weight_decay, eps=adam_eps)
+        self._adam.param_groups.clear()
         super().__init__(list(matrices), dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, scale=scale,
                                               steps=steps, muon=True))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() < 2:
-                    raise ValueError(f"a matrix has at least 2 dimensions, got {tuple(p.shape)}")
         others = list(others)
-        self._adam = None
-        if others:
-            self._adam = GroupedAdam(others, lr=adam_lr, weight_decay=adam_weight_decay, eps=adam_eps)
-            for group in self._adam.param_groups:
-                group["muon"] = False
-            both = {id(p) for g in self.param_groups for p in g["params"]}
-            if any(id(p) in both for g in self._adam.param_groups for p in g["params"]):
-                raise ValueError("a parameter is listed among the matrices and among the others")
-            self.param_groups += self._adam.param_groups
+        for group in others if others and isinstance(others[0], dict) else [{"params": others}] if others else []:
+            self.add_param_group({**group, "muon": False})
+
+    def add_param_group(self, param_group):
+        """A group of matrices, or, with `muon` False, of parameters that step as GroupedAdam's with this optimiser's Adam defaults."""
+        if param_group.get("muon", True):
+            super().add_param_group(param_group)
+            group = self.param_groups[-1]
+            bad = next((p for p in group["params"] if p.dim() < 2), None)
+            if bad is None and group["scale"] in ops.MUON_SCALES:
+                return
+            self.param_groups.pop()
+            if bad is not None:
+                raise ValueError(f"a matrix has at least 2 dimensions, got {tuple(bad.shape)} (vectors: a group with muon=False)")
+            raise ValueError(f"scale: expected one of {sorted(ops.MUON_SCALES)}, got {group['scale']!r}")
         self._share()
+        self._adam.add_param_group(param_group)
+        group = self._adam.param_groups.pop()
+        both = {id(p) for g in self.param_groups if g["muon"] for p in g["params"]}
+        if any(id(p) in both for p in group["params"]):
+            raise ValueError("a parameter is listed among the matrices and among the others")
+        self.param_groups.append(group)
 
     def _share(self):
         """Adam works on this optimiser's own state and groups."""
-        if self._adam is not None:
-            self._adam.state = self.state
-            self._adam.param_groups = [g for g in self.param_groups if not g["muon"]]
+        self._adam.state = self.state
+        self._adam.param_groups = [g for g in self.param_groups if not g["muon"]]
 
     def load_state_dict(self, state_dict):
         if [g.get("muon") for g in state_dict["param_groups"]] != [g["muon"] for g in self.param_groups]:
@@ -156,7 +164,6 @@ class MuonAdam(torch.optim.Optimizer):
             saved = state_dict["state"].get(i, {}).get("momentum_buffer")
             if saved is not None:
                 self.state[p]["momentum_buffer"] = saved.detach().to(device=p.device, dtype=torch.float32, copy=True)
-        self._share()
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -164,7 +171,8 @@ class MuonAdam(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if self._adam is not None:
+        self._share()
+        if self._adam.param_groups:
             self._adam.step()
         buckets = {}
         for group in self.param_groups:

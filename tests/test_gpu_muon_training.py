@@ -89,6 +89,42 @@ def test_muon_adam_refusals():
         make_optimizer(net, optim="sgd")
 
 
+def test_groups_added_later_step_as_what_they_say_they_are(monkeypatch):
+    from boostmvsnerfs_amd import ops
+    from boostmvsnerfs_amd.train import GroupedAdam, MuonAdam
+    stepped = []
+    monkeypatch.setattr(ops, "muon_step", lambda params, *args: stepped.append((list(params), args[2])))
+    mats, rest = _mixed()
+    for others in ([], rest[:1]):                            # with and without an Adam group from the start
+        opt = MuonAdam(mats[:1], others, lr=0.1, adam_lr=1e-3, adam_eps=1e-6)
+        late, twin = torch.nn.Parameter(torch.randn(7)), None
+        twin = torch.nn.Parameter(late.detach().clone())
+        adam = GroupedAdam([twin], lr=1e-3, eps=1e-6)
+        opt.add_param_group({"params": late, "muon": False})
+        opt.add_param_group({"params": [mats[1]], "lr": 0.5})
+        for p in (*mats, *rest, late, twin):
+            p.grad = torch.full_like(p, 0.1)
+        for _ in range(2):
+            stepped.clear()
+            opt.step(), adam.step()
+            assert torch.equal(late, twin) and float(opt.state[late]["step"]) == float(adam.state[twin]["step"])
+            assert [(len(ps), lr) for ps, lr in stepped] == [(1, 0.1), (1, 0.5)]
+            assert stepped[0][0][0] is mats[0] and stepped[1][0][0] is mats[1]
+        assert set(opt.param_groups[-2]) == set(adam.param_groups[0]) | {"muon"}
+        n = len(opt.param_groups)
+        for bad, match in (({"params": [torch.nn.Parameter(torch.zeros(5))]}, "2 dimensions"),
+                           ({"params": [torch.nn.Parameter(torch.zeros(5, 5))], "scale": "x"}, "scale"),
+                           ({"params": [mats[0]], "muon": False}, "among the others"), ({"params": [late]}, "more than one parameter group"),
+                           ({"params": [late], "muon": False}, "more than one parameter group")):
+            with pytest.raises(ValueError, match=match):
+                opt.add_param_group(bad)
+            assert len(opt.param_groups) == n                # refused as a whole
+        saved = copy.deepcopy(opt.state_dict())
+        opt.load_state_dict(saved)
+        opt.step(), adam.step()
+        assert torch.equal(late, twin)
+
+
 def test_convert_group_norm():
     from boostmvsnerfs_amd.config import make_cfg, set_cfg
     from boostmvsnerfs_amd.networks.enerf.cnn import CostRegNet
