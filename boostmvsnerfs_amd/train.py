@@ -121,8 +121,8 @@ class MuonAdam(torch.optim.Optimizer):
 
     def __init__(self, matrices, others=(), lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, scale="shape", steps=5,
                  adam_lr=5e-4, adam_weight_decay=0.0, adam_eps=1e-8):
-        self._adam = GroupedAdam([{"params": []}], lr=adam_lr, weight_decay=adam_weight_decay, eps=adam_eps)
-        self._adam.param_groups.clear()
+        self._adam_defaults = dict(lr=adam_lr, weight_decay=adam_weight_decay, eps=adam_eps)
+        self._make_adam()
         super().__init__(list(matrices), dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, scale=scale,
                                               steps=steps, muon=True))
         others = list(others)
@@ -148,6 +148,19 @@ class MuonAdam(torch.optim.Optimizer):
         if any(id(p) in both for p in group["params"]):
             raise ValueError("a parameter is listed among the matrices and among the others")
         self.param_groups.append(group)
+
+    def _make_adam(self):
+        self._adam = GroupedAdam([{"params": []}], **self._adam_defaults)      # (_share gives it its groups)
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "_adam_defaults": self._adam_defaults}
+
+    def __setstate__(self, state):
+        """copy.deepcopy and pickle: the groups and the state come back, Adam's part is made again (load_state_dict comes here
+        with groups and state alone)."""
+        super().__setstate__(state)
+        if "_adam" not in self.__dict__:
+            self._make_adam()
 
     def _share(self):
         """Adam works on this optimiser's own state and groups."""

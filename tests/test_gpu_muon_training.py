@@ -125,6 +125,52 @@ def test_groups_added_later_step_as_what_they_say_they_are(monkeypatch):
         assert torch.equal(late, twin)
 
 
+@pytest.mark.parametrize("how", ["deepcopy", "pickle", "torch"])
+def test_muon_adam_survives_copies(how, monkeypatch):
+    import io
+    import pickle
+
+    from boostmvsnerfs_amd import ops
+    from boostmvsnerfs_amd.train import MuonAdam
+    lists = []
+    monkeypatch.setattr(ops, "muon_step", lambda *args: lists.append(args))
+    mats, rest = _mixed()
+    opt = MuonAdam(mats, rest, lr=0.1, adam_lr=1e-3, adam_eps=1e-6, adam_weight_decay=0.1)
+
+    def grads(o):
+        for g in o.param_groups:
+            for p in g["params"]:
+                p.grad = torch.full_like(p, 0.1)
+    grads(opt)
+    opt.step()
+    opt.state[mats[0]]["momentum_buffer"].fill_(0.5)
+    if how == "deepcopy":
+        twin = copy.deepcopy(opt)
+    elif how == "pickle":
+        twin = pickle.loads(pickle.dumps(opt))
+    else:
+        f = io.BytesIO()
+        torch.save(opt, f)
+        f.seek(0)
+        twin = torch.load(f, weights_only=False)             # (this test's own bytes)
+    mine, theirs = ([p for g in o.param_groups for p in g["params"]] for o in (opt, twin))
+    assert not {id(p) for p in mine} & {id(p) for p in theirs}
+    for o in (opt, twin):
+        o.add_param_group({"params": torch.nn.Parameter(torch.ones(3)), "muon": False})
+        grads(o)
+        lists.clear()
+        o.step()
+        (params, gs, momenta, *rest_args), = lists
+        assert [id(p) for p in params] == [id(p) for p in (mine if o is opt else theirs)[:2]] and rest_args[0] == 0.1
+        assert all(m is o.state[p]["momentum_buffer"] for p, m in zip(params, momenta)) and float(momenta[0][0, 0]) == 0.5
+    for g, h in zip(opt.param_groups, twin.param_groups):
+        assert {k: v for k, v in g.items() if k != "params"} == {k: v for k, v in h.items() if k != "params"}
+        for p, q in zip(g["params"], h["params"]):
+            assert torch.equal(p, q)                         # Adam's moved alike, from the copied state
+            assert set(opt.state[p]) == set(twin.state[q]) and all(torch.equal(opt.state[p][k], twin.state[q][k]) for k in opt.state[p])
+    assert not torch.equal(opt.param_groups[1]["params"][0], _mixed()[1][0])
+
+
 def test_convert_group_norm():
     from boostmvsnerfs_amd.config import make_cfg, set_cfg
     from boostmvsnerfs_amd.networks.enerf.cnn import CostRegNet
