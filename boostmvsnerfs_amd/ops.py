@@ -1634,6 +1634,64 @@ def newton_schulz(mats, steps=5, coeffs=NS_COEFFS, eps=NS_EPS):
     return out
 
 
+def _hits(coeffs, target, steps):
+    """Whether sum c v = target has a solution with lo <= v <= hi for (c, lo, hi) in `coeffs`, c > 0 falling; `steps`: a list of
+    how many values may still be tried (none left: it might have)."""
+    if not coeffs:
+        return target == 0
+    (c, lo, hi), rest = coeffs[0], coeffs[1:]
+    least, most = sum(k * v for k, v, _ in rest), sum(k * v for k, _, v in rest)
+    # the others make least ... most: c v has to be in target - most ... target - least
+    for v in range(max(lo, -((most - target) // c)), min(hi, (target - least) // c) + 1):
+        steps[0] -= 1
+        if steps[0] < 0 or _hits(rest, target - c * v, steps):
+            return True
+    return False
+
+
+def _written_twice(tensors):
+    """Whether two of the tensors share a byte, or one of them has two elements at one place.  Exact for strided tensors whose axes
+    nest, as slices and permutations of one tensor do; what would take long to tell is taken as shared."""
+    def axes(t):
+        return [(s * t.element_size(), n) for s, n in zip(t.stride(), t.shape) if n > 1] + [(1, t.element_size())]
+
+    spans = []
+    for i, t in enumerate(tensors):
+        reach = t.numel() * t.element_size() - 1
+        if torch._debug_has_internal_overlap(t) != 0:          # (0: dense, in any order of its axes)
+            reach = 0
+            for s, n in sorted(axes(t)):                       # an axis has to step over all that the finer ones reach
+                if s <= reach:
+                    return True
+                reach += s * (n - 1)
+        first = t.data_ptr()
+        spans.append((t.get_device(), first, first + reach, i))
+    spans.sort()
+    open_, end = [], (-2, 0)                                   # what may reach this far, and the furthest
+    for device, first, last, i in spans:
+        if (device, first) > end:
+            open_, end = [(first, last, i)], (device, last)
+            continue
+        t = tensors[i]
+        for start, far, k in open_:
+            if far < first:
+                continue
+            o = tensors[k]
+            # an address of both: o's start + o's axes = t's start + t's axes
+            ranges = {}
+            for s, n in axes(o):
+                lo, hi = ranges.get(s, (0, 0))
+                ranges[s] = lo, hi + n - 1
+            for s, n in axes(t):
+                lo, hi = ranges.get(s, (0, 0))
+                ranges[s] = lo - n + 1, hi
+            if _hits([(s, *ranges[s]) for s in sorted(ranges, reverse=True)], first - start, [100000]):
+                return True
+        open_.append((first, last, i))
+        end = max(end, (device, last))
+    return False
+
+
 MUON_SCALES = {
     "shape": lambda rows, cols: max(1.0, rows / cols) ** 0.5,      # an update of unit spectral norm per output
     "rms": lambda rows, cols: 0.2 * max(rows, cols) ** 0.5,        # an update of an Adam step's root mean square
@@ -1665,16 +1723,19 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
         if not (isinstance(m, torch.Tensor) and m.shape == p.shape and m.dtype == torch.float32 and m.get_device() == p.get_device()):
             _gpu_float(m, f"momenta[{i}]", p)
             raise ValueError(f"momenta[{i}]: expected {tuple(p.shape)} float32, got {tuple(m.shape)} {m.dtype}")
+    with torch.no_grad():
+        dense, written = [_c(t) for t in params], [_c(t) for t in momenta]
+    if any(a is not b for a, b in zip(dense, params)) or any(a is not b for a, b in zip(written, momenta)):
+        # (the library sees the copies, which do not overlap)
+        if _written_twice([t for _, idx in kinds for i in idx for t in (params[i], momenta[i])]):
+            raise RuntimeError("muon_step: a weight or a momentum overlaps another tensor (is one listed twice?) or itself")
     lib = _lib.load()
     for (_, dtype), idx in kinds:
         with torch.no_grad(), _on_device_of(params[idx[0]]):
             n = len(idx)
             rows, cols = _sides(sizes, idx)
             scales = (C.c_float * n)(*[lr * MUON_SCALES[scale](*sizes[i]) for i in idx])
-            p, m = [_c(params[i]) for i in idx], [_c(momenta[i]) for i in idx]
-            if any(a is not params[i] or b is not momenta[i] for a, b, i in zip(p, m, idx)):      # (copies do not overlap)
-                if len({t.data_ptr() for i in idx for t in (params[i], momenta[i])}) < 2 * n:
-                    raise RuntimeError("muon_step: a weight or a momentum overlaps another tensor (is one listed twice?)")
+            p, m = [dense[i] for i in idx], [written[i] for i in idx]
             ws = _ns_workspace(lib, n, rows, cols, dtype, p[0].device)
             with _region("muon_step"):
                 rc = lib.bmv_muon_step(n, _pointers(p), _pointers([_c(grads[i]) for i in idx]), _pointers(m), rows, cols, scales,

@@ -359,6 +359,78 @@ def test_overlaps_are_refused_by_the_entry_points():
     assert lib.bmv_newton_schulz(1, ptrs(A), ptrs(G), rows, cols, 7, 5, *COEFFS, 1e-7, C.c_void_p(W), 1 << 40, None) == -1
 
 
+def test_strided_tensors_that_share_elements_are_found():
+    """The host's check against marking every byte, for slices, permutations and windows of one storage."""
+    from boostmvsnerfs_amd.ops import _written_twice
+
+    def marked(tensors, size):
+        seen = torch.zeros(size, dtype=torch.int32)
+        base = tensors[0].untyped_storage().data_ptr()
+        for t in tensors:
+            at = torch.zeros(t.shape, dtype=torch.long) + (t.data_ptr() - base)
+            for d, (s, n) in enumerate(zip(t.stride(), t.shape)):
+                at = at + (torch.arange(n) * s * t.element_size()).view([-1 if k == d else 1 for k in range(t.dim())])
+            for b in range(t.element_size()):
+                seen.index_add_(0, at.flatten() + b, torch.ones(at.numel(), dtype=torch.int32))
+        return bool((seen > 1).any())
+    flat = torch.zeros(4096)
+    wide = flat[:960].view(8, 120)
+    half = flat.view(torch.bfloat16)
+    cube = flat[:1920].view(4, 8, 6, 10)
+    cases = [[wide[:, :40], wide[:, 40:]], [wide[:, :41], wide[:, 40:]], [wide[:, ::2], wide[:, 1::2]], [wide[:, ::2], wide[:, 1::3]],
+             [wide[::2], wide[1::2]], [wide[:4].t(), wide[4:].t()], [wide[:5].t(), wide[4:].t()], [wide.t(), wide[3:4, 7:9]],
+             [wide, flat[960:968].view(2, 4)], [wide, flat[959:967].view(2, 4)], [cube[:, :4], cube[:, 4:]],
+             [cube.permute(0, 2, 3, 1)[:2], cube.permute(3, 2, 1, 0)[..., 2:]], [cube.permute(0, 2, 3, 1)[:3], cube.permute(3, 2, 1, 0)[..., 2:]],
+             [cube[..., 0], cube[..., 9], cube[..., 4:6]], [cube[..., 0], cube[..., 5], cube[..., 4:6]],
+             [wide[:, :40], half[80:160].view(8, 10)], [wide[:, 40:80], half[:80].view(8, 10)], [wide[:, :40], half[81:160]],
+             [flat[:64].view(8, 8), flat[:64].view(8, 8).t()], [wide[:, 0:1], wide[:, 1:2]], [flat[:1].expand(4), wide[1:]], [flat[5:6].expand(2, 3)],
+             [flat.as_strided((4, 4), (2, 1))], [flat.as_strided((4, 4), (4, 1)), flat.as_strided((4, 4), (4, 1), 16)]]
+    found = [marked(c, 4 * 4096) for c in cases]
+    assert [_written_twice(c) for c in cases] == found and 8 < sum(found) < 20
+    g = torch.Generator().manual_seed(0)
+    hits = 0
+    for _ in range(300):                                     # two windows of one grid, at random
+        pair = []
+        for _ in range(2):
+            (a, b), (c, d) = (sorted(torch.randint(0, 13, (2,), generator=g).tolist()) for _ in range(2))
+            s, k = (int(torch.randint(1, 4, (1,), generator=g)) for _ in range(2))
+            v = flat[:156].view(12, 13)[a:b + 1:s, c:d + 1:k]
+            pair.append(v.t() if torch.randint(0, 2, (1,), generator=g) else v)
+        want = marked(pair, 4 * 4096)
+        hits += want
+        assert _written_twice(pair) == want, [(v.shape, v.stride(), v.storage_offset()) for v in pair]
+    assert 50 < hits < 250
+
+
+@gpu
+def test_muon_step_of_slices_of_one_tensor():
+    """Column slices of one weight step as weights of their own where they are disjoint, and are refused where they are not."""
+    from boostmvsnerfs_amd import ops
+    g = torch.Generator().manual_seed(5)
+    w, gr = torch.randn(12, 40, generator=g).cuda(), torch.randn(12, 40, generator=g).cuda()
+    cut = [(0, 15), (15, 40)]
+    want = [w[:, a:b].contiguous() for a, b in cut]
+    kept, m0 = w.clone(), [torch.zeros_like(v) for v in want]
+    ops.muon_step(want, [gr[:, a:b].contiguous() for a, b in cut], m0, 0.1)
+    for cols, bad in ((cut, False), ([(0, 16), (15, 40)], True), ([(0, 40), (15, 20)], True)):
+        w.copy_(kept)
+        parts, grads = [w[:, a:b] for a, b in cols], [gr[:, a:b] for a, b in cols]
+        momenta = [torch.zeros(v.shape, device="cuda") for v in parts]
+        if bad:
+            with pytest.raises(RuntimeError, match="overlaps"):
+                ops.muon_step(parts, grads, momenta, 0.1)
+            assert torch.equal(w, kept) and not any(m.any() for m in momenta)
+        else:
+            ops.muon_step(parts, grads, momenta, 0.1)
+            assert all(torch.equal(a, b) for a, b in zip(parts + momenta, want + m0))
+    # a weight that is one element many times, and a strided momentum over a dense weight
+    one = torch.zeros(1, 4, device="cuda").expand(3, 4)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ops.muon_step([one], [torch.ones(3, 4, device="cuda")], [torch.zeros(3, 4, device="cuda")], 0.1)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        ops.muon_step([w[:4]], [gr[:4]], [w.as_strided((4, 40), (80, 1))], 0.1)
+
+
 @gpu
 def test_refusals_on_the_gpu():
     from boostmvsnerfs_amd import ops
