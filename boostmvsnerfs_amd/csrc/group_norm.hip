@@ -570,7 +570,7 @@ template <int TPU>
 __device__ __forceinline__ GnPl gn_pl(const GnArgs& a, long bid) {
   GnPl p;
   const unsigned unit = (unsigned)bid * (kGnThreads / TPU) + (TPU == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
-  p.on = unit < (unsigned)a.N * a.C * a.chunks;           // (fewer than 2^32: gn_bad_shape)
+  p.on = unit < (unsigned)a.N * a.C * a.chunks;           // (at most max(N C, 8192) units: gn_plan, gn_bad)
   p.t = threadIdx.x & (TPU - 1);
   const unsigned plane = unit / a.chunks;
   p.k = (int)(unit - plane * a.chunks), p.plane = plane;
@@ -769,6 +769,7 @@ __global__ void __launch_bounds__(kGnThreads) gn_pl_bwd_apply_kernel(GnArgs a) {
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
+constexpr long kGnThreadsMost = (1l << 32) - 1;      // of a launch
 constexpr int kGnMaxJoin = 1024;      // double2 that a workgroup of the apply launch joins; above, one more launch does
 constexpr int kGnFew = 384;           // workgroups, fewer of which cost more than that launch (200416 x 19 fp16, 19 groups: 80 us with 53, 33)
 
@@ -860,6 +861,8 @@ static GnPlan gn_plan(int N, int C, long S, int G, int dtype, int last, bool bac
     p.finish = a.pieces > (p.tpu == 64 ? kGnMaxJoin / 4 : kGnMaxJoin);
     p.whole = gn_whole(a.M / p.V);
   }
+  if ((long)N * (p.last ? C / std::max(p.held, 1) : G) * p.whole > kGnThreadsMost) p.whole = 0;
+  a.dwb = (C + 7) / 8;
   p.part = (long)N * G * a.pieces, p.fin = p.finish ? (long)N * G : 0, p.partc = (long)N * C * a.npc;
   return p;
 }
@@ -916,7 +919,7 @@ static void gn_fwd_launch(const GnPlan& p, GnArgs a, bool silu, hipStream_t st) 
 template <int DT, int V, bool SILU>
 static void gn_bwd_launch(const GnPlan& p, GnArgs a, hipStream_t st) {
   const dim3 grid((unsigned)p.wgs), block(kGnThreads);
-  a.dwb = a.partc ? (a.C + 7) / 8 : 0;
+  if (!a.partc) a.dwb = 0;
   if (p.last) hipLaunchKernelGGL((gn_cl_bwd_reduce_kernel<DT, V, SILU>), grid, block, 0, st, a);
   else if (p.tpu == 256) hipLaunchKernelGGL((gn_pl_bwd_reduce_kernel<DT, V, 256, SILU>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((gn_pl_bwd_reduce_kernel<DT, V, 64, SILU>), grid, block, 0, st, a);
@@ -968,11 +971,14 @@ static const char* gn_bad(const bmv_group_norm_spec* s) {
   if (s->param_dtype != 0 && s->param_dtype != s->dtype) return "weight and bias are 32-bit or of the map's type";
   if (s->act != 0 && s->act != 1) return "unknown activation";
   if (!(s->eps >= 0.)) return "eps must not be negative";
-  if ((long)s->N * s->C > (1l << 24) || s->S > (1l << 40) / ((long)s->N * s->C)) return "the map is too large";
+  if ((long)s->N * s->C > (1l << 24) || s->S > (1l << 40) / ((long)s->N * s->C)) return "the map is too large (N C up to 2^24, N C S up to 2^40)";
   return nullptr;
 }
-static GnPlan gn_plan_of(const bmv_group_norm_spec* s, bool backward) {
-  return gn_plan(s->N, s->C, s->S, s->G, s->dtype, s->channels_last, backward);
+// the plan of a call, or why there is none
+static const char* gn_plan_of(const bmv_group_norm_spec* s, bool backward, GnPlan& p) {
+  if (const char* bad = gn_bad(s)) return bad;
+  p = gn_plan(s->N, s->C, s->S, s->G, s->dtype, s->channels_last, backward);
+  return (p.wgs + p.a.dwb) * kGnThreads > kGnThreadsMost ? "the map has too many workgroups for a launch" : nullptr;
 }
 
 }  // namespace bmv
@@ -982,19 +988,19 @@ using namespace bmv;
 extern "C" {
 
 long bmv_group_norm_workspace(const bmv_group_norm_spec* spec, int backward) {
-  const char* bad = gn_bad(spec);
+  GnPlan p;
+  const char* bad = gn_plan_of(spec, backward != 0, p);
   BMV_REQUIRE(!bad, "bmv_group_norm_workspace: %s", bad);
-  const GnPlan p = gn_plan_of(spec, backward != 0);
   return 2 * (p.part + p.fin + (backward ? p.partc : 0));
 }
 
 int bmv_group_norm_fwd(const bmv_group_norm_spec* spec, const void* x, const void* weight, const void* bias, double* stats,
                        double* workspace, void* y, bmv_stream_t stream) {
-  const char* bad = gn_bad(spec);
+  GnPlan p;
+  const char* bad = gn_plan_of(spec, false, p);
   BMV_REQUIRE(!bad, "bmv_group_norm_fwd: %s", bad);
   BMV_REQUIRE(x && stats && workspace && y, "bmv_group_norm_fwd: null pointer");
   BMV_REQUIRE(gn_aligned(x) && gn_aligned(y) && gn_aligned(workspace), "bmv_group_norm_fwd: x, y and workspace begin at 16-byte addresses");
-  const GnPlan p = gn_plan_of(spec, false);
   GnArgs a = p.a;
   a.x = x, a.w = weight, a.b = bias, a.out = y, a.wdt = spec->param_dtype, a.eps = spec->eps, a.slope = spec->slope;
   a.mean = stats, a.rstd = stats + (long)a.N * a.G;
@@ -1005,12 +1011,12 @@ int bmv_group_norm_fwd(const bmv_group_norm_spec* spec, const void* x, const voi
 
 int bmv_group_norm_bwd(const bmv_group_norm_spec* spec, const void* x, const void* dy, const void* weight, const void* bias,
                        const double* stats, double* workspace, void* dx, void* dweight, void* dbias, bmv_stream_t stream) {
-  const char* bad = gn_bad(spec);
+  GnPlan p;
+  const char* bad = gn_plan_of(spec, true, p);
   BMV_REQUIRE(!bad, "bmv_group_norm_bwd: %s", bad);
   BMV_REQUIRE(x && dy && stats && workspace && dx, "bmv_group_norm_bwd: null pointer");
   BMV_REQUIRE(gn_aligned(x) && gn_aligned(dy) && gn_aligned(dx) && gn_aligned(workspace),
               "bmv_group_norm_bwd: x, dy, dx and workspace begin at 16-byte addresses");
-  const GnPlan p = gn_plan_of(spec, true);
   GnArgs a = p.a;
   a.x = x, a.dy = dy, a.w = weight, a.b = bias, a.out = dx, a.dw = dweight, a.db = dbias, a.wdt = spec->param_dtype, a.slope = spec->slope;
   a.mean = const_cast<double*>(stats), a.rstd = a.mean + (long)a.N * a.G;

@@ -1527,7 +1527,7 @@ def group_norm_end(plan, x, dy, weight, bias, buf, want_params=True):
 def group_norm_fwd(x, groups, weight=None, bias=None, eps=1e-5, relu=False):
     """Group norm with an activation of x (N,C,*spatial), fp32 / bf16 / fp16, channel-last or planar (any other strides are
     copied to planar): y = act((x - mean) / sqrt(var + eps) * weight + bias), statistics over a sample's C / groups channels.
-    `relu`: False, True, a leaky slope, or "silu".  weight / bias (C): fp32 or x's type, or None.
+    `relu`: False, True, a leaky slope, or "silu".  weight / bias (C): fp32 or x's type, or None.  N C up to 2^24.
     -> y (x's layout and type), mean, rstd (N, groups; float64, what `group_norm_bwd` reads)."""
     y, plan, buf = group_norm_begin(x, groups, weight, bias, eps, relu)
     return (y, *buf[:plan.stats].view(2, x.shape[0], int(groups)).unbind())

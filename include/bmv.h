@@ -352,6 +352,7 @@ int bmv_bn_train_bwd(const float* x, const float* y, const float* dy, const floa
  * y = act((x - mean) rstd w + b) with the mean and (biased) variance of a sample's group of C / G channels, rstd =
  * 1 / sqrt(var + eps); act 0: v > 0 ? v : slope * v (1 none, 0 ReLU), act 1: v / (1 + exp(-v)) (slope ignored).
  * stats: mean (N, G), then rstd (N, G), 64-bit: the backward recomputes z and decides its sign with them.
+ * N C up to 2^24 and N C S up to 2^40, and fewer than 2^32 threads in a launch (C = 1: N up to 2^24 - 2); anything larger is refused.
  * workspace: bmv_group_norm_workspace(...) doubles (backward = 1 for the gradients' call), at a 16-byte address. */
 typedef struct {
   int N, C, G, dtype, param_dtype, channels_last, act;

@@ -368,6 +368,38 @@ def test_group_norm_refusals():
         ops.group_norm_fwd([1.0], 2)
 
 
+def test_group_norm_refuses_maps_whose_launches_would_be_too_large():
+    """The host's sizes, in front of any launch: 2^32 threads are one too many."""
+    import ctypes as C
+
+    from boostmvsnerfs_amd import _lib
+    lib = _lib.load()
+
+    def size(backward=0, **kw):
+        return lib.bmv_group_norm_workspace(C.byref(_lib.GroupNormSpec(**{"G": 1, "S": 1, "channels_last": 1, **kw})), backward)
+    for backward in (0, 1):
+        assert size(backward, N=1 << 23, C=1) > 0 and size(backward, N=1 << 14, C=1 << 10) > 0
+        assert size(backward, N=1 << 23, C=1, S=1 << 17, channels_last=0) > 0
+        assert size(backward, N=1 << 24, C=1) == -1 and b"too many workgroups" in lib.bmv_last_error()
+        assert size(backward, N=(1 << 24) - 1, C=1) == -1             # (with the workgroups of the parameters' gradients)
+        assert size(backward, N=1 << 14, C=(1 << 10) + 1) == -1 and b"too large" in lib.bmv_last_error()
+        assert size(backward, N=1 << 23, C=1, S=(1 << 17) + 1) == -1 and b"too large" in lib.bmv_last_error()
+
+
+@gpu
+def test_group_norm_of_very_many_groups_that_a_workgroup_would_hold():
+    """2^22 groups of 2049 values: held by 1024 threads each they would be 2^32 threads, so they take two launches."""
+    from boostmvsnerfs_amd import ops
+    x, dy, w, b = _make(512, 1, (2049,), torch.float16, "planar", seed=6)
+    ref = _formula(x, dy, 1, w, b, 1e-5, True)
+    many = x.cuda().repeat(1 << 13, 1, 1)
+    y, mean, rstd = ops.group_norm_fwd(many, 1, w.cuda(), b.cuda(), 1e-5, True)
+    _close(y[:512], ref["y"], 2.0 ** -11 * ref["y"].abs() + 6 * E32 * ref["mag_y"] + 2.0 ** -25, "y")
+    _close(rstd[:512], ref["rstd"], 1e-12 * ref["rstd"], "rstd")
+    for k in range(0, 1 << 22, 512 * 256):
+        assert all(torch.equal(v[k:k + 512 * 256].view(256, 512, -1), v[:512].view(1, 512, -1).expand(256, -1, -1)) for v in (y, mean, rstd)), k
+
+
 @gpu
 def test_group_norm_refusals_on_the_gpu():
     from boostmvsnerfs_amd import _lib, ops
