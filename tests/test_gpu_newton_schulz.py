@@ -150,6 +150,46 @@ def test_newton_schulz_large_matrices():
         _check(ops.newton_schulz(u.cuda()), u)
 
 
+def _through_tiles(mats, **kw):
+    from boostmvsnerfs_amd import _lib, ops
+    _lib.set_tuning("BMV_NS_SHORT", 0)
+    _lib.set_tuning("BMV_NS_BLOCK_K", 0)
+    try:
+        return ops.newton_schulz(mats, **kw)
+    finally:
+        _lib.set_tuning("BMV_NS_SHORT", None)
+        _lib.set_tuning("BMV_NS_BLOCK_K", None)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_newton_schulz_whole_tiles_and_cut_ones_in_one_launch(dtype):
+    """Lists of more than 512 tiles: 512 are a workgroup each, the rest is cut along k.  40 matrices of 15 symmetric tiles and 25
+    others (600 and 1000 a launch), tall and wide, on and off the tiles' borders; the matrices repeat, so that each is in whole
+    tiles and in cut ones."""
+    kinds = [_grad(m, n, seed).to(dtype) for seed, (m, n) in enumerate([(520, 600), (600, 520), (513, 640), (640, 577), (640, 640)])]
+    on_gpu = [v.cuda() for v in kinds]
+    refs = [_iterate(u) for u in kinds]
+    out = _through_tiles(on_gpu * 8)
+    again = _through_tiles(on_gpu * 8)
+    u_out = torch.finfo(dtype).eps / 2
+    for k, (got, twice) in enumerate(zip(out, again)):
+        want, tol = refs[k % 5]
+        small = 2.0 ** -25 * math.sqrt(want.numel()) if dtype == torch.float16 else 0.0
+        assert torch.equal(got, twice), k
+        assert float((got.double().cpu() - want).norm()) <= tol + u_out * float(want.norm()) + small, (k, tuple(want.shape))
+
+
+@gpu
+def test_newton_schulz_tiles_of_more_than_one_super_row():
+    """A short side of nine tiles: the second super-row of both enumerations, alone (all cut) and twelve times (540 symmetric
+    tiles and 972 others: whole and cut)."""
+    u = _grad(1100, 1030, 5)
+    want, tol = _iterate(u)
+    for got in _through_tiles([u.cuda()]) + _through_tiles([u.cuda()] * 12):
+        assert float((got.double().cpu() - want).norm()) <= tol + 2.0 ** -24 * float(want.norm())
+
+
 @gpu
 def test_newton_schulz_lists_that_fill_the_card():
     """bf16 symmetric products in blocks of 128 x 64, which are taken where the list keeps the compute units busy: panels of one
