@@ -16,11 +16,12 @@
 //
 // What bounds it: bytes, and for small maps the launches.  Two launches each way: sums of a chunk per workgroup -> partials; then
 // every workgroup joins the partials of the groups it touches (always in the same order: bit-reproducible, no atomics) and writes
-// its chunk, which it finds in its XCD's L2 or the last-level cache because the chunk -> workgroup map of both launches is the
-// same.  Where a workgroup holds all of a group in registers the forward is one launch.
-//   3 x 8 x 512 x 640 fp32 (31.5 MB), ReLU: forward 9.9 + 11.7 us (the second 5.4 TB/s), backward 16.5 + 17.0 (5.6 TB/s)
-//   4 x 320 x 64 x 64 bf16 (10.5 MB), SiLU: forward 18.5 us;  1 x 64 x 8 x 8 x 10 fp32: 5.6 us, one launch
-//   1 x 8 x 64 x 64 x 80 planar (10.5 MB), leaky: forward 10.5 us, backward 16
+// its chunk.  The forward's two launches have the same chunk -> workgroup map, so it finds the chunk in its XCD's L2; the
+// backward's second has the workgroups of dw and db in front (ceil(C / 8): another XCD where that is no multiple of 8) and finds it
+// in the last-level cache.  Where a workgroup holds all of a group in registers the forward is one launch.  Averages of 20 runs:
+//   3 x 8 x 512 x 640 fp32 (31.5 MB), ReLU: forward 10.9 + 11.8 us (the second 5.3 TB/s), backward 17.1 + 17.5 (5.4 TB/s)
+//   4 x 320 x 64 x 64 bf16 (10.5 MB), SiLU: forward 19.3 us, the pair among others;  1 x 64 x 8 x 8 x 10 fp32: 6.4 us, one launch
+//   1 x 8 x 64 x 64 x 80 planar (10.5 MB), leaky: forward 6.1 + 7.4 us, backward 7.7 + 8.2
 #include <algorithm>
 
 #include "bmv_common.hpp"
@@ -71,7 +72,7 @@ struct GnArgs {
   long per;                      // rows (values of a plane) of a chunk
   int pieces, npc;               // pieces a (sample, group) is joined from; pieces per channel of partc
   int slab_pieces;               // channel-last: slabs that share a group (1 where slabs hold whole groups)
-  int dwb;                       // backward: workgroups behind the map's that finish dw and db
+  int dwb;                       // backward: workgroups in front of the map's that finish dw and db
   float slope;
   double eps;
 };

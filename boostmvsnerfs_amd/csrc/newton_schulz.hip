@@ -8,7 +8,8 @@
 // Numbers.  A near-zero singular value grows by a = 3.4 a step, and with it whatever error X carried in its direction: the
 // products need more accuracy than the result's type has.  They run on the bf16 matrix cores with every fp32 operand as
 // three bf16 pieces (hi + mid + lo: its 24 significand bits exactly) and the six products that are not below 2^-25, sums in
-// fp32: 2.5 PFLOP/s / 6 against the 0.157 of the fp32 matrix instructions.  |U|_F is a 64-bit sum.
+// fp32: 2.5 PFLOP/s / 6 against the 0.157 of the fp32 matrix instructions.  |U|_F is a 64-bit sum; for short sides of up to 128
+// it is the root of the fp32 trace of U U^T, so a norm of more than 1.8e19 makes the result NaN there.
 //
 // All types: a bf16 or fp16 matrix' result is the fp32 result of the same values, rounded once.
 //
@@ -24,10 +25,10 @@
 // partial tiles the joining launch adds in a fixed order.  That launch also applies the polynomial, splits the values and writes
 // both orientations.  A product of the whole list is one launch: a workgroup finds its matrix in a table of the kernel arguments.
 //
-// What bounds it.  4096 x 4096 fp32: Q X takes 612 us, 1347 TFLOP/s of bf16 products -- a large product of the library reaches
-// 1247 on this card --, with the matrix pipe 66 % busy at the 1.9 GHz that its power leaves.  Joins are 10 ... 20 % on top
-// (4096 x 4096: 100 of 1365 us a step) and move their bytes at 4 ... 5 TB/s.  Below 1000 or so it is the chain: 15 launches, of
-// which 7.5 us each are start, first operands and end.
+// What bounds it.  4096 x 4096 fp32: Q X takes 612 ... 647 us by the card, 1275 ... 1347 TFLOP/s of bf16 products -- a large product
+// of the library reaches 1247 --, with the matrix pipe 66 % busy at the 1.9 GHz that its power leaves.  Joins are 7 ... 20 % on
+// top (4096 x 4096: 100 of 1365 ... 1410 us a step) and move their bytes at 4 ... 5 TB/s.  Below 1000 or so it is the chain: 15
+// launches, of which 7.5 us each are start, first operands and end.
 //
 // Matrices with a short side of up to 128 (every layer of the networks here) go another way, one launch a step: see below.
 #include <algorithm>

@@ -1612,7 +1612,8 @@ def newton_schulz(mats, steps=5, coeffs=NS_COEFFS, eps=NS_EPS):
     `coeffs` = (a, b, c) -- singular values towards 1, singular vectors kept.  `mats`: a tensor, or a list of tensors (one set
     of launches for all), of 2 dimensions or more (what is behind the first is flattened: convolution kernels), fp32, bf16 or
     fp16.  Computed at fp32 accuracy whatever the
-    type, rounded once.  -> new tensors of the same shapes and types."""
+    type, rounded once; a non-finite value makes its matrix NaN, and so does a norm above 1.8e19 where the short side is at most 128.
+    -> new tensors of the same shapes and types."""
     if torch.is_tensor(mats):
         return newton_schulz([mats], steps, coeffs, eps)[0]
     mats = list(mats)
